@@ -58,6 +58,9 @@ EXPORTED_SYMBOLS = (
     "ahr_graph_lca", "ahr_graph_lca_workspace", "ahr_graph_lca_large", "ahr_graph_info",
     "ahr_search_layout", "ahr_search_host", "ahr_graph_env_layout", "ahr_graph_env_step",
     "ahr_graph_env_step_host",
+    "ahr_attn_plan_build", "ahr_attn_forward", "ahr_attn_backward",
+    "ahr_rope_ws_bytes", "ahr_qk_norm_rope", "ahr_qk_norm_rope_backward",
+    "ahr_pool_plan_build", "ahr_pool_mean", "ahr_pool_mean_backward",
 )
 
 
@@ -74,6 +77,46 @@ class RerankParams(ctypes.Structure):
         ("layer_boost", ctypes.c_double * 4),
         ("type_mask", ctypes.c_int), ("member_top_m", ctypes.c_int), ("top_k", ctypes.c_int),
     ]
+
+
+class AttnShape(ctypes.Structure):
+    """struct ahr_attn_shape (include/ahr.h)."""
+    _fields_ = [("dtype", ctypes.c_int32), ("heads", ctypes.c_int32), ("kv_heads", ctypes.c_int32),
+                ("head_dim", ctypes.c_int32), ("causal", ctypes.c_int32), ("backward", ctypes.c_int32),
+                ("prefix", ctypes.c_int64)]
+
+
+class AttnPlan(ctypes.Structure):
+    """struct ahr_attn_plan (include/ahr.h)."""
+    _fields_ = [("shape", AttnShape), ("tokens", ctypes.c_int64), ("key_tokens", ctypes.c_int64),
+                ("ints", ctypes.c_int64), ("ws_bytes", ctypes.c_int64), ("part_rows", ctypes.c_int64),
+                ("n_rows", ctypes.c_int32), ("n_keys", ctypes.c_int32), ("n_join", ctypes.c_int32),
+                ("waves", ctypes.c_int32), ("planes", ctypes.c_int32), ("key_waves", ctypes.c_int32)]
+
+
+class Tensor3(ctypes.Structure):
+    """struct ahr_tensor3 (include/ahr.h)."""
+    _fields_ = [("p", ctypes.c_void_p), ("ts", ctypes.c_int64), ("hs", ctypes.c_int64)]
+
+
+class AttnArgs(ctypes.Structure):
+    """struct ahr_attn_args (include/ahr.h)."""
+    _fields_ = [("plan", ctypes.POINTER(AttnPlan)), ("lists", ctypes.c_void_p), ("scale", ctypes.c_float),
+                ("reserved", ctypes.c_int32), ("q", Tensor3), ("k", Tensor3), ("v", Tensor3), ("prefix_k", Tensor3),
+                ("prefix_v", Tensor3), ("o", Tensor3), ("lse", ctypes.c_void_p), ("d_o", Tensor3), ("dq", Tensor3),
+                ("dk", Tensor3), ("dv", Tensor3), ("ws", ctypes.c_void_p), ("ws_bytes", ctypes.c_int64)]
+
+
+class RopeArgs(ctypes.Structure):
+    """struct ahr_rope_args (include/ahr.h)."""
+    _fields_ = [("dtype", ctypes.c_int32), ("heads", ctypes.c_int32), ("kv_heads", ctypes.c_int32),
+                ("head_dim", ctypes.c_int32), ("rot", ctypes.c_int32), ("interleaved", ctypes.c_int32),
+                ("tokens", ctypes.c_int64), ("n_pos", ctypes.c_int64), ("eps", ctypes.c_float),
+                ("reserved", ctypes.c_int32), ("q", Tensor3), ("k", Tensor3), ("yq", Tensor3), ("yk", Tensor3),
+                ("dq", Tensor3), ("dk", Tensor3), ("wq", ctypes.c_void_p), ("wk", ctypes.c_void_p),
+                ("cos", ctypes.c_void_p), ("sin", ctypes.c_void_p), ("positions", ctypes.c_void_p),
+                ("dwq", ctypes.c_void_p), ("dwk", ctypes.c_void_p), ("ws", ctypes.c_void_p),
+                ("ws_bytes", ctypes.c_int64)]
 
 
 _lib: Optional[ctypes.CDLL] = None
@@ -130,6 +173,17 @@ def _declare(lib: ctypes.CDLL) -> None:
         "ahr_graph_env_step_host": ([_P, _I, _I, _I, _I, _I, _P, _L, _P, _P, _L, _P, _P], _I),
         "ahr_search_host": ([_P, _P, _P, _I, _I, _P, _L, ctypes.POINTER(RerankParams), _I, _P, _L, _P, _P], _I),
     }
+    sig.update({
+        "ahr_attn_plan_build": ([_P, _P, _I, ctypes.POINTER(AttnShape), ctypes.POINTER(AttnPlan), _P, _L], _I),
+        "ahr_attn_forward": ([ctypes.POINTER(AttnArgs), _P], _I),
+        "ahr_attn_backward": ([ctypes.POINTER(AttnArgs), _P], _I),
+        "ahr_rope_ws_bytes": ([_L, _I, _P], _I),
+        "ahr_qk_norm_rope": ([ctypes.POINTER(RopeArgs), _P], _I),
+        "ahr_qk_norm_rope_backward": ([ctypes.POINTER(RopeArgs), _P], _I),
+        "ahr_pool_plan_build": ([_P, _I, _P, _L, _P], _I),
+        "ahr_pool_mean": ([_I, _P, _L, _I, _P, _I, _I, _I, _P, _P, _P, _L, _P], _I),
+        "ahr_pool_mean_backward": ([_I, _P, _I, _P, _I, _I, _I, _P, _P, _P, _P], _I),
+    })
     for name, (args, res) in sig.items():
         if not hasattr(lib, name):  # reported by the export test, not here
             continue

@@ -1,0 +1,574 @@
+// Attention over packed sequences, forward (include/ahr.h ahr_attn_forward), and the host planner of
+// both directions.
+//
+// For a row (query token t, head h) with keys j: o = sum_j p_j v_j / sum_j p_j, p_j = 2^(c s_j - m),
+// s_j = q . k_j, c = scale log2(e). One pass over the keys with a running reference m: p and the
+// accumulators are relative to m, which is raised (and they are rescaled) only when a tile's maximum
+// exceeds it by more than 8, so p <= 2^8 and almost every tile skips the rescale.
+//
+// Layout. A workgroup takes 32 rows per wave; the rows of a tile are (token, head of the group), so
+// the query heads that share a key head read its keys once. Scores are computed transposed,
+// S^T = K Q^T (32x32x16 MFMA): a lane then holds one row's scores of 16 keys, the maximum and sum
+// stay within the lane and its other half, and S^T's registers are, converted to 16 bits, exactly the
+// second operand of O^T = V^T P^T when V^T is read with its keys in accumulator order (col_frag). Keys
+// and values go through LDS by DMA, double buffered, one barrier per 64 keys.
+#include "ahr_attn_common.h"
+
+#include <algorithm>
+#include <cmath>
+#include <cstring>
+#include <vector>
+
+namespace ahr {
+namespace attn {
+
+constexpr float kRaise = 8.f;  // how far (log2) a score may exceed the reference before it is raised
+
+template <typename T, int DP, int NW>
+__global__ __launch_bounds__(NW * 64, 2) void attn_fwd_kernel(Params p) {
+  typedef typename Elem<T>::v8 v8;
+  constexpr int NC = DP / 8, KS = DP / 16, DB = DP / 32;
+  constexpr int kTile = kKeys * DP * 2;
+  extern __shared__ __attribute__((aligned(16))) char smem[];  // [2][K tile, V tile]
+  const int lane = threadIdx.x & 63, h = lane >> 5, n = lane & 31;
+  const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  const int hk = blockIdx.x % p.kv_heads;
+  const RowItem it = p.rows[blockIdx.x / p.kv_heads];
+  const int dim = p.dim;
+
+  if (DP != dim) {  // the chunks past dim are never loaded
+    for (int i = threadIdx.x; i < 4 * kTile / 16; i += NW * 64) reinterpret_cast<f32x4*>(smem)[i] = f32x4{0, 0, 0, 0};
+    __syncthreads();
+  }
+
+  // this lane's row
+  const int n_rows = it.nq * p.group;
+  const int row = wave * 32 + n;
+  const bool live = row < n_rows;
+  const int tok = live ? (row * p.group_inv) >> 16 : 0;
+  const int head = hk * p.group + (live ? row - tok * p.group : 0);
+  const int lim = live ? (p.causal ? min(it.klen, it.koff + tok + 1) : it.klen) : 0;  // own keys it reads
+  const bool wave_live = wave * 32 < n_rows;
+
+  v8 qf[KS];
+  {
+    const char* qp = p.q + ((int64_t)(it.q0 + tok) * p.q_ts + (int64_t)head * p.q_hs) * 2;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      const int d = (2 * ks + h) * 8;
+      v8 z = {};
+      qf[ks] = (live && (DP == dim || d < dim)) ? *reinterpret_cast<const v8*>(qp + d * 2) : z;
+    }
+  }
+  // smallest and largest number of own keys that a row of this wave reads
+  int lim_lo, lim_hi;
+  {
+    const int first = (wave * 32 * p.group_inv) >> 16, last = ((min(wave * 32 + 32, n_rows) - 1) * p.group_inv) >> 16;
+    lim_lo = p.causal ? min(it.klen, it.koff + first + 1) : it.klen;
+    lim_hi = p.causal ? min(it.klen, it.koff + last + 1) : it.klen;
+  }
+
+  f32x16 acc[DB];
+#pragma unroll
+  for (int b = 0; b < DB; ++b)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) acc[b][r] = 0.f;
+  float m = -INFINITY, l = 0.f;  // reference (of c s) and this half-lane's part of the sum
+  const float c = p.scale_log2;
+
+  const Stager<NC, NW, kKeys> stager(wave, lane);
+  const int np = (it.pe - it.pb + kKeys - 1) / kKeys;
+  const int nt = np + (it.ke - it.kb + kKeys - 1) / kKeys;
+  auto stage = [&](int t, int buf) {
+    const bool pre = t < np;
+    const int kt = pre ? it.pb + t * kKeys : it.kb + (t - np) * kKeys;
+    const int have = min(kKeys, (pre ? it.pe : it.ke) - kt);
+    const int64_t kts = pre ? p.pk_ts : p.k_ts, vts = pre ? p.pv_ts : p.v_ts;
+    const char* kb = pre ? p.pk + ((int64_t)kt * kts + hk * p.pk_hs) * 2
+                         : p.k + ((int64_t)(it.k0 + kt) * kts + hk * p.k_hs) * 2;
+    const char* vb = pre ? p.pv + ((int64_t)kt * vts + hk * p.pv_hs) * 2
+                         : p.v + ((int64_t)(it.k0 + kt) * vts + hk * p.v_hs) * 2;
+    const int kst = (int)kts * 2, vst = (int)vts * 2;
+    const __amdgpu_buffer_rsrc_t kr = dense::tile_rsrc_u(kb, (uint32_t)((have - 1) * kst + dim * 2));
+    const __amdgpu_buffer_rsrc_t vr = dense::tile_rsrc_u(vb, (uint32_t)((have - 1) * vst + dim * 2));
+    char* tile = smem + buf * 2 * kTile;
+    stager.load(kr, tile, dim, [&](int r) { return min(r, have - 1) * kst; });
+    stager.load(vr, tile + kTile, dim, [&](int r) { return min(r, have - 1) * vst; });
+  };
+
+  if (nt > 0) stage(0, 0);
+  for (int t = 0; t < nt; ++t) {
+    __syncthreads();  // tile t has landed (vmcnt(0)), tile t - 1 is no longer read
+    if (t + 1 < nt) stage(t + 1, (t + 1) & 1);
+    const bool pre = t < np;
+    const int kt = pre ? it.pb + t * kKeys : it.kb + (t - np) * kKeys;
+    const int end = pre ? it.pe : min(it.ke, lim_hi);   // no row of the wave reads from here on
+    if (!wave_live || kt >= end) continue;
+    const char* kt_lds = smem + (t & 1) * 2 * kTile;
+    const char* vt_lds = kt_lds + kTile;
+
+    f32x16 s[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[u][r] = 0.f;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+      for (int u = 0; u < 2; ++u) s[u] = Elem<T>::mma(row_frag<T, NC>(kt_lds, u * 32 + n, ks, h), qf[ks], s[u]);
+
+    // keys that a row does not read: selected away, whatever their scores are
+    const int stop = pre ? it.pe : it.ke;
+    if (kt + kKeys > stop || (!pre && kt + kKeys > lim_lo)) {
+      const int mine = (pre ? it.pe : min(lim, it.ke)) - kt;
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[u][r] = u * 32 + acc_row(r, h) < mine ? s[u][r] : -INFINITY;
+    }
+
+    float top = s[0][0];
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) top = fmaxf(top, s[u][r]);
+    top = fmaxf(top, other_half(top)) * c;
+    if (__any(top > m + kRaise)) {  // (m = -inf before the first key)
+      const float to = fmaxf(m, top);
+      const float f = to == -INFINITY ? 1.f : ex2(m - to);
+      l *= f;
+#pragma unroll
+      for (int b = 0; b < DB; ++b)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[b][r] *= f;
+      m = to;
+    }
+    const float ref = m == -INFINITY ? 0.f : m;
+    float add = 0.f;
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        s[u][r] = ex2(fmaf(s[u][r], c, -ref));
+        add += s[u][r];
+      }
+    l += add;
+
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const v8 pf = acc_frag<T>(s[g >> 1], (g & 1) * 8);
+#pragma unroll
+      for (int b = 0; b < DB; ++b) acc[b] = Elem<T>::mma(col_frag<T, NC>(vt_lds, g * 16, b, lane), pf, acc[b]);
+    }
+  }
+
+  if (!live) return;
+  l += other_half(l);
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  const float lse = l == 0.f ? -INFINITY : m + __log2f(l);
+  if (it.plane >= 0) {
+    const int64_t at = ((int64_t)it.plane * p.prows + it.prow + tok) * p.heads + head;
+    if (h == 0) p.part_l[at] = lse;
+    float* op = p.part_o + at * dim;
+#pragma unroll
+    for (int b = 0; b < DB; ++b)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const int d = b * 32 + g * 8 + h * 4;
+        if (DP == dim || d < dim)
+          *reinterpret_cast<f32x4*>(op + d) = f32x4{acc[b][4 * g] * inv, acc[b][4 * g + 1] * inv,
+                                                    acc[b][4 * g + 2] * inv, acc[b][4 * g + 3] * inv};
+      }
+    return;
+  }
+  if (p.lse && h == 0) p.lse[(int64_t)(it.q0 + tok) * p.heads + head] = lse;
+  char* op = p.o + ((int64_t)(it.q0 + tok) * p.o_ts + (int64_t)head * p.o_hs) * 2;
+#pragma unroll
+  for (int b = 0; b < DB; ++b)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int d = b * 32 + g * 8 + h * 4;
+      if (DP == dim || d < dim)
+        store4<T>(op + d * 2, acc[b][4 * g] * inv, acc[b][4 * g + 1] * inv, acc[b][4 * g + 2] * inv,
+                  acc[b][4 * g + 3] * inv);
+    }
+}
+
+// Joins partial results: o = sum_i 2^(lse_i - max) o_i / sum_i 2^(lse_i - max). One wave per row;
+// each plane is read once.
+template <typename T>
+__global__ __launch_bounds__(256) void attn_join_kernel(Params p) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const JoinItem it = p.join[blockIdx.x / p.heads];
+  const int head = blockIdx.x % p.heads;
+  const int64_t plane = p.prows * p.heads;
+  for (int i = wave; i < it.nq; i += 4) {
+    const int64_t at = (int64_t)(it.prow + i) * p.heads + head;
+    float top = -INFINITY;
+    for (int j = lane; j < it.np; j += 64) top = fmaxf(top, p.part_l[at + j * plane]);
+#pragma unroll
+    for (int x = 1; x < 64; x *= 2) top = fmaxf(top, __shfl_xor(top, x, 64));
+    const float ref = top == -INFINITY ? 0.f : top;
+    float sum = 0.f, a = 0.f, b = 0.f;
+    const bool have = lane * 2 < p.dim;
+    for (int j = 0; j < it.np; ++j) {
+      const float w = ex2(p.part_l[at + j * plane] - ref);
+      sum += w;
+      if (have) {
+        const float2 x = *reinterpret_cast<const float2*>(p.part_o + (at + j * plane) * p.dim + lane * 2);
+        a = fmaf(w, x.x, a);
+        b = fmaf(w, x.y, b);
+      }
+    }
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    if (p.lse && lane == 0) p.lse[(int64_t)(it.q0 + i) * p.heads + head] = sum == 0.f ? -INFINITY : ref + __log2f(sum);
+    if (have) {
+      T* o = reinterpret_cast<T*>(p.o) + (int64_t)(it.q0 + i) * p.o_ts + (int64_t)head * p.o_hs + lane * 2;
+      o[0] = (T)(a * inv);
+      o[1] = (T)(b * inv);
+    }
+  }
+}
+
+// ---- host: plans ---------------------------------------------------------------------------
+
+static int64_t up(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+struct Lists {
+  std::vector<RowItem> rows;
+  std::vector<KeyItem> keys;
+  std::vector<JoinItem> join;
+  int waves = 4, key_waves = 4, planes = 0;
+  int64_t prows = 0;
+};
+
+struct Seq {
+  int64_t q0, k0;
+  int qlen, klen;
+};
+
+// own keys that tokens [t, t + n) of a sequence may read
+static int keys_of(const Seq& s, bool causal, int t, int n) {
+  if (!causal) return s.klen;
+  return (int)std::max<int64_t>(0, std::min<int64_t>(s.klen, (int64_t)s.klen - s.qlen + t + n));
+}
+
+// Forward lists. A tile takes `rows` rows; where there are fewer workgroups than fill the chip the key
+// ranges are cut and joined.
+static void plan_rows(const std::vector<Seq>& seqs, const ahr_attn_shape& sh, int64_t prefix, bool may_split, Lists& L) {
+  const int G = sh.heads / sh.kv_heads;
+  int64_t total = 0;
+  for (const Seq& s : seqs) total += s.qlen;
+  auto tiles_at = [&](int rows) {  // row tiles when a tile holds whole tokens of one sequence
+    const int per = std::max(1, rows / G);
+    int64_t n = 0;
+    for (const Seq& s : seqs) n += up(s.qlen, per);
+    return n;
+  };
+  int waves = 4;
+  const int least = (G + 31) / 32 <= 1 ? 1 : ((G + 31) / 32 <= 2 ? 2 : 4);
+  while (waves > least && (tiles_at(waves * 32) * sh.kv_heads < 512 ||
+                           tiles_at(waves * 32) * waves > tiles_at(least * 32) * least * 5 / 4))
+    waves /= 2;
+  L.waves = waves;
+  const int per = std::max(1, waves * 32 / G);  // tokens of a tile
+
+  // the shared prefix: read within each sequence's tiles, or by tiles over all tokens and joined
+  const int64_t ptiles = up(prefix, kKeys);
+  bool apart = false;
+  if (prefix > 0) {
+    const int64_t within = tiles_at(waves * 32), across = up(total, per);
+    apart = may_split && (across * 5 < within * 4 || within * sh.kv_heads < 512);
+  }
+  struct Part { size_t item; int pieces; };
+  std::vector<RowItem> base;
+  std::vector<int> load;
+  for (const Seq& s : seqs)
+    for (int t = 0; t < s.qlen; t += per) {
+      RowItem r;
+      memset(&r, 0, sizeof r);
+      r.q0 = (int32_t)(s.q0 + t);
+      r.nq = std::min(per, s.qlen - t);
+      r.k0 = (int32_t)s.k0;
+      r.klen = s.klen;
+      r.koff = s.klen - s.qlen + t;
+      r.ke = keys_of(s, sh.causal, t, r.nq);
+      r.pe = apart ? 0 : (int32_t)prefix;
+      r.plane = -1;
+      base.push_back(r);
+      load.push_back((int)(up(r.ke, kKeys) + (apart ? 0 : ptiles)));
+    }
+  const int64_t prow_all = apart ? total : 0;
+  int64_t work = 0;
+  for (int x : load) work += x;
+  const int64_t ptl = apart ? up(total, per) : 0;  // prefix row tiles
+  work += ptl * ptiles;
+  const int64_t blocks = ((int64_t)base.size() + ptl) * sh.kv_heads;
+  // pieces of about `chunk` key tiles, at least four (256 keys), so that about 1024 workgroups run
+  int64_t chunk = INT32_MAX;
+  if (may_split && (blocks < 512 || apart)) chunk = std::max<int64_t>(4, up(work * sh.kv_heads, 1024));
+
+  int prefix_pieces = 0;
+  if (apart) {
+    prefix_pieces = (int)std::max<int64_t>(1, up(ptiles, chunk));
+    const int64_t step = up(ptiles, prefix_pieces) * kKeys;
+    prefix_pieces = (int)up(prefix, step);
+    for (int64_t t = 0; t < total; t += per)
+      for (int i = 0; i < prefix_pieces; ++i) {
+        RowItem r;
+        memset(&r, 0, sizeof r);
+        r.q0 = (int32_t)t;
+        r.nq = (int32_t)std::min<int64_t>(per, total - t);
+        r.pb = (int32_t)(i * step);
+        r.pe = (int32_t)std::min<int64_t>(prefix, (i + 1) * step);
+        r.plane = i;
+        r.prow = (int32_t)t;
+        L.rows.push_back(r);
+      }
+    L.planes = prefix_pieces;
+    L.prows = prow_all;
+  }
+  for (size_t b = 0; b < base.size(); ++b) {
+    RowItem r = base[b];
+    int pieces = load[b] > chunk + chunk / 2 ? (int)up(load[b], chunk) : 1;
+    if (pieces == 1 && !apart) {
+      L.rows.push_back(r);
+      continue;
+    }
+    // the key tiles of the item, prefix first, dealt to its pieces
+    const int64_t own0 = apart ? 0 : ptiles;
+    const int64_t step = up(load[b], pieces);
+    const int64_t prow = apart ? r.q0 : L.prows;
+    int made = prefix_pieces;
+    if (load[b] > 0)
+      for (int64_t t = 0; t < load[b]; t += step) {
+        RowItem x = r;
+        const int64_t e = std::min<int64_t>(load[b], t + step);
+        x.pb = (int32_t)std::min<int64_t>(r.pe, t * kKeys);
+        x.pe = (int32_t)std::min<int64_t>(r.pe, e * kKeys);
+        x.kb = (int32_t)std::min<int64_t>(r.ke, std::max<int64_t>(0, t - own0) * kKeys);
+        x.ke = (int32_t)std::min<int64_t>(r.ke, std::max<int64_t>(0, e - own0) * kKeys);
+        x.plane = made++;
+        x.prow = (int32_t)prow;
+        L.rows.push_back(x);
+      }
+    L.planes = std::max(L.planes, made);
+    if (!apart) L.prows += r.nq;
+    L.join.push_back(JoinItem{r.q0, r.nq, (int32_t)prow, made});
+  }
+  std::stable_sort(L.rows.begin(), L.rows.end(), [](const RowItem& a, const RowItem& b) {
+    return (a.pe - a.pb) + (a.ke - a.kb) > (b.pe - b.pb) + (b.ke - b.kb);  // longest first
+  });
+}
+
+static void plan_keys(const std::vector<Seq>& seqs, const ahr_attn_shape& sh, Lists& L) {
+  auto tiles_at = [&](int keys) {
+    int64_t n = 0;
+    for (const Seq& s : seqs) n += up(s.klen, keys);
+    return n;
+  };
+  int waves = 4;
+  while (waves > 1 && (tiles_at(waves * 32) * sh.kv_heads < 512 || tiles_at(waves * 32) * waves > tiles_at(32) * 5 / 4))
+    waves /= 2;
+  L.key_waves = waves;
+  const int per = waves * 32;
+  for (const Seq& s : seqs)
+    for (int j = 0; j < s.klen; j += per) {
+      KeyItem k;
+      memset(&k, 0, sizeof k);
+      k.k0 = (int32_t)(s.k0 + j);
+      k.nk = std::min(per, s.klen - j);
+      k.kpos = j;
+      k.klen = s.klen;
+      k.q0 = (int32_t)s.q0;
+      k.qlen = s.qlen;
+      k.t0 = sh.causal ? (int32_t)std::min<int64_t>(s.qlen, std::max<int64_t>(0, (int64_t)j - (s.klen - s.qlen))) : 0;
+      L.keys.push_back(k);
+    }
+  std::stable_sort(L.keys.begin(), L.keys.end(),
+                   [](const KeyItem& a, const KeyItem& b) { return a.qlen - a.t0 > b.qlen - b.t0; });
+}
+
+static int check_shape(const ahr_attn_shape& sh) {
+  if (sh.dtype != AHR_F16 && sh.dtype != AHR_BF16) return fail(AHR_EUNSUP, "attention takes f16 and bf16");
+  if (sh.heads < 1 || sh.kv_heads < 1 || sh.heads % sh.kv_heads) return fail(AHR_EINVAL, "heads must be a positive multiple of kv_heads");
+  if (sh.heads / sh.kv_heads > kMaxGroup) return fail(AHR_EUNSUP, "more than 128 query heads share a key head");
+  if (sh.head_dim < 8 || sh.head_dim % 8 || sh.head_dim > kMaxDim) return fail(AHR_EUNSUP, "head_dim must be a multiple of 8, at most 128");
+  if (sh.prefix < 0 || sh.prefix > INT32_MAX - kKeys) return fail(AHR_EINVAL, "prefix out of range");
+  if (sh.backward && sh.prefix) return fail(AHR_EUNSUP, "a shared prefix has no backward pass");
+  if ((sh.causal | sh.backward) & ~1) return fail(AHR_EINVAL, "causal and backward are 0 or 1");
+  return AHR_OK;
+}
+
+static int build(const int32_t* q_len, const int32_t* k_len, int n, const ahr_attn_shape& sh, ahr_attn_plan* plan,
+                 int32_t* buf, int64_t cap) {
+  std::vector<Seq> seqs((size_t)n);
+  int64_t t = 0, tk = 0;
+  for (int i = 0; i < n; ++i) {
+    const int a = q_len[i], b = k_len ? k_len[i] : a;
+    if (a < 0 || b < 0) return fail(AHR_EINVAL, "negative length");
+    seqs[i] = Seq{t, tk, a, b};
+    t += a;
+    tk += b;
+  }
+  if (t > INT32_MAX / 2 || tk > INT32_MAX / 2) return fail(AHR_EINVAL, "more than 2^30 packed tokens");
+  Lists L;
+  plan_rows(seqs, sh, sh.backward ? 0 : sh.prefix, !sh.backward, L);
+  if (sh.backward) plan_keys(seqs, sh, L);
+  const int64_t blocks = (int64_t)std::max(std::max(L.rows.size(), L.keys.size()) * (size_t)sh.kv_heads, L.join.size() * (size_t)sh.heads);
+  if (blocks > INT32_MAX / 2) return fail(AHR_EINVAL, "too many work items");
+  memset(plan, 0, sizeof *plan);
+  plan->shape = sh;
+  plan->tokens = t;
+  plan->key_tokens = tk;
+  plan->n_rows = (int32_t)L.rows.size();
+  plan->n_keys = (int32_t)L.keys.size();
+  plan->n_join = (int32_t)L.join.size();
+  plan->waves = L.waves;
+  plan->key_waves = L.key_waves;
+  plan->planes = L.planes;
+  plan->part_rows = L.prows;
+  plan->ints = (int64_t)(L.rows.size() * sizeof(RowItem) + L.keys.size() * sizeof(KeyItem) + L.join.size() * sizeof(JoinItem)) / 4;
+  plan->ws_bytes = sh.backward ? t * sh.heads * 4 : (int64_t)L.planes * L.prows * sh.heads * (sh.head_dim + 1) * 4;
+  if (!buf) return AHR_OK;
+  if (cap < plan->ints) return fail(AHR_EINVAL, "buffer smaller than the plan's lists");
+  char* b = reinterpret_cast<char*>(buf);
+  memcpy(b, L.rows.data(), L.rows.size() * sizeof(RowItem));
+  b += L.rows.size() * sizeof(RowItem);
+  memcpy(b, L.keys.data(), L.keys.size() * sizeof(KeyItem));
+  b += L.keys.size() * sizeof(KeyItem);
+  memcpy(b, L.join.data(), L.join.size() * sizeof(JoinItem));
+  return AHR_OK;
+}
+
+// ---- host: argument checks and launches ------------------------------------------------------
+
+static int check_tensor(const ahr_tensor3& t, int64_t rows, int heads, int dim, const char* name) {
+  if (rows == 0) return AHR_OK;
+  if (!t.p) return fail(AHR_EINVAL, std::string(name) + ": null tensor");
+  if (reinterpret_cast<uintptr_t>(t.p) % 16 || t.ts % 8 || t.hs % 8) return fail(AHR_EINVAL, std::string(name) + ": rows must start at multiples of 16 bytes");
+  // 32-bit offsets within a staged tile: 64 tokens and all heads
+  if (t.ts < 0 || t.hs < 0 || t.ts > (1 << 23) || t.hs > ((int64_t)1 << 29) / heads) return fail(AHR_EUNSUP, std::string(name) + ": stride too large");
+  (void)dim;
+  return AHR_OK;
+}
+
+static int fill(const ahr_attn_args* a, bool backward, Params* out) {
+  if (!a || !a->plan) return fail(AHR_EINVAL, "null arguments");
+  const ahr_attn_plan& pl = *a->plan;
+  const ahr_attn_shape& sh = pl.shape;
+  int st = check_shape(sh);
+  if (st != AHR_OK) return st;
+  if ((sh.backward != 0) != backward) return fail(AHR_EINVAL, backward ? "not a backward plan" : "not a forward plan");
+  if (!(a->scale > 0.f) || !std::isfinite(a->scale)) return fail(AHR_EINVAL, "scale must be positive and finite");
+  if (pl.ints > 0 && !a->lists) return fail(AHR_EINVAL, "null plan lists");
+  if (pl.ws_bytes > 0 && (!a->ws || a->ws_bytes < pl.ws_bytes || reinterpret_cast<uintptr_t>(a->ws) % 16)) return fail(AHR_EINVAL, "workspace smaller than the plan's ws_bytes, or not aligned");
+  const struct { const ahr_tensor3* t; int64_t rows; int heads; const char* name; bool on; } all[] = {
+      {&a->q, pl.tokens, sh.heads, "q", true},           {&a->k, pl.key_tokens, sh.kv_heads, "k", true},
+      {&a->v, pl.key_tokens, sh.kv_heads, "v", true},    {&a->prefix_k, sh.prefix, sh.kv_heads, "prefix_k", !backward},
+      {&a->prefix_v, sh.prefix, sh.kv_heads, "prefix_v", !backward}, {&a->o, pl.tokens, sh.heads, "o", true},
+      {&a->d_o, pl.tokens, sh.heads, "d_o", backward},   {&a->dq, pl.tokens, sh.heads, "dq", backward},
+      {&a->dk, pl.key_tokens, sh.kv_heads, "dk", backward}, {&a->dv, pl.key_tokens, sh.kv_heads, "dv", backward}};
+  for (const auto& x : all)
+    if (x.on && (st = check_tensor(*x.t, x.rows, x.heads, sh.head_dim, x.name)) != AHR_OK) return st;
+  if (backward && pl.tokens > 0 && !a->lse) return fail(AHR_EINVAL, "null lse");
+  Params p;
+  memset(&p, 0, sizeof p);
+  p.q = (const char*)a->q.p, p.q_ts = a->q.ts, p.q_hs = a->q.hs;
+  p.k = (const char*)a->k.p, p.k_ts = a->k.ts, p.k_hs = a->k.hs;
+  p.v = (const char*)a->v.p, p.v_ts = a->v.ts, p.v_hs = a->v.hs;
+  p.pk = (const char*)a->prefix_k.p, p.pk_ts = a->prefix_k.ts, p.pk_hs = a->prefix_k.hs;
+  p.pv = (const char*)a->prefix_v.p, p.pv_ts = a->prefix_v.ts, p.pv_hs = a->prefix_v.hs;
+  p.o = (char*)a->o.p, p.o_ts = a->o.ts, p.o_hs = a->o.hs;
+  p.d_o = (const char*)a->d_o.p, p.do_ts = a->d_o.ts, p.do_hs = a->d_o.hs;
+  p.dq = (char*)a->dq.p, p.dq_ts = a->dq.ts, p.dq_hs = a->dq.hs;
+  p.dk = (char*)a->dk.p, p.dk_ts = a->dk.ts, p.dk_hs = a->dk.hs;
+  p.dv = (char*)a->dv.p, p.dv_ts = a->dv.ts, p.dv_hs = a->dv.hs;
+  p.lse = a->lse;
+  if (backward) {
+    p.delta = (float*)a->ws;
+  } else {
+    p.part_o = (float*)a->ws;  // [planes][prows][heads][dim], then the lse of each
+    p.part_l = (float*)a->ws + (int64_t)pl.planes * pl.part_rows * sh.heads * sh.head_dim;
+  }
+  p.prows = pl.part_rows;
+  p.n_rows = pl.n_rows, p.n_keys = pl.n_keys, p.n_join = pl.n_join;
+  p.rows = reinterpret_cast<const RowItem*>(a->lists);
+  p.keys = reinterpret_cast<const KeyItem*>(p.rows + pl.n_rows);
+  p.join = reinterpret_cast<const JoinItem*>(p.keys + pl.n_keys);
+  p.heads = sh.heads, p.kv_heads = sh.kv_heads, p.group = sh.heads / sh.kv_heads;
+  p.group_inv = (65536 + p.group - 1) / p.group;  // x / group = x * group_inv >> 16 for x < 512
+  p.dim = sh.head_dim, p.causal = sh.causal;
+  p.scale = a->scale;
+  p.scale_log2 = (float)((double)a->scale * 1.4426950408889634);
+  *out = p;
+  return AHR_OK;
+}
+
+template <typename T, int DP, int NW>
+static int launch_fwd(const Params& p, hipStream_t s) {
+  constexpr int lds = 4 * kKeys * DP * 2;
+  static std::atomic<uint64_t> done{0};
+  ensure_lds_attr(done, reinterpret_cast<const void*>(attn_fwd_kernel<T, DP, NW>), lds);
+  attn_fwd_kernel<T, DP, NW><<<dim3((unsigned)(p.n_rows * p.kv_heads)), NW * 64, lds, s>>>(p);
+  AHR_HIP(hipGetLastError());
+  if (p.n_join) {
+    attn_join_kernel<T><<<dim3((unsigned)(p.n_join * p.heads)), 256, 0, s>>>(p);
+    AHR_HIP(hipGetLastError());
+  }
+  return AHR_OK;
+}
+
+template <typename T, int DP>
+static int launch_fwd_w(const Params& p, int waves, hipStream_t s) {
+  if (waves == 1) return launch_fwd<T, DP, 1>(p, s);
+  if (waves == 2) return launch_fwd<T, DP, 2>(p, s);
+  return launch_fwd<T, DP, 4>(p, s);
+}
+
+template <typename T>
+static int launch_fwd_d(const Params& p, int waves, hipStream_t s) {
+  if (p.dim <= 32) return launch_fwd_w<T, 32>(p, waves, s);
+  if (p.dim <= 64) return launch_fwd_w<T, 64>(p, waves, s);
+  if (p.dim <= 96) return launch_fwd_w<T, 96>(p, waves, s);
+  return launch_fwd_w<T, 128>(p, waves, s);
+}
+
+}  // namespace attn
+}  // namespace ahr
+
+extern "C" {
+
+int ahr_attn_plan_build(const int32_t* q_len, const int32_t* k_len, int n, const ahr_attn_shape* shape,
+                        ahr_attn_plan* plan, int32_t* buf, int64_t cap) {
+  using namespace ahr;
+  if (!shape || !plan || n < 0 || (n > 0 && !q_len)) return fail(AHR_EINVAL, "null lengths, shape or plan");
+  int st = attn::check_shape(*shape);
+  if (st != AHR_OK) return st;
+  try {
+    return attn::build(q_len, k_len, n, *shape, plan, buf, cap);
+  } catch (...) {
+    return fail(AHR_ENOMEM, "out of host memory for the work lists");
+  }
+}
+
+int ahr_attn_forward(const ahr_attn_args* a, void* stream) {
+  using namespace ahr;
+  attn::Params p;
+  int st = attn::fill(a, false, &p);
+  if (st != AHR_OK) return st;
+  if (p.n_rows == 0) return AHR_OK;
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  if (a->plan->shape.dtype == AHR_BF16) return attn::launch_fwd_d<__bf16>(p, a->plan->waves, s);
+  return attn::launch_fwd_d<_Float16>(p, a->plan->waves, s);
+}
+
+int ahr_attn_backward(const ahr_attn_args* a, void* stream) {
+  using namespace ahr;
+  attn::Params p;
+  int st = attn::fill(a, true, &p);
+  if (st != AHR_OK) return st;
+  return attn::launch_backward(a, p, reinterpret_cast<hipStream_t>(stream));
+}
+
+}  // extern "C"

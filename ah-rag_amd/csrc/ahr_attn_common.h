@@ -1,0 +1,124 @@
+// Device helpers of the packed-attention kernels (gfx950): element types, the LDS swizzle of a
+// staged tile, fragment reads and the LDS-DMA that fills it.
+#pragma once
+
+#include "ahr_attn.h"
+#include "ahr_dense_common.h"
+
+namespace ahr {
+namespace attn {
+
+using dense::bf16x8;
+using dense::f16x8;
+using dense::f32x16;
+using dense::f32x4;
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+
+template <typename T>
+struct Elem;
+template <>
+struct Elem<__bf16> {
+  typedef bf16x8 v8;
+  typedef bf16x4 v4;
+  static constexpr bool kNarrow = false;
+  static __device__ __forceinline__ f32x16 mma(v8 a, v8 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+  }
+};
+template <>
+struct Elem<_Float16> {
+  typedef f16x8 v8;
+  typedef f16x4 v4;
+  static constexpr bool kNarrow = true;  // a 5-bit exponent
+  static __device__ __forceinline__ f32x16 mma(v8 a, v8 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+  }
+};
+
+// A staged tile holds rows of NC = DP / 8 chunks of 16 B without padding; chunk c of row r sits in
+// slot c ^ swz<NC>(r). It serves both ways a tile is read: 16-B row fragments (32 rows, the same
+// chunk) reach all sixteen 16-B slots of the 256-B bank row within a lane group, and transposed
+// 8-B reads (4 rows x 64 B) reach its four 64-B parts.
+template <int NC>
+__device__ __forceinline__ int swz(int r) {
+  if constexpr (NC == 16) return ((r & 3) << 2) | ((r >> 2) & 3);
+  if constexpr (NC == 8) return ((r & 2) << 1) | ((r >> 2) & 3);
+  return (r >> 2) & 3;
+}
+
+// 8 consecutive elements of row r at chunk 2 * ks + h: an A operand of 32x32x16 whose rows are the
+// tile's rows (lane l: row l & 31, k = 8 * (l >> 5) + 0..7).
+template <typename T, int NC>
+__device__ __forceinline__ typename Elem<T>::v8 row_frag(const char* tile, int r, int ks, int h) {
+  return *reinterpret_cast<const typename Elem<T>::v8*>(tile + r * (NC * 16) + (((2 * ks + h) ^ swz<NC>(r)) << 4));
+}
+
+// The transposed operand: rows of the result are 32 columns (block db) of the tile, k runs over 16
+// of its rows from r0 in the order in which a 32x32 accumulator holds them (lane half h: rows
+// 4h..4h+3, 8+4h..8+4h+3), so that accumulator values become the other operand without moving
+// between lanes. Each 16-lane group of the read transposes 4 rows x 16 columns.
+template <typename T, int NC>
+__device__ __forceinline__ typename Elem<T>::v8 col_frag(const char* tile, int r0, int db, int lane) {
+  typedef __attribute__((address_space(3))) s16x4* lds4;
+  const int h = lane >> 5, lr = (lane & 15) >> 2;
+  const int c = db * 4 + ((lane >> 4) & 1) * 2 + ((lane & 3) >> 1);
+  const int ra = r0 + 4 * h + lr, rb = ra + 8;
+  const char* pa = tile + ra * (NC * 16) + ((c ^ swz<NC>(ra)) << 4) + (lane & 1) * 8;
+  const char* pb = tile + rb * (NC * 16) + ((c ^ swz<NC>(rb)) << 4) + (lane & 1) * 8;
+  const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)pa);
+  const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)pb);
+  const s16x8 ab = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+  return __builtin_bit_cast(typename Elem<T>::v8, ab);
+}
+
+// values x[o .. o+7] of an accumulator as the other operand
+template <typename T>
+__device__ __forceinline__ typename Elem<T>::v8 acc_frag(const f32x16& x, int o) {
+  typename Elem<T>::v8 f;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) f[j] = (T)x[o + j];
+  return f;
+}
+
+// row of a 32x32 accumulator register r in lane half h
+__device__ __forceinline__ int acc_row(int r, int h) { return (r & 3) + 8 * (r >> 2) + 4 * h; }
+
+__device__ __forceinline__ float other_half(float x) { return __shfl_xor(x, 32, 64); }
+
+__device__ __forceinline__ float ex2(float x) { return __builtin_amdgcn_exp2f(x); }
+
+template <typename T>
+__device__ __forceinline__ void store4(char* p, float a, float b, float c, float d) {
+  typename Elem<T>::v4 x;
+  x[0] = (T)a;
+  x[1] = (T)b;
+  x[2] = (T)c;
+  x[3] = (T)d;
+  *reinterpret_cast<typename Elem<T>::v4*>(p) = x;
+}
+
+// LDS-DMA of tile rows: the NC * ROWS / 64 16-B-per-lane loads are dealt to the NW waves.
+template <int NC, int NW, int ROWS>
+struct Stager {
+  static constexpr int kPer = NC * ROWS / 64 / NW;
+  int wave, lane;
+  __device__ __forceinline__ Stager(int w, int l) : wave(w), lane(l) {}
+  // off(row) -> byte offset of the row from the descriptor's base (rows past the range repeat a
+  // valid one: every load stays inside the tensors). Chunks past dim are left alone (zeroed once).
+  template <typename F>
+  __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t r, char* tile, int dim, F off) const {
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const int ci = (i * NW + wave) * 64 + lane;
+      const int row = ci / NC, c = (ci % NC) ^ swz<NC>(row);
+      if (NC * 8 == dim || c * 8 < dim)
+        dense::blds16(r, (uint32_t)(off(row) + c * 16), tile + (i * NW + wave) * 1024);
+    }
+  }
+};
+
+}  // namespace attn
+}  // namespace ahr

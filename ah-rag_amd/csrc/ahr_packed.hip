@@ -1,0 +1,607 @@
+// Row operators of packed sequences: q/k norm with rotation, and mean pooling (include/ahr.h).
+//
+// Both are bound by memory: every value is read once and written once, the reductions stay in
+// registers, and sums that cross workgroups go through fp32 partial rows added in a fixed order.
+#include "ahr_common.h"
+#include "ahr.h"
+
+#include <algorithm>
+#include <cmath>
+#include <cstring>
+#include <type_traits>
+
+namespace ahr {
+namespace packed {
+
+template <typename T, int N>
+__device__ __forceinline__ void load_f32(float* to, const T* from) {  // N consecutive, aligned to N * sizeof(T) or 16 B
+  constexpr int W = (int)sizeof(T) * N >= 16 ? 16 / (int)sizeof(T) : N;
+#pragma unroll
+  for (int i = 0; i < N; i += W) {
+    typedef T vec __attribute__((ext_vector_type(W)));
+    const vec v = *reinterpret_cast<const vec*>(from + i);
+#pragma unroll
+    for (int j = 0; j < W; ++j) to[i + j] = (float)v[j];
+  }
+}
+template <typename T, int N>
+__device__ __forceinline__ void store_f32(T* to, const float* from) {
+  constexpr int W = (int)sizeof(T) * N >= 16 ? 16 / (int)sizeof(T) : N;
+#pragma unroll
+  for (int i = 0; i < N; i += W) {
+    typedef T vec __attribute__((ext_vector_type(W)));
+    vec v;
+#pragma unroll
+    for (int j = 0; j < W; ++j) v[j] = (T)from[i + j];
+    *reinterpret_cast<vec*>(to + i) = v;
+  }
+}
+
+struct Rope {
+  const void *q, *k, *yq, *yk;
+  void *oq, *ok;  // forward: outputs; backward: gradients
+  int64_t q_ts, q_hs, k_ts, k_hs, yq_ts, yq_hs, yk_ts, yk_hs, oq_ts, oq_hs, ok_ts, ok_hs;
+  const float *wq, *wk, *cos, *sin;
+  const int32_t* pos;
+  float* part;  // backward: [blocks][2][dim]
+  int64_t tokens, n_pos;
+  int heads, kv_heads, dim, rot;
+  float eps;
+};
+
+// Vector form (rot == head_dim, a multiple of 16, aligned rows). LPR lanes share a head's row; a lane
+// owns 8 pairs of the rotation: elements a = e0 .. e0+7 and b = e0 + dim/2 .. (interleaved: 16
+// consecutive elements, pair i = (2i, 2i+1)), so the rotation needs no exchange between lanes. A wave
+// takes one token at a time and keeps the lane's cos and sin for all its heads. BWD: dx and the
+// weights' gradients; each lane adds its part of dw over its tokens in registers, the workgroup joins
+// them into one partial row.
+template <typename T, int DIM, bool IL, bool BWD>
+__global__ __launch_bounds__(256) void rope_vec_kernel(Rope p) {
+  constexpr int LPR = DIM / 16;          // lanes of a row
+  constexpr int RPW = 64 / LPR;          // rows of a wave (lanes past RPW * LPR idle)
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int sub = lane / LPR, li = lane % LPR;
+  const bool on = sub < RPW;
+  const int e0 = IL ? li * 16 : li * 8;
+  const bool normed = p.wq != nullptr;
+  float w[2][16], dw[2][16];
+#pragma unroll
+  for (int s = 0; s < 2; ++s)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int e = IL ? e0 + i : (i < 8 ? e0 + i : DIM / 2 + e0 + i - 8);
+      w[s][i] = normed ? (s ? p.wk : p.wq)[e] : 1.f;
+      dw[s][i] = 0.f;
+    }
+  const int all = p.heads + p.kv_heads;
+  // heads of a token are dealt to gridDim.y slices
+  const int first = blockIdx.y * RPW, step = gridDim.y * RPW;
+  for (int64_t t = (int64_t)blockIdx.x * 4 + wave; t < p.tokens; t += (int64_t)gridDim.x * 4) {
+    const int64_t at = p.pos[t];
+    const bool known = at >= 0 && at < p.n_pos;
+    float c[8], s[8];
+    {
+      const int64_t o = (known ? at : 0) * (DIM / 2) + li * 8;
+      load_f32<float, 8>(c, p.cos + o);
+      load_f32<float, 8>(s, p.sin + o);
+      if (!known) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) c[i] = s[i] = NAN;
+      }
+    }
+    for (int h0 = first; h0 < all; h0 += step) {
+      const int hd = h0 + sub;
+      const bool have = on && hd < all;
+      const bool is_k = hd >= p.heads;
+      const int hh = is_k ? hd - p.heads : hd;
+      float x[16], y[16];
+      if (have) {
+        const T* xp = (const T*)(is_k ? p.k : p.q) + (is_k ? t * p.k_ts + hh * p.k_hs : t * p.q_ts + hh * p.q_hs);
+        if (IL) {
+          load_f32<T, 16>(x, xp + e0);
+        } else {
+          load_f32<T, 8>(x, xp + e0);
+          load_f32<T, 8>(x + 8, xp + DIM / 2 + e0);
+        }
+        if (BWD) {
+          const T* yp = (const T*)(is_k ? p.yk : p.yq) + (is_k ? t * p.yk_ts + hh * p.yk_hs : t * p.yq_ts + hh * p.yq_hs);
+          if (IL) {
+            load_f32<T, 16>(y, yp + e0);
+          } else {
+            load_f32<T, 8>(y, yp + e0);
+            load_f32<T, 8>(y + 8, yp + DIM / 2 + e0);
+          }
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) x[i] = y[i] = 0.f;
+      }
+      float r = 1.f;
+      if (normed) {
+        float sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) sum = fmaf(x[i], x[i], sum);
+#pragma unroll
+        for (int m = 1; m < 64; m *= 2)
+          if (m < LPR) sum += __shfl_xor(sum, m, 64);
+        r = 1.f / sqrtf(sum * (1.f / DIM) + p.eps);
+      }
+      const int sl = is_k ? 1 : 0;
+      float o[16];
+      if (!BWD) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int a = IL ? 2 * i : i, b = IL ? 2 * i + 1 : i + 8;
+          const float na = x[a] * r * (sl ? w[1][a] : w[0][a]), nb = x[b] * r * (sl ? w[1][b] : w[0][b]);
+          o[a] = na * c[i] - nb * s[i];
+          o[b] = nb * c[i] + na * s[i];
+        }
+      } else {
+        // dn = R^T dy; dw += dn x r; dx = r (dn w - x r^2 mean(dn w x))
+        float dot = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int a = IL ? 2 * i : i, b = IL ? 2 * i + 1 : i + 8;
+          float da = y[a] * c[i] + y[b] * s[i], db = y[b] * c[i] - y[a] * s[i];
+          const float ua = da * x[a] * r, ub = db * x[b] * r;
+          // (idle rows hold zeros; an unknown position's NaN belongs to rows that exist)
+          if (have) {
+            dw[0][a] += sl ? 0.f : ua;
+            dw[0][b] += sl ? 0.f : ub;
+            dw[1][a] += sl ? ua : 0.f;
+            dw[1][b] += sl ? ub : 0.f;
+          }
+          da *= sl ? w[1][a] : w[0][a];
+          db *= sl ? w[1][b] : w[0][b];
+          dot = fmaf(da, x[a], fmaf(db, x[b], dot));
+          o[a] = da;
+          o[b] = db;
+        }
+        if (normed) {
+#pragma unroll
+          for (int m = 1; m < 64; m *= 2)
+            if (m < LPR) dot += __shfl_xor(dot, m, 64);
+          const float f = dot * (1.f / DIM) * r * r;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) o[i] = r * (o[i] - x[i] * f);
+        }
+      }
+      if (have) {
+        T* op = (T*)(is_k ? p.ok : p.oq) + (is_k ? t * p.ok_ts + hh * p.ok_hs : t * p.oq_ts + hh * p.oq_hs);
+        if (IL) {
+          store_f32<T, 16>(op + e0, o);
+        } else {
+          store_f32<T, 8>(op + e0, o);
+          store_f32<T, 8>(op + DIM / 2 + e0, o + 8);
+        }
+      }
+    }
+  }
+  if (BWD && normed) {
+    // the rows of a wave, then the four waves, in a fixed order
+    __shared__ float acc[4][RPW][2][DIM];
+    if (on) {
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int e = IL ? e0 + i : (i < 8 ? e0 + i : DIM / 2 + e0 + i - 8);
+          acc[wave][sub][s][e] = dw[s][i];
+        }
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < 2 * DIM; i += 256) {
+      float sum = 0.f;
+      for (int a = 0; a < 4; ++a)
+        for (int b = 0; b < RPW; ++b) sum += acc[a][b][i / DIM][i % DIM];
+      p.part[((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * 2 * DIM + i] = sum;
+    }
+  }
+}
+
+// General form: any even head_dim up to 512, any even rot <= head_dim, any alignment; one wave per
+// head row at a time, element e of a row in lane e % 64. Rotation partners are read from memory again.
+template <typename T, bool BWD>
+__global__ __launch_bounds__(256) void rope_any_kernel(Rope p, int il) {
+  constexpr int E = 8;  // 512 / 64
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const bool normed = p.wq != nullptr;
+  const int all = p.heads + p.kv_heads, half = p.rot / 2;
+  float dw[2][E];
+#pragma unroll
+  for (int i = 0; i < E; ++i) dw[0][i] = dw[1][i] = 0.f;
+  for (int64_t row = (int64_t)blockIdx.x * 4 + wave; row < p.tokens * all; row += (int64_t)gridDim.x * 4) {
+    const int64_t t = row / all;
+    const int hd = (int)(row - t * all);
+    const bool is_k = hd >= p.heads;
+    const int hh = is_k ? hd - p.heads : hd;
+    const T* xp = (const T*)(is_k ? p.k : p.q) + (is_k ? t * p.k_ts + hh * p.k_hs : t * p.q_ts + hh * p.q_hs);
+    const T* yp = (const T*)(is_k ? p.yk : p.yq) + (is_k ? t * p.yk_ts + hh * p.yk_hs : t * p.yq_ts + hh * p.yq_hs);
+    T* op = (T*)(is_k ? p.ok : p.oq) + (is_k ? t * p.ok_ts + hh * p.ok_hs : t * p.oq_ts + hh * p.oq_hs);
+    const float* w = is_k ? p.wk : p.wq;
+    const int64_t at = p.pos[t];
+    const bool known = at >= 0 && at < p.n_pos;
+    const float* cp = p.cos + (known ? at : 0) * half;
+    const float* sp = p.sin + (known ? at : 0) * half;
+    float sum = 0.f;
+    if (normed)
+      for (int e = lane; e < p.dim; e += 64) sum = fmaf((float)xp[e], (float)xp[e], sum);
+#pragma unroll
+    for (int m = 1; m < 64; m *= 2) sum += __shfl_xor(sum, m, 64);
+    const float r = normed ? 1.f / sqrtf(sum / p.dim + p.eps) : 1.f;
+    float dot = 0.f, g[E];
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+      const int e = lane + 64 * i;
+      g[i] = 0.f;
+      if (e >= p.dim) continue;
+      // the other element of e's pair, its table entry, and the sign of its sine term
+      const bool turned = e < p.rot;
+      const int mate = !turned ? e : (il ? e ^ 1 : (e < half ? e + half : e - half));
+      const int ti = !turned ? 0 : (il ? e >> 1 : (e < half ? e : e - half));
+      const float sg = (il ? (e & 1) : e >= half) ? 1.f : -1.f;
+      const float c = turned ? (known ? cp[ti] : NAN) : (known ? 1.f : NAN);
+      const float s = turned ? (known ? sp[ti] : NAN) : 0.f;
+      if (!BWD) {
+        const float a = (float)xp[e] * r * (normed ? w[e] : 1.f), b = (float)xp[mate] * r * (normed ? w[mate] : 1.f);
+        g[i] = a * c + sg * b * s;
+      } else {
+        float d = (float)yp[e] * c - sg * (float)yp[mate] * s;
+        const float x = (float)xp[e];
+        if (is_k) dw[1][i] += d * x * r; else dw[0][i] += d * x * r;
+        if (normed) d *= w[e];
+        dot = fmaf(d, x, dot);
+        g[i] = d;
+      }
+    }
+    if (BWD && normed) {
+#pragma unroll
+      for (int m = 1; m < 64; m *= 2) dot += __shfl_xor(dot, m, 64);
+      const float f = dot / p.dim * r * r;
+#pragma unroll
+      for (int i = 0; i < E; ++i)
+        if (lane + 64 * i < p.dim) g[i] = r * (g[i] - (float)xp[lane + 64 * i] * f);
+    }
+#pragma unroll
+    for (int i = 0; i < E; ++i)
+      if (lane + 64 * i < p.dim) op[lane + 64 * i] = (T)g[i];
+  }
+  if (BWD && normed) {
+    __shared__ float acc[4][2][512];
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+      acc[wave][0][lane + 64 * i] = dw[0][i];
+      acc[wave][1][lane + 64 * i] = dw[1][i];
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < 2 * p.dim; i += 256) {
+      const int s = i / p.dim, e = i % p.dim;
+      p.part[(int64_t)blockIdx.x * 2 * p.dim + i] = acc[0][s][e] + acc[1][s][e] + acc[2][s][e] + acc[3][s][e];
+    }
+  }
+}
+
+// dw = the sum of the workgroups' partial rows: a workgroup per 16 columns, 16 threads a column
+__global__ __launch_bounds__(256) void rope_dw_kernel(const float* part, int blocks, int dim, float* dwq, float* dwk) {
+  __shared__ float acc[16][17];
+  const int col = blockIdx.x * 16 + (threadIdx.x & 15), y = threadIdx.x >> 4;
+  float s = 0.f;
+  if (col < 2 * dim)
+    for (int b = y; b < blocks; b += 16) s += part[(int64_t)b * 2 * dim + col];
+  acc[y][threadIdx.x & 15] = s;
+  __syncthreads();
+  if (y == 0 && col < 2 * dim) {
+    float t = 0.f;
+    for (int i = 0; i < 16; ++i) t += acc[i][threadIdx.x & 15];
+    (col < dim ? dwq : dwk)[col % dim] = t;
+  }
+}
+
+constexpr int kRopeBlocks = 1024;
+
+static int64_t rope_ws(int dim) { return (int64_t)kRopeBlocks * 2 * dim * 4; }
+
+static int rope_check(const ahr_rope_args* a, bool bwd) {
+  if (!a) return fail(AHR_EINVAL, "null arguments");
+  if (a->dtype != AHR_F32 && a->dtype != AHR_F16 && a->dtype != AHR_BF16) return fail(AHR_EINVAL, "unknown dtype");
+  if (a->heads < 0 || a->kv_heads < 0 || a->heads + a->kv_heads < 1 || a->heads > 65536 || a->kv_heads > 65536) return fail(AHR_EINVAL, "heads out of range");
+  if (a->head_dim < 2 || a->head_dim % 2 || a->head_dim > 512) return fail(AHR_EUNSUP, "head_dim must be even, at most 512");
+  if (a->rot < 2 || a->rot % 2 || a->rot > a->head_dim) return fail(AHR_EINVAL, "rot must be even, between 2 and head_dim");
+  if (a->tokens < 0 || a->n_pos < 0) return fail(AHR_EINVAL, "negative size");
+  if ((a->wq == nullptr) != (a->wk == nullptr)) return fail(AHR_EINVAL, "one norm weight without the other");
+  if (!(a->eps >= 0.f) || !std::isfinite(a->eps)) return fail(AHR_EINVAL, "eps must be finite and not negative");
+  if (a->tokens == 0) return AHR_OK;
+  if (a->n_pos < 1 || !a->cos || !a->sin || !a->positions) return fail(AHR_EINVAL, "null positions or table");
+  const ahr_tensor3 *t[6] = {&a->q, &a->yq, &a->dq, &a->k, &a->yk, &a->dk};
+  for (int i = 0; i < 6; ++i) {
+    if ((i < 3 ? a->heads : a->kv_heads) == 0 || (i % 3 == 2 && !bwd)) continue;
+    if (!t[i]->p || t[i]->ts < 0 || t[i]->hs < 0) return fail(AHR_EINVAL, "null tensor or negative stride");
+  }
+  if (bwd && a->wq) {
+    if (!a->dwq || !a->dwk) return fail(AHR_EINVAL, "null weight gradients");
+    if (!a->ws || a->ws_bytes < rope_ws(a->head_dim)) return fail(AHR_EINVAL, "workspace smaller than ahr_rope_ws_bytes");
+  }
+  return AHR_OK;
+}
+
+template <typename T, bool BWD>
+static int rope_launch(const ahr_rope_args* a, const Rope& p, hipStream_t s) {
+  const ahr_tensor3* t[6] = {&a->q, &a->yq, &a->dq, &a->k, &a->yk, &a->dk};
+  const int al = 16 / (int)sizeof(T);
+  bool vec = a->rot == a->head_dim;
+  for (int i = 0; i < 6; ++i) {
+    if ((i < 3 ? a->heads : a->kv_heads) == 0 || (i % 3 == 2 && !BWD)) continue;
+    vec = vec && reinterpret_cast<uintptr_t>(t[i]->p) % 16 == 0 && t[i]->ts % al == 0 && t[i]->hs % al == 0;
+  }
+  vec = vec && reinterpret_cast<uintptr_t>(p.cos) % 16 == 0 && reinterpret_cast<uintptr_t>(p.sin) % 16 == 0;
+  const int all = a->heads + a->kv_heads;
+  int blocks = 0;
+  const int il = a->interleaved;
+#define AHR_ROPE(D)                                                                                     \
+  {                                                                                                     \
+    const int rpw = 64 / (D / 16), rounds = (all + rpw - 1) / rpw;                                      \
+    const int64_t want = (a->tokens + 3) / 4;                                                           \
+    /* few tokens: a token's heads are spread over more waves, for latency */                           \
+    int gy = 1;                                                                                         \
+    while (gy < rounds && want * gy < 512) gy *= 2;                                                     \
+    const int gx = (int)std::min<int64_t>(want, BWD ? kRopeBlocks / gy : 65536);                        \
+    blocks = gx * gy;                                                                                   \
+    if (il) rope_vec_kernel<T, D, true, BWD><<<dim3(gx, gy), 256, 0, s>>>(p);                           \
+    else rope_vec_kernel<T, D, false, BWD><<<dim3(gx, gy), 256, 0, s>>>(p);                             \
+  }
+  if (vec && a->head_dim == 32) AHR_ROPE(32)
+  else if (vec && a->head_dim == 64) AHR_ROPE(64)
+  else if (vec && a->head_dim == 128) AHR_ROPE(128)
+  else if (vec && a->head_dim == 256) AHR_ROPE(256)
+  else {
+    blocks = (int)std::min<int64_t>((a->tokens * all + 3) / 4, BWD ? kRopeBlocks : 65536);
+    rope_any_kernel<T, BWD><<<dim3(blocks), 256, 0, s>>>(p, il);
+  }
+#undef AHR_ROPE
+  AHR_HIP(hipGetLastError());
+  if (BWD && a->wq) {
+    rope_dw_kernel<<<dim3((2 * a->head_dim + 15) / 16), 256, 0, s>>>(p.part, blocks, a->head_dim, a->dwq, a->dwk);
+    AHR_HIP(hipGetLastError());
+  }
+  return AHR_OK;
+}
+
+template <bool BWD>
+static int rope(const ahr_rope_args* a, void* stream) {
+  const int st = rope_check(a, BWD);
+  if (st != AHR_OK) return st;
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  Rope p;
+  memset(&p, 0, sizeof p);
+  p.q = a->q.p, p.q_ts = a->q.ts, p.q_hs = a->q.hs;
+  p.k = a->k.p, p.k_ts = a->k.ts, p.k_hs = a->k.hs;
+  const ahr_tensor3 &oq = BWD ? a->dq : a->yq, &ok = BWD ? a->dk : a->yk;
+  p.yq = a->yq.p, p.yq_ts = a->yq.ts, p.yq_hs = a->yq.hs;
+  p.yk = a->yk.p, p.yk_ts = a->yk.ts, p.yk_hs = a->yk.hs;
+  p.oq = oq.p, p.oq_ts = oq.ts, p.oq_hs = oq.hs;
+  p.ok = ok.p, p.ok_ts = ok.ts, p.ok_hs = ok.hs;
+  p.wq = a->wq, p.wk = a->wk, p.cos = a->cos, p.sin = a->sin, p.pos = a->positions;
+  p.part = (float*)a->ws;
+  p.tokens = a->tokens, p.n_pos = a->n_pos;
+  p.heads = a->heads, p.kv_heads = a->kv_heads, p.dim = a->head_dim, p.rot = a->rot;
+  p.eps = a->eps;
+  if (a->tokens == 0) {
+    if (BWD && a->wq) {  // no rows: zero weight gradients
+      rope_dw_kernel<<<dim3((2 * a->head_dim + 15) / 16), 256, 0, s>>>(p.part, 0, a->head_dim, a->dwq, a->dwk);
+      AHR_HIP(hipGetLastError());
+    }
+    return AHR_OK;
+  }
+  if (a->dtype == AHR_F32) return rope_launch<float, BWD>(a, p, s);
+  if (a->dtype == AHR_F16) return rope_launch<_Float16, BWD>(a, p, s);
+  return rope_launch<__bf16, BWD>(a, p, s);
+}
+
+// ---- mean pooling ----------------------------------------------------------------------------
+
+constexpr float kPoolEps = 1e-12f;
+
+// Sum of a chunk's rows: a workgroup per chunk and 64 * V columns, its four waves take every fourth row.
+template <typename T, int V>
+__global__ __launch_bounds__(256) void pool_sum_kernel(const T* rows, int64_t rs, int width, const int4* chunks, float* ws) {
+  __shared__ float acc[4][64 * V];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int4 ch = chunks[blockIdx.x];
+  const int col = (blockIdx.y * 64 + lane) * V;
+  float s[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) s[i] = 0.f;
+  if (col < width) {
+    const T* p = rows + (int64_t)ch.x * rs + col;
+#pragma unroll 4
+    for (int r = wave; r < ch.y; r += 4) {
+      float x[V];
+      load_f32<T, V>(x, p + (int64_t)r * rs);
+#pragma unroll
+      for (int i = 0; i < V; ++i) s[i] += x[i];
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < V; ++i) acc[wave][i * 64 + lane] = s[i];
+  __syncthreads();
+  float* o = ws + (int64_t)blockIdx.x * width + (int64_t)blockIdx.y * 64 * V;
+  for (int i = threadIdx.x; i < 64 * V; i += 256) {  // column i = lane' * V + part
+    const int j = (i % V) * 64 + i / V;
+    if (blockIdx.y * 64 * V + i < width) o[i] = acc[0][j] + acc[1][j] + acc[2][j] + acc[3][j];
+  }
+}
+
+__device__ __forceinline__ float block_sum(float x, float* red) {
+#pragma unroll
+  for (int m = 1; m < 64; m *= 2) x += __shfl_xor(x, m, 64);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = x;
+  __syncthreads();
+  x = red[0] + red[1] + red[2] + red[3];
+  __syncthreads();
+  return x;
+}
+
+// mean and norm of a sequence: its chunks' sums in order
+__global__ __launch_bounds__(256) void pool_mean_kernel(const float* ws, int width, const int2* seqs, int normalize, float* out,
+                                                        float* norm) {
+  __shared__ float red[4];
+  const int2 sq = seqs[blockIdx.x];
+  const int n = (sq.x + AHR_POOL_CHUNK - 1) / AHR_POOL_CHUNK;
+  float* o = out + (int64_t)blockIdx.x * width;
+  float ss = 0.f;
+  for (int c = threadIdx.x; c < width; c += 256) {
+    float s = 0.f;
+    for (int i = 0; i < n; ++i) s += ws[(int64_t)(sq.y + i) * width + c];
+    s = sq.x > 0 ? s / (float)sq.x : 0.f;
+    o[c] = s;
+    ss = fmaf(s, s, ss);
+  }
+  const float nm = sqrtf(block_sum(ss, red));
+  if (threadIdx.x == 0 && norm) norm[blockIdx.x] = nm;
+  if (!normalize) return;
+  const float d = fmaxf(nm, kPoolEps);
+  for (int c = threadIdx.x; c < width; c += 256) o[c] /= d;  // (each thread its own values)
+}
+
+// Gradient of the rows: the same for every row of a sequence, (d_out - out (out . d_out)) / (norm rows),
+// written to the rows of one chunk.
+template <typename T, int V>
+__global__ __launch_bounds__(256) void pool_grad_kernel(T* d_rows, int width, const int4* chunks, const int2* seqs, int normalize,
+                                                        const float* d_out, const float* out, const float* norm) {
+  __shared__ float red[4];
+  const int4 ch = chunks[blockIdx.x];
+  const float* dy = d_out + (int64_t)ch.z * width;
+  const float* y = out + (int64_t)ch.z * width;
+  float dot = 0.f, d = 1.f;
+  if (normalize) {
+    const float nm = norm[ch.z];
+    if (nm >= kPoolEps) {  // below it the division is by a constant
+      for (int c = threadIdx.x; c < width; c += 256) dot = fmaf(dy[c], y[c], dot);
+    }
+    dot = block_sum(dot, red);
+    d = fmaxf(nm, kPoolEps);
+  }
+  const float f = 1.f / (d * (float)seqs[ch.z].x);
+  T* p = d_rows + (int64_t)ch.x * width;
+  for (int c = threadIdx.x * V; c < width; c += 256 * V) {
+    float g[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) g[i] = (dy[c + i] - (normalize ? y[c + i] * dot : 0.f)) * f;
+    for (int r = 0; r < ch.y; ++r) store_f32<T, V>(p + (int64_t)r * width + c, g);
+  }
+}
+
+template <typename T>
+static int pool_sum(const void* rows, int64_t rs, int width, const int4* chunks, int n_chunks, float* ws, hipStream_t s) {
+  constexpr int V = 16 / (int)sizeof(T);
+  if (width % V == 0 && rs % V == 0 && reinterpret_cast<uintptr_t>(rows) % 16 == 0)
+    pool_sum_kernel<T, V><<<dim3(n_chunks, (width + 64 * V - 1) / (64 * V)), 256, 0, s>>>((const T*)rows, rs, width, chunks, ws);
+  else
+    pool_sum_kernel<T, 1><<<dim3(n_chunks, (width + 63) / 64), 256, 0, s>>>((const T*)rows, rs, width, chunks, ws);
+  AHR_HIP(hipGetLastError());
+  return AHR_OK;
+}
+
+template <typename T>
+static int pool_grad(void* d_rows, int width, const int4* chunks, int n_chunks, const int2* seqs, int normalize,
+                     const float* d_out, const float* out, const float* norm, hipStream_t s) {
+  constexpr int V = 16 / (int)sizeof(T);
+  if (width % V == 0 && reinterpret_cast<uintptr_t>(d_rows) % 16 == 0)
+    pool_grad_kernel<T, V><<<n_chunks, 256, 0, s>>>((T*)d_rows, width, chunks, seqs, normalize, d_out, out, norm);
+  else
+    pool_grad_kernel<T, 1><<<n_chunks, 256, 0, s>>>((T*)d_rows, width, chunks, seqs, normalize, d_out, out, norm);
+  AHR_HIP(hipGetLastError());
+  return AHR_OK;
+}
+
+}  // namespace packed
+}  // namespace ahr
+
+extern "C" {
+
+int ahr_rope_ws_bytes(int64_t tokens, int head_dim, int64_t* bytes) {
+  if (!bytes || tokens < 0 || head_dim < 2 || head_dim > 512) return ahr::fail(AHR_EINVAL, "null output or bad size");
+  *bytes = ahr::packed::rope_ws(head_dim);
+  return AHR_OK;
+}
+
+int ahr_qk_norm_rope(const ahr_rope_args* a, void* stream) { return ahr::packed::rope<false>(a, stream); }
+
+int ahr_qk_norm_rope_backward(const ahr_rope_args* a, void* stream) { return ahr::packed::rope<true>(a, stream); }
+
+int ahr_pool_plan_build(const int32_t* lengths, int n, int32_t* buf, int64_t cap, int* n_chunks) {
+  using namespace ahr;
+  if (n < 0 || (n > 0 && !lengths) || !n_chunks) return fail(AHR_EINVAL, "null lengths or output");
+  int64_t count = 0, tokens = 0;
+  for (int i = 0; i < n; ++i) {
+    if (lengths[i] < 0) return fail(AHR_EINVAL, "negative length");
+    count += ((int64_t)lengths[i] + AHR_POOL_CHUNK - 1) / AHR_POOL_CHUNK;
+    tokens += lengths[i];
+  }
+  if (tokens > INT32_MAX / 2) return fail(AHR_EINVAL, "more than 2^30 packed tokens");
+  *n_chunks = (int)count;
+  if (!buf) return AHR_OK;
+  if (cap < count * 4 + (int64_t)n * 2) return fail(AHR_EINVAL, "buffer smaller than the lists");
+  int32_t* c = buf;
+  int32_t* s = buf + count * 4;
+  int32_t row = 0, made = 0;
+  for (int i = 0; i < n; ++i) {
+    s[2 * i] = lengths[i];
+    s[2 * i + 1] = made;
+    for (int32_t t = 0; t < lengths[i]; t += AHR_POOL_CHUNK, ++made, c += 4) {
+      c[0] = row + t;
+      c[1] = std::min<int32_t>(AHR_POOL_CHUNK, lengths[i] - t);
+      c[2] = i;
+      c[3] = 0;
+    }
+    row += lengths[i];
+  }
+  return AHR_OK;
+}
+
+static int pool_check(int dtype, int width, const int32_t* lists, int n_chunks, int n) {
+  using namespace ahr;
+  if (dtype != AHR_F32 && dtype != AHR_F16 && dtype != AHR_BF16) return fail(AHR_EINVAL, "unknown dtype");
+  if (width < 1 || width > (1 << 20)) return fail(AHR_EINVAL, "width out of range");
+  if (n < 0 || n_chunks < 0 || (n > 0 && !lists) || reinterpret_cast<uintptr_t>(lists) % 16) return fail(AHR_EINVAL, "null or unaligned lists");
+  return AHR_OK;
+}
+
+int ahr_pool_mean(int dtype, const void* rows, int64_t rs, int width, const int32_t* lists, int n_chunks, int n,
+                  int normalize, float* out, float* norm, float* ws, int64_t ws_bytes, void* stream) {
+  using namespace ahr;
+  int st = pool_check(dtype, width, lists, n_chunks, n);
+  if (st != AHR_OK) return st;
+  if (n == 0) return AHR_OK;
+  if (!out || rs < 0 || (n_chunks > 0 && (!rows || !ws))) return fail(AHR_EINVAL, "null tensor or negative stride");
+  if (ws_bytes < (int64_t)n_chunks * width * 4) return fail(AHR_EINVAL, "workspace too small");
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  const int4* ch = reinterpret_cast<const int4*>(lists);
+  const int2* sq = reinterpret_cast<const int2*>(lists + (int64_t)n_chunks * 4);
+  if (n_chunks > 0) {
+    if (dtype == AHR_F32) st = packed::pool_sum<float>(rows, rs, width, ch, n_chunks, ws, s);
+    else if (dtype == AHR_F16) st = packed::pool_sum<_Float16>(rows, rs, width, ch, n_chunks, ws, s);
+    else st = packed::pool_sum<__bf16>(rows, rs, width, ch, n_chunks, ws, s);
+    if (st != AHR_OK) return st;
+  }
+  packed::pool_mean_kernel<<<n, 256, 0, s>>>(ws, width, sq, normalize, out, norm);
+  AHR_HIP(hipGetLastError());
+  return AHR_OK;
+}
+
+int ahr_pool_mean_backward(int dtype, void* d_rows, int width, const int32_t* lists, int n_chunks, int n, int normalize,
+                           const float* d_out, const float* out, const float* norm, void* stream) {
+  using namespace ahr;
+  int st = pool_check(dtype, width, lists, n_chunks, n);
+  if (st != AHR_OK) return st;
+  if (n_chunks == 0) return AHR_OK;
+  if (!d_rows || !d_out || (normalize && (!out || !norm))) return fail(AHR_EINVAL, "null tensor");
+  hipStream_t s = reinterpret_cast<hipStream_t>(stream);
+  const int4* ch = reinterpret_cast<const int4*>(lists);
+  const int2* sq = reinterpret_cast<const int2*>(lists + (int64_t)n_chunks * 4);
+  if (dtype == AHR_F32) return packed::pool_grad<float>(d_rows, width, ch, n_chunks, sq, normalize, d_out, out, norm, s);
+  if (dtype == AHR_F16) return packed::pool_grad<_Float16>(d_rows, width, ch, n_chunks, sq, normalize, d_out, out, norm, s);
+  return packed::pool_grad<__bf16>(d_rows, width, ch, n_chunks, sq, normalize, d_out, out, norm, s);
+}
+
+}  // extern "C"

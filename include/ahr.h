@@ -355,6 +355,110 @@ int ahr_graph_lca_large(ahr_graph* g, const int32_t* inputs, int B, int n_in, in
 
 int ahr_graph_info(const ahr_graph* g, int64_t* n_nodes, int64_t* n_edges);
 
+/* ------------------------------------------------------------------------------------------
+ * Packed sequences: the operators of a transformer over a batch whose sequences lie behind each
+ * other without padding (the sentence encoder's forward and its fine-tuning step). Tensors are
+ * device memory in AHR_F16 or AHR_BF16 unless stated; strides are in elements, the last dimension
+ * is contiguous. Replaces, for the encoder that the reference calls as a library
+ * (hierarchical_graph.py:655-656, :709-712), the padded attention and pooling of that library.
+ * ---------------------------------------------------------------------------------------- */
+
+typedef struct ahr_attn_shape {
+  int32_t dtype;      /* AHR_F16 or AHR_BF16 */
+  int32_t heads;      /* query heads: a multiple of kv_heads, at most 128 times as many */
+  int32_t kv_heads;
+  int32_t head_dim;   /* a multiple of 8, at most 128 */
+  int32_t causal;     /* 1: query i of a sequence with nq queries and nk keys reads the keys
+                         j <= i + nk - nq (the last query reads every key); 0: every key */
+  int32_t backward;   /* 1: work lists for ahr_attn_backward, 0: for ahr_attn_forward */
+  int64_t prefix;     /* keys of a prefix that every query of every sequence reads too (forward only) */
+} ahr_attn_shape;
+
+/* Sizes of a plan: the work lists that ahr_attn_plan_build lays out for the lengths of one batch.
+ * The lists (`ints` int32 values) are copied to the device by the caller, once, and used by every
+ * call on that batch. Opaque apart from ints and ws_bytes. */
+typedef struct ahr_attn_plan {
+  ahr_attn_shape shape;
+  int64_t tokens, key_tokens;   /* packed query tokens and keys */
+  int64_t ints;                 /* int32 values of the lists */
+  int64_t ws_bytes;             /* workspace of one call */
+  int64_t part_rows;
+  int32_t n_rows, n_keys, n_join, waves, planes, key_waves;
+} ahr_attn_plan;
+
+/* Host only. q_len / k_len: host int32 [n], >= 0 (k_len NULL: as q_len). buf NULL: fills *plan alone;
+ * else also writes plan->ints values to buf (capacity cap). */
+int ahr_attn_plan_build(const int32_t* q_len, const int32_t* k_len, int n, const ahr_attn_shape* shape,
+                        ahr_attn_plan* plan, int32_t* buf, int64_t cap);
+
+typedef struct ahr_tensor3 {  /* [tokens][heads][head_dim] */
+  void* p;
+  int64_t ts, hs;             /* strides of a token and of a head: multiples of 8, p 16-B aligned */
+} ahr_tensor3;
+
+typedef struct ahr_attn_args {
+  const ahr_attn_plan* plan;  /* host */
+  const int32_t* lists;       /* device: the plan's lists */
+  float scale;                /* > 0 */
+  int32_t reserved;
+  ahr_tensor3 q, k, v;        /* q [tokens][heads], k and v [key_tokens][kv_heads] */
+  ahr_tensor3 prefix_k, prefix_v; /* [prefix][kv_heads], or null with prefix 0 */
+  ahr_tensor3 o;              /* forward: written; backward: read. [tokens][heads] */
+  float* lse;                 /* [tokens][heads] fp32: log2 of the sum of 2^(scale log2(e) q.k) of each
+                                 row, -inf where it reads no key; forward writes it (NULL: not
+                                 wanted), backward reads it */
+  ahr_tensor3 d_o;            /* backward: gradient of o, and the gradients that it writes */
+  ahr_tensor3 dq, dk, dv;
+  void* ws;                   /* device, plan->ws_bytes, 16-B aligned */
+  int64_t ws_bytes;
+} ahr_attn_args;
+
+/* o = softmax(scale q k^T) v within each sequence. A row that reads no key gives zeros. Allocates
+ * nothing and synchronises nothing: capturable. */
+int ahr_attn_forward(const ahr_attn_args* a, void* stream);
+/* dq, dk, dv from d_o, with o and lse of the forward pass. No atomics: the same inputs give the same
+ * bits. Gradients of a key head are summed over its query heads in fp32. */
+int ahr_attn_backward(const ahr_attn_args* a, void* stream);
+
+/* RMS norm of each head of q and k times a weight, and the rotation by the token's position, in one
+ * pass: y = R(n), n = x w / sqrt(mean(x^2) + eps); the rotation turns the pairs (n_i, n_{i + rot/2})
+ * (interleaved: (n_2i, n_2i+1)), i < rot/2, by the angle whose cos and sin are table rows
+ * [positions[t]] (fp32 [n_pos][rot/2]); elements from rot on are only normed. Weights fp32 [head_dim],
+ * both NULL: rotation alone. A position outside [0, n_pos) gives NaN rows. head_dim even, <= 512.
+ * dtype: AHR_F32 / F16 / BF16. */
+typedef struct ahr_rope_args {
+  int32_t dtype, heads, kv_heads, head_dim, rot, interleaved;
+  int64_t tokens, n_pos;
+  float eps;
+  int32_t reserved;
+  ahr_tensor3 q, k;           /* inputs (any alignment of the elements) */
+  ahr_tensor3 yq, yk;         /* forward: outputs; backward: the outputs' gradients (read) */
+  ahr_tensor3 dq, dk;         /* backward: written */
+  const float *wq, *wk, *cos, *sin;
+  const int32_t* positions;   /* [tokens] */
+  float *dwq, *dwk;           /* backward: fp32 [head_dim], or NULL with wq NULL */
+  void* ws;                   /* backward: ahr_rope_ws_bytes */
+  int64_t ws_bytes;
+} ahr_rope_args;
+int ahr_rope_ws_bytes(int64_t tokens, int head_dim, int64_t* bytes);
+int ahr_qk_norm_rope(const ahr_rope_args* a, void* stream);
+int ahr_qk_norm_rope_backward(const ahr_rope_args* a, void* stream);
+
+/* Mean over the rows of each sequence in fp32, then (normalize) division by max(L2 norm, 1e-12).
+ * The work lists of a batch's lengths (host int32 [n]) are laid out once by ahr_pool_plan_build: chunks
+ * of at most AHR_POOL_CHUNK rows, int32 [n_chunks][4], then int32 [n][2]; buf NULL: *n_chunks alone.
+ * The caller copies them to the device (16-B aligned). */
+#define AHR_POOL_CHUNK 64
+int ahr_pool_plan_build(const int32_t* lengths, int n, int32_t* buf, int64_t cap, int* n_chunks);
+/* rows [tokens][width] in dtype (AHR_F32 / F16 / BF16), row stride rs elements. out fp32 [n][width];
+ * norm fp32 [n] (NULL: not wanted): the norm of the mean, for the backward pass. A sequence without
+ * rows gives zeros. ws: n_chunks * width * 4 bytes. Capturable. */
+int ahr_pool_mean(int dtype, const void* rows, int64_t rs, int width, const int32_t* lists, int n_chunks, int n,
+                  int normalize, float* out, float* norm, float* ws, int64_t ws_bytes, void* stream);
+/* d_rows [tokens][width] (contiguous, dtype) from d_out, and out and norm of the forward pass, fp32. */
+int ahr_pool_mean_backward(int dtype, void* d_rows, int width, const int32_t* lists, int n_chunks, int n, int normalize,
+                           const float* d_out, const float* out, const float* norm, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
