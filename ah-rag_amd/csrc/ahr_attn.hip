@@ -24,10 +24,102 @@ namespace attn {
 
 constexpr float kRaise = 8.f;  // how far (log2) a score may exceed the reference before it is raised
 
+// What a wave carries from tile to tile: its 32 rows' queries, and one row for each lane (the other
+// half-lane the same row, other keys).
+template <typename T, int DP>
+struct FwdState {
+  typename Elem<T>::v8 qf[DP / 16];
+  f32x16 acc[DP / 32];  // o, transposed
+  float m, l;           // reference (of c s), this half-lane's part of the sum
+};
+
+// One staged tile of keys and values (cur) for one wave: the first `mine` keys count for this lane's
+// row; `cut`: not the same 64 for all rows of the wave.
+// (cur is restrict: the reads must not wait for the DMA that fills the other buffer meanwhile.)
+template <typename T, int DP>
+__device__ __forceinline__ void fwd_tile(const char* __restrict__ cur, FwdState<T, DP>& st, bool cut, int mine, float c, int lane) {
+  typedef typename Elem<T>::v8 v8;
+  constexpr int NC = DP / 8, KS = DP / 16, DB = DP / 32;
+  constexpr int kTile = kKeys * DP * 2;
+  const int h = lane >> 5, n = lane & 31;
+  f32x16 s[2];
+#pragma unroll
+  for (int u = 0; u < 2; ++u)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s[u][r] = 0.f;
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+    for (int u = 0; u < 2; ++u) s[u] = Elem<T>::mma(row_frag<T, NC>(cur, u * 32 + n, ks, h), st.qf[ks], s[u]);
+
+  if (cut) {  // keys that a row does not read: selected away, whatever their scores are
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[u][r] = u * 32 + acc_row(r, h) < mine ? s[u][r] : -INFINITY;
+  }
+
+  float top = s[0][0];
+#pragma unroll
+  for (int u = 0; u < 2; ++u)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) top = fmaxf(top, s[u][r]);
+  top = fmaxf(top, other_half(top)) * c;
+  if (__any(top > st.m + kRaise)) {  // (m = -inf before the first key)
+    const float to = fmaxf(st.m, top);
+    const float f = to == -INFINITY ? 1.f : ex2(st.m - to);
+    st.l *= f;
+#pragma unroll
+    for (int b = 0; b < DB; ++b)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) st.acc[b][r] *= f;
+    st.m = to;
+  }
+  const float ref = st.m == -INFINITY ? 0.f : st.m;
+  float add = 0.f;
+#pragma unroll
+  for (int u = 0; u < 2; ++u)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      s[u][r] = ex2(fmaf(s[u][r], c, -ref));
+      add += s[u][r];
+    }
+  st.l += add;
+
+#pragma unroll
+  for (int g = 0; g < 4; ++g) {
+    const v8 pf = acc_frag<T>(s[g >> 1], (g & 1) * 8);
+#pragma unroll
+    for (int b = 0; b < DB; ++b) st.acc[b] = Elem<T>::mma(col_frag<T, NC>(cur + kTile, g * 16, b, lane), pf, st.acc[b]);
+  }
+}
+
+template <typename T, int DP, int NW>
+__device__ __forceinline__ void fwd_step(const char* __restrict__ cur, char* __restrict__ nxt, FwdState<T, DP>& st,
+                                         const Stager<DP / 8, NW, kKeys>& stager, const Params& p, const RowItem& it, int hk, int t, int np,
+                                         int nt, bool wave_live, int lim, int lim_lo, int lim_hi, int lane) {
+  auto stage = [&](int t) {
+    const bool pre = t < np;
+    const int kt = pre ? it.pb + t * kKeys : it.kb + (t - np) * kKeys;
+    const int have = min(kKeys, (pre ? it.pe : it.ke) - kt);
+    const int64_t at = pre ? kt : (int64_t)it.k0 + kt;
+    const int64_t kts = pre ? p.pk_ts : p.k_ts, vts = pre ? p.pv_ts : p.v_ts;
+    stage_kv<DP, NW>(nxt, stager, (pre ? p.pk : p.k) + (at * kts + hk * (pre ? p.pk_hs : p.k_hs)) * 2,
+                     (pre ? p.pv : p.v) + (at * vts + hk * (pre ? p.pv_hs : p.v_hs)) * 2, kts, vts, have, p.dim);
+  };
+  if (t + 1 < nt) stage(t + 1);
+  if (t < 0) return;
+  const bool pre = t < np;
+  const int kt = pre ? it.pb + t * kKeys : it.kb + (t - np) * kKeys;
+  const int stop = pre ? it.pe : it.ke;
+  if (!wave_live || (!pre && kt >= lim_hi)) return;  // no row of the wave reads from here on
+  fwd_tile<T, DP>(cur, st, kt + kKeys > stop || (!pre && kt + kKeys > lim_lo), (pre ? stop : min(lim, stop)) - kt, p.scale_log2, lane);
+}
+
 template <typename T, int DP, int NW>
 __global__ __launch_bounds__(NW * 64, 2) void attn_fwd_kernel(Params p) {
   typedef typename Elem<T>::v8 v8;
-  constexpr int NC = DP / 8, KS = DP / 16, DB = DP / 32;
+  constexpr int KS = DP / 16, DB = DP / 32;
   constexpr int kTile = kKeys * DP * 2;
   extern __shared__ __attribute__((aligned(16))) char smem[];  // [2][K tile, V tile]
   const int lane = threadIdx.x & 63, h = lane >> 5, n = lane & 31;
@@ -49,123 +141,44 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_fwd_kernel(Params p) {
   const int head = hk * p.group + (live ? row - tok * p.group : 0);
   const int lim = live ? (p.causal ? min(it.klen, it.koff + tok + 1) : it.klen) : 0;  // own keys it reads
   const bool wave_live = wave * 32 < n_rows;
+  // smallest and largest number of own keys that a row of this wave reads
+  const int first = (wave * 32 * p.group_inv) >> 16, last = ((min(wave * 32 + 32, n_rows) - 1) * p.group_inv) >> 16;
+  const int lim_lo = p.causal ? min(it.klen, it.koff + first + 1) : it.klen;
+  const int lim_hi = p.causal ? min(it.klen, it.koff + last + 1) : it.klen;
 
-  v8 qf[KS];
+  FwdState<T, DP> st;
   {
     const char* qp = p.q + ((int64_t)(it.q0 + tok) * p.q_ts + (int64_t)head * p.q_hs) * 2;
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
       const int d = (2 * ks + h) * 8;
-      v8 z = {};
-      qf[ks] = (live && (DP == dim || d < dim)) ? *reinterpret_cast<const v8*>(qp + d * 2) : z;
+      const v8 z = {};
+      st.qf[ks] = (live && (DP == dim || d < dim)) ? *reinterpret_cast<const v8*>(qp + d * 2) : z;
     }
   }
-  // smallest and largest number of own keys that a row of this wave reads
-  int lim_lo, lim_hi;
-  {
-    const int first = (wave * 32 * p.group_inv) >> 16, last = ((min(wave * 32 + 32, n_rows) - 1) * p.group_inv) >> 16;
-    lim_lo = p.causal ? min(it.klen, it.koff + first + 1) : it.klen;
-    lim_hi = p.causal ? min(it.klen, it.koff + last + 1) : it.klen;
-  }
-
-  f32x16 acc[DB];
 #pragma unroll
   for (int b = 0; b < DB; ++b)
 #pragma unroll
-    for (int r = 0; r < 16; ++r) acc[b][r] = 0.f;
-  float m = -INFINITY, l = 0.f;  // reference (of c s) and this half-lane's part of the sum
-  const float c = p.scale_log2;
+    for (int r = 0; r < 16; ++r) st.acc[b][r] = 0.f;
+  st.m = -INFINITY;
+  st.l = 0.f;
 
-  const Stager<NC, NW, kKeys> stager(wave, lane);
+  const Stager<DP / 8, NW, kKeys> stager(wave, lane);
   const int np = (it.pe - it.pb + kKeys - 1) / kKeys;
   const int nt = np + (it.ke - it.kb + kKeys - 1) / kKeys;
-  auto stage = [&](int t, int buf) {
-    const bool pre = t < np;
-    const int kt = pre ? it.pb + t * kKeys : it.kb + (t - np) * kKeys;
-    const int have = min(kKeys, (pre ? it.pe : it.ke) - kt);
-    const int64_t kts = pre ? p.pk_ts : p.k_ts, vts = pre ? p.pv_ts : p.v_ts;
-    const char* kb = pre ? p.pk + ((int64_t)kt * kts + hk * p.pk_hs) * 2
-                         : p.k + ((int64_t)(it.k0 + kt) * kts + hk * p.k_hs) * 2;
-    const char* vb = pre ? p.pv + ((int64_t)kt * vts + hk * p.pv_hs) * 2
-                         : p.v + ((int64_t)(it.k0 + kt) * vts + hk * p.v_hs) * 2;
-    const int kst = (int)kts * 2, vst = (int)vts * 2;
-    const __amdgpu_buffer_rsrc_t kr = dense::tile_rsrc_u(kb, (uint32_t)((have - 1) * kst + dim * 2));
-    const __amdgpu_buffer_rsrc_t vr = dense::tile_rsrc_u(vb, (uint32_t)((have - 1) * vst + dim * 2));
-    char* tile = smem + buf * 2 * kTile;
-    stager.load(kr, tile, dim, [&](int r) { return min(r, have - 1) * kst; });
-    stager.load(vr, tile + kTile, dim, [&](int r) { return min(r, have - 1) * vst; });
-  };
-
-  if (nt > 0) stage(0, 0);
-  for (int t = 0; t < nt; ++t) {
-    __syncthreads();  // tile t has landed (vmcnt(0)), tile t - 1 is no longer read
-    if (t + 1 < nt) stage(t + 1, (t + 1) & 1);
-    const bool pre = t < np;
-    const int kt = pre ? it.pb + t * kKeys : it.kb + (t - np) * kKeys;
-    const int end = pre ? it.pe : min(it.ke, lim_hi);   // no row of the wave reads from here on
-    if (!wave_live || kt >= end) continue;
-    const char* kt_lds = smem + (t & 1) * 2 * kTile;
-    const char* vt_lds = kt_lds + kTile;
-
-    f32x16 s[2];
-#pragma unroll
-    for (int u = 0; u < 2; ++u)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) s[u][r] = 0.f;
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-      for (int u = 0; u < 2; ++u) s[u] = Elem<T>::mma(row_frag<T, NC>(kt_lds, u * 32 + n, ks, h), qf[ks], s[u]);
-
-    // keys that a row does not read: selected away, whatever their scores are
-    const int stop = pre ? it.pe : it.ke;
-    if (kt + kKeys > stop || (!pre && kt + kKeys > lim_lo)) {
-      const int mine = (pre ? it.pe : min(lim, it.ke)) - kt;
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) s[u][r] = u * 32 + acc_row(r, h) < mine ? s[u][r] : -INFINITY;
-    }
-
-    float top = s[0][0];
-#pragma unroll
-    for (int u = 0; u < 2; ++u)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) top = fmaxf(top, s[u][r]);
-    top = fmaxf(top, other_half(top)) * c;
-    if (__any(top > m + kRaise)) {  // (m = -inf before the first key)
-      const float to = fmaxf(m, top);
-      const float f = to == -INFINITY ? 1.f : ex2(m - to);
-      l *= f;
-#pragma unroll
-      for (int b = 0; b < DB; ++b)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) acc[b][r] *= f;
-      m = to;
-    }
-    const float ref = m == -INFINITY ? 0.f : m;
-    float add = 0.f;
-#pragma unroll
-    for (int u = 0; u < 2; ++u)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        s[u][r] = ex2(fmaf(s[u][r], c, -ref));
-        add += s[u][r];
-      }
-    l += add;
-
-#pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      const v8 pf = acc_frag<T>(s[g >> 1], (g & 1) * 8);
-#pragma unroll
-      for (int b = 0; b < DB; ++b) acc[b] = Elem<T>::mma(col_frag<T, NC>(vt_lds, g * 16, b, lane), pf, acc[b]);
+  if (nt > 0) {
+    fwd_step<T, DP, NW>(smem, smem, st, stager, p, it, hk, -1, np, nt, false, 0, 0, 0, lane);  // the first tile's loads
+    for (int t = 0; t < nt; ++t) {
+      tile_barrier();  // tile t has landed, tile t - 1 is no longer read
+      fwd_step<T, DP, NW>(smem + (t & 1) * 2 * kTile, smem + ((t + 1) & 1) * 2 * kTile, st, stager, p, it, hk, t, np, nt, wave_live, lim,
+                          lim_lo, lim_hi, lane);
     }
   }
 
   if (!live) return;
-  l += other_half(l);
+  const float l = st.l + other_half(st.l);
   const float inv = l == 0.f ? 0.f : 1.f / l;
-  const float lse = l == 0.f ? -INFINITY : m + __log2f(l);
+  const float lse = l == 0.f ? -INFINITY : st.m + __log2f(l);
   if (it.plane >= 0) {
     const int64_t at = ((int64_t)it.plane * p.prows + it.prow + tok) * p.heads + head;
     if (h == 0) p.part_l[at] = lse;
@@ -176,8 +189,8 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_fwd_kernel(Params p) {
       for (int g = 0; g < 4; ++g) {
         const int d = b * 32 + g * 8 + h * 4;
         if (DP == dim || d < dim)
-          *reinterpret_cast<f32x4*>(op + d) = f32x4{acc[b][4 * g] * inv, acc[b][4 * g + 1] * inv,
-                                                    acc[b][4 * g + 2] * inv, acc[b][4 * g + 3] * inv};
+          *reinterpret_cast<f32x4*>(op + d) = f32x4{st.acc[b][4 * g] * inv, st.acc[b][4 * g + 1] * inv,
+                                                    st.acc[b][4 * g + 2] * inv, st.acc[b][4 * g + 3] * inv};
       }
     return;
   }
@@ -189,8 +202,8 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_fwd_kernel(Params p) {
     for (int g = 0; g < 4; ++g) {
       const int d = b * 32 + g * 8 + h * 4;
       if (DP == dim || d < dim)
-        store4<T>(op + d * 2, acc[b][4 * g] * inv, acc[b][4 * g + 1] * inv, acc[b][4 * g + 2] * inv,
-                  acc[b][4 * g + 3] * inv);
+        store4<T>(op + d * 2, st.acc[b][4 * g] * inv, st.acc[b][4 * g + 1] * inv, st.acc[b][4 * g + 2] * inv,
+                  st.acc[b][4 * g + 3] * inv);
     }
 }
 

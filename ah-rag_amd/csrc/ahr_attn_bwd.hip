@@ -12,8 +12,6 @@
 namespace ahr {
 namespace attn {
 
-constexpr int kRowsB = 64;  // query rows of one staged tile
-
 // f16 holds ds only within 2^-24 .. 2^16, and ds of a long row with small gradients lies below it:
 // its accumulators hold ds times a power of two, chosen from the first values so that their largest
 // becomes 2^12 .. 2^13 and lowered (with the accumulators) when later ones pass 2^15. bf16 has fp32's
@@ -45,30 +43,190 @@ __global__ __launch_bounds__(256) void attn_delta_kernel(Params p, int64_t rows)
   if (r < rows && d == 0) p.delta[r] = x;
 }
 
-// dk, dv of NW * 32 keys of one key head
-template <typename T, int DP, int NW>
-__global__ __launch_bounds__(NW * 64, DP > 64 ? 1 : 2) void attn_dkv_kernel(Params p) {
+// f16: ds of the tile times the state's factor, which is chosen and lowered here (ROW: one factor for each
+// row, held by its lane; else one for the wave). acc: the accumulators that hold ds already.
+template <int DB, bool ROW>
+__device__ __forceinline__ void scale_ds(f32x16& g, f32x16 (&acc)[DB], float& sc) {
+  float most = 0.f;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) most = fmaxf(most, fabsf(g[r]));
+  if (ROW) most = fmaxf(most, other_half(most));
+  bool grow = (most * sc > kWide || (sc == 0.f && most > 0.f)) && most < INFINITY;
+  if (__any(grow)) {
+    if (!ROW) {
+      most = most < INFINITY ? most : 0.f;
+#pragma unroll
+      for (int x = 1; x < 64; x *= 2) most = fmaxf(most, __shfl_xor(most, x, 64));
+      grow = true;
+    }
+    const float to = grow ? pick_scale(most) : sc, f = grow && sc != 0.f ? to / sc : 1.f;
+#pragma unroll
+    for (int b = 0; b < DB; ++b)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[b][r] *= f;
+    sc = to;
+  }
+  const float mul = sc == 0.f ? 1.f : sc;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) g[r] *= mul;
+}
+
+// ---- dk, dv ------------------------------------------------------------------------------------
+
+// A wave's 32 keys: their rows of k and v, and the transposed sums.
+template <typename T, int DP>
+struct KeyState {
+  typename Elem<T>::v8 kf[DP / 16], vf[DP / 16];
+  f32x16 gk[DP / 32], gv[DP / 32];
+  float sc;  // factor of ds in gk (0: none chosen yet)
+};
+
+// 32 query rows (from row u0 of the staged tiles) against the wave's keys. have: rows of the tile that
+// exist; reads(x): whether row x of the tile reads this lane's key, asked only if `cut`.
+template <typename T, int DP, typename F>
+__device__ __forceinline__ void key_tile(const char* __restrict__ q_lds, const char* __restrict__ o_lds, const float* __restrict__ f, int rows,
+                                         KeyState<T, DP>& st, int u0, bool cut, F reads, float c, int lane) {
   typedef typename Elem<T>::v8 v8;
   constexpr int NC = DP / 8, KS = DP / 16, DB = DP / 32;
-  constexpr int kTile = kRowsB * DP * 2;
-  constexpr int kBuf = 2 * kTile + 2 * kRowsB * 4;  // q tile, do tile, lse, delta
+  const int h = lane >> 5, n = lane & 31;
+  f32x16 s, g;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) s[r] = g[r] = 0.f;
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks) s = Elem<T>::mma(row_frag<T, NC>(q_lds, u0 + n, ks, h), st.kf[ks], s);
+#pragma unroll
+  for (int ks = 0; ks < KS; ++ks) g = Elem<T>::mma(row_frag<T, NC>(o_lds, u0 + n, ks, h), st.vf[ks], g);
+#pragma unroll
+  for (int r4 = 0; r4 < 4; ++r4) {
+    const f32x4 ls = *reinterpret_cast<const f32x4*>(f + u0 + r4 * 8 + h * 4);
+    const f32x4 de = *reinterpret_cast<const f32x4*>(f + rows + u0 + r4 * 8 + h * 4);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = r4 * 4 + i;
+      s[r] = ex2(fmaf(s[r], c, -ls[i]));
+      g[r] = s[r] * (g[r] - de[i]);
+    }
+  }
+  if (cut) {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const bool in = reads(u0 + acc_row(r, h));
+      s[r] = in ? s[r] : 0.f;
+      g[r] = in ? g[r] : 0.f;
+    }
+  }
+  if constexpr (Elem<T>::kNarrow) {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s[r] *= 0x1p14f;
+    scale_ds<DB, false>(g, st.gk, st.sc);
+  }
+#pragma unroll
+  for (int k2 = 0; k2 < 2; ++k2) {
+    const v8 pf = acc_frag<T>(s, k2 * 8), df = acc_frag<T>(g, k2 * 8);
+#pragma unroll
+    for (int b = 0; b < DB; ++b) {
+      st.gv[b] = Elem<T>::mma(col_frag<T, NC>(o_lds, u0 + k2 * 16, b, lane), pf, st.gv[b]);
+      st.gk[b] = Elem<T>::mma(col_frag<T, NC>(q_lds, u0 + k2 * 16, b, lane), df, st.gk[b]);
+    }
+  }
+}
+
+// The query rows of an item, tile by tile.
+struct KeyWalk {
+  int G, ginv, coff, n_tok;
+  int64_t n_rows;
+};
+
+template <typename T, int DP, int RW>
+struct KeyCfg {
+  static constexpr int kRows = RW == 4 ? 128 : 64;      // query rows of a staged tile
+  static constexpr int kTile = kRows * DP * 2;
+  static constexpr int kBuf = 2 * kTile + 2 * kRows * 4;  // q tile, do tile, lse, delta
+  static constexpr int kPer = kRows / 32 / RW;            // 32-row parts of a tile for each wave
+};
+
+template <typename T, int DP, int KW, int RW>
+__device__ __forceinline__ void key_step(const char* __restrict__ cur, char* __restrict__ nxt, KeyState<T, DP>& st,
+                                         const Stager<DP / 8, KW * RW, KeyCfg<T, DP, RW>::kRows>& stager, const Params& p, const KeyItem& it,
+                                         const KeyWalk& w, int hk, int t, int nt, bool wave_live, int rw, int j, int j_hi, int lane) {
+  typedef KeyCfg<T, DP, RW> Cfg;
+  const int G = w.G;
+  float st_l = 0.f, st_d = 0.f;  // lse and delta of the next tile's row, on their way to LDS
+  if (t + 1 < nt) {
+    const int64_t r0 = (int64_t)(t + 1) * Cfg::kRows;
+    const int tok0 = (int)(r0 / G), g0 = (int)(r0 - (int64_t)tok0 * G);
+    const int have = (int)min((int64_t)Cfg::kRows, w.n_rows - r0);
+    const int64_t at = it.q0 + it.t0 + tok0;
+    const int qts = (int)p.q_ts * 2, qhs = (int)p.q_hs * 2, ots = (int)p.do_ts * 2, ohs = (int)p.do_hs * 2;
+    const uint32_t span = (uint32_t)((g0 + have - 1) / G);  // tokens past the first
+    const __amdgpu_buffer_rsrc_t qr =
+        dense::tile_rsrc_u(p.q + (at * p.q_ts + (int64_t)hk * G * p.q_hs) * 2, span * qts + (G - 1) * qhs + p.dim * 2);
+    const __amdgpu_buffer_rsrc_t dr =
+        dense::tile_rsrc_u(p.d_o + (at * p.do_ts + (int64_t)hk * G * p.do_hs) * 2, span * ots + (G - 1) * ohs + p.dim * 2);
+    auto off = [&](int r, int ts, int hs) {
+      const int x = g0 + min(r, have - 1);
+      const int tk = (x * w.ginv) >> 16;
+      return tk * ts + (x - tk * G) * hs;
+    };
+    stager.load(qr, nxt, p.dim, [&](int r) { return off(r, qts, qhs); });
+    stager.load(dr, nxt + Cfg::kTile, p.dim, [&](int r) { return off(r, ots, ohs); });
+    if (threadIdx.x < Cfg::kRows) {
+      const int r = threadIdx.x, x = g0 + min(r, have - 1), tk = (x * w.ginv) >> 16;
+      const int64_t i = (at + tk) * p.heads + hk * G + (x - tk * G);
+      st_l = p.lse[i];
+      st_d = p.delta[i];
+    }
+  }
+  if (t >= 0 && wave_live) {
+    const int64_t r0 = (int64_t)t * Cfg::kRows;
+    const int tok0 = (int)(r0 / G), g0 = (int)(r0 - (int64_t)tok0 * G);
+    const int have = (int)min((int64_t)Cfg::kRows, w.n_rows - r0);
+    const float* f = reinterpret_cast<const float*>(cur + 2 * Cfg::kTile);
+#pragma unroll
+    for (int u = 0; u < Cfg::kPer; ++u) {
+      const int u0 = (rw * Cfg::kPer + u) * 32;
+      if (u0 >= have) break;
+      // a row reads keys j <= coff + its token; the rows' tokens rise
+      const int tok_lo = it.t0 + tok0 + (((g0 + u0) * w.ginv) >> 16);
+      const bool cut = u0 + 32 > have || (p.causal && j_hi > w.coff + tok_lo);
+      key_tile<T, DP>(cur, cur + Cfg::kTile, f, Cfg::kRows, st, u0, cut,
+                      [&](int x) { return x < have && (!p.causal || j <= w.coff + it.t0 + tok0 + (((g0 + x) * w.ginv) >> 16)); },
+                      p.scale_log2, lane);
+    }
+  }
+  if (t + 1 < nt && threadIdx.x < Cfg::kRows) {
+    float* f = reinterpret_cast<float*>(nxt + 2 * Cfg::kTile);
+    f[threadIdx.x] = st_l;
+    f[Cfg::kRows + threadIdx.x] = st_d;
+  }
+}
+
+// dk, dv of KW * 32 keys of one key head. RW groups of waves take different rows of each staged tile and
+// are added through LDS at the end, in order: where there are few key tiles (or causal ones of very
+// different length) that shortens the longest workgroup without partial sums in memory.
+template <typename T, int DP, int KW, int RW>
+__global__ __launch_bounds__(KW * RW * 64, DP > 64 || RW == 4 ? 1 : 2) void attn_dkv_kernel(Params p) {
+  typedef typename Elem<T>::v8 v8;
+  typedef KeyCfg<T, DP, RW> Cfg;
+  constexpr int KS = DP / 16, DB = DP / 32, NW = KW * RW;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int lane = threadIdx.x & 63, h = lane >> 5, n = lane & 31;
   const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  const int kw = wave % KW, rw = wave / KW;
   const int hk = blockIdx.x % p.kv_heads;
   const KeyItem it = p.keys[blockIdx.x / p.kv_heads];
   const int dim = p.dim;
 
   if (DP != dim) {
     for (int b = 0; b < 2; ++b)
-      for (int i = threadIdx.x; i < 2 * kTile / 16; i += NW * 64)
-        reinterpret_cast<f32x4*>(smem + b * kBuf)[i] = f32x4{0, 0, 0, 0};
+      for (int i = threadIdx.x; i < 2 * Cfg::kTile / 16; i += NW * 64)
+        reinterpret_cast<f32x4*>(smem + b * Cfg::kBuf)[i] = f32x4{0, 0, 0, 0};
     __syncthreads();
   }
 
-  const int key = wave * 32 + n;
+  const int key = kw * 32 + n;
   const bool live = key < it.nk;
-  v8 kf[KS], vf[KS];
+  KeyState<T, DP> st;
   {
     const int64_t at = it.k0 + (live ? key : 0);
     const char* kp = p.k + (at * p.k_ts + (int64_t)hk * p.k_hs) * 2;
@@ -78,143 +236,70 @@ __global__ __launch_bounds__(NW * 64, DP > 64 ? 1 : 2) void attn_dkv_kernel(Para
       const int d = (2 * ks + h) * 8;
       const v8 z = {};
       const bool in = live && (DP == dim || d < dim);
-      kf[ks] = in ? *reinterpret_cast<const v8*>(kp + d * 2) : z;
-      vf[ks] = in ? *reinterpret_cast<const v8*>(vp + d * 2) : z;
+      st.kf[ks] = in ? *reinterpret_cast<const v8*>(kp + d * 2) : z;
+      st.vf[ks] = in ? *reinterpret_cast<const v8*>(vp + d * 2) : z;
     }
   }
-  f32x16 gk[DB], gv[DB];
 #pragma unroll
   for (int b = 0; b < DB; ++b)
 #pragma unroll
-    for (int r = 0; r < 16; ++r) gk[b][r] = gv[b][r] = 0.f;
+    for (int r = 0; r < 16; ++r) st.gk[b][r] = st.gv[b][r] = 0.f;
+  st.sc = Elem<T>::kNarrow ? 0.f : 1.f;
 
-  const Stager<NC, NW, kRowsB> stager(wave, lane);
-  const int G = p.group;
-  const int coff = it.klen - it.qlen;
-  const int n_tok = it.qlen - it.t0;              // query tokens that matter
-  const int64_t n_rows = (int64_t)n_tok * G;      // and their rows
-  const int nt = (int)((n_rows + kRowsB - 1) / kRowsB);
-  float st_l = 0.f, st_d = 0.f;  // lse and delta of the next tile's row, on their way to LDS
-  auto stage = [&](int t, int buf) {
-    const int64_t r0 = (int64_t)t * kRowsB;
-    const int tok0 = (int)(r0 / G), g0 = (int)(r0 - (int64_t)tok0 * G);
-    const int have = (int)min((int64_t)kRowsB, n_rows - r0);
-    const int64_t at = it.q0 + it.t0 + tok0;
-    const int qts = (int)p.q_ts * 2, qhs = (int)p.q_hs * 2, ots = (int)p.do_ts * 2, ohs = (int)p.do_hs * 2;
-    const uint32_t span = (uint32_t)((g0 + have - 1) / G);  // tokens past the first
-    const __amdgpu_buffer_rsrc_t qr = dense::tile_rsrc_u(p.q + (at * p.q_ts + (int64_t)hk * G * p.q_hs) * 2,
-                                                         span * qts + (G - 1) * qhs + dim * 2);
-    const __amdgpu_buffer_rsrc_t dr = dense::tile_rsrc_u(p.d_o + (at * p.do_ts + (int64_t)hk * G * p.do_hs) * 2,
-                                                         span * ots + (G - 1) * ohs + dim * 2);
-    char* tile = smem + buf * kBuf;
-    auto off = [&](int r, int ts, int hs) {
-      const int x = g0 + min(r, have - 1);
-      const int tk = (x * p.group_inv) >> 16;
-      return tk * ts + (x - tk * G) * hs;
-    };
-    stager.load(qr, tile, dim, [&](int r) { return off(r, qts, qhs); });
-    stager.load(dr, tile + kTile, dim, [&](int r) { return off(r, ots, ohs); });
-    if (threadIdx.x < kRowsB) {
-      const int r = threadIdx.x, x = g0 + min(r, have - 1), tk = (x * p.group_inv) >> 16;
-      const int64_t i = (at + tk) * p.heads + hk * G + (x - tk * G);
-      st_l = p.lse[i];
-      st_d = p.delta[i];
-    }
-  };
-  auto land = [&](int buf) {
-    float* f = reinterpret_cast<float*>(smem + buf * kBuf + 2 * kTile);
-    if (threadIdx.x < kRowsB) {
-      f[threadIdx.x] = st_l;
-      f[kRowsB + threadIdx.x] = st_d;
-    }
-  };
-
-  const bool wave_live = wave * 32 < it.nk;
-  const int j = it.kpos + key;                               // this lane's key in its sequence
-  const int j_hi = it.kpos + min(wave * 32 + 31, it.nk - 1);  // the wave's last
-  const float c = p.scale_log2;
-  float sc = Elem<T>::kNarrow ? 0.f : 1.f;  // factor of ds in gk (0: none chosen yet)
+  const Stager<DP / 8, NW, Cfg::kRows> stager(wave, lane);
+  KeyWalk w;
+  w.G = p.group;
+  w.ginv = p.group_inv;
+  w.coff = it.klen - it.qlen;
+  w.n_tok = it.qlen - it.t0;              // query tokens that matter
+  w.n_rows = (int64_t)w.n_tok * p.group;  // and their rows
+  const int nt = (int)((w.n_rows + Cfg::kRows - 1) / Cfg::kRows);
+  const bool wave_live = kw * 32 < it.nk;
+  const int j = it.kpos + key;                             // this lane's key in its sequence
+  const int j_hi = it.kpos + min(kw * 32 + 31, it.nk - 1);  // the wave's last
   if (nt > 0) {
-    stage(0, 0);
-    land(0);
+    key_step<T, DP, KW, RW>(smem, smem, st, stager, p, it, w, hk, -1, nt, false, rw, j, j_hi, lane);
+    for (int t = 0; t < nt; ++t) {
+      tile_barrier();
+      key_step<T, DP, KW, RW>(smem + (t & 1) * Cfg::kBuf, smem + ((t + 1) & 1) * Cfg::kBuf, st, stager, p, it, w, hk, t, nt, wave_live, rw, j,
+                              j_hi, lane);
+    }
   }
-  for (int t = 0; t < nt; ++t) {
-    __syncthreads();
-    if (t + 1 < nt) stage(t + 1, (t + 1) & 1);
-    const int64_t r0 = (int64_t)t * kRowsB;
-    const int tok0 = (int)(r0 / G), g0 = (int)(r0 - (int64_t)tok0 * G);
-    const int have = (int)min((int64_t)kRowsB, n_rows - r0);
-    const char* q_lds = smem + (t & 1) * kBuf;
-    const char* o_lds = q_lds + kTile;
-    const float* f = reinterpret_cast<const float*>(o_lds + kTile);
-    if (wave_live) {
+  float k_out = p.scale / (st.sc == 0.f ? 1.f : st.sc);
+  const float v_out = Elem<T>::kNarrow ? 0x1p-14f : 1.f;
+  if constexpr (RW > 1) {
+    float* sum = reinterpret_cast<float*>(smem);  // [kw][register][lane], one group of waves at a time
 #pragma unroll
-      for (int u = 0; u < kRowsB / 32; ++u) {
-        if (u * 32 >= have) break;
-        f32x16 s, g;
+    for (int b = 0; b < DB; ++b)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[r] = g[r] = 0.f;
+      for (int r = 0; r < 16; ++r) st.gk[b][r] *= k_out;
+    k_out = 1.f;
+    for (int o = 1; o < RW; ++o) {
+      __syncthreads();
+      float* at = sum + kw * (2 * DB * 16 * 64) + lane;
+      if (rw == o) {
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) s = Elem<T>::mma(row_frag<T, NC>(q_lds, u * 32 + n, ks, h), kf[ks], s);
+        for (int b = 0; b < DB; ++b)
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) g = Elem<T>::mma(row_frag<T, NC>(o_lds, u * 32 + n, ks, h), vf[ks], g);
-        // a row reads keys j <= coff + its token; the rows' tokens rise
-        const int tok_lo = it.t0 + tok0 + (((g0 + u * 32) * p.group_inv) >> 16);
-        const bool cut = u * 32 + 32 > have || (p.causal && j_hi > coff + tok_lo);
-#pragma unroll
-        for (int r4 = 0; r4 < 4; ++r4) {
-          const f32x4 ls = *reinterpret_cast<const f32x4*>(f + u * 32 + r4 * 8 + h * 4);
-          const f32x4 de = *reinterpret_cast<const f32x4*>(f + kRowsB + u * 32 + r4 * 8 + h * 4);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int r = r4 * 4 + i;
-            float pr = ex2(fmaf(s[r], c, -ls[i]));
-            float ds = pr * (g[r] - de[i]);
-            if (cut) {
-              const int x = u * 32 + r4 * 8 + h * 4 + i;
-              const int tok = it.t0 + tok0 + (((g0 + x) * p.group_inv) >> 16);
-              const bool reads = x < have && (!p.causal || j <= coff + tok);
-              pr = reads ? pr : 0.f;
-              ds = reads ? ds : 0.f;
-            }
-            s[r] = Elem<T>::kNarrow ? pr * 0x1p14f : pr;
-            g[r] = ds;
+          for (int r = 0; r < 16; ++r) {
+            at[(b * 16 + r) * 64] = st.gk[b][r];
+            at[(DB * 16 + b * 16 + r) * 64] = st.gv[b][r];
           }
-        }
-        if constexpr (Elem<T>::kNarrow) {  // one factor for the wave: dk sums over its rows
-          float most = 0.f;
+      }
+      __syncthreads();
+      if (rw == 0) {
 #pragma unroll
-          for (int r = 0; r < 16; ++r) most = fmaxf(most, fabsf(g[r]));
-          if (__any((most * sc > kWide || (sc == 0.f && most > 0.f)) && most < INFINITY)) {
-            most = most < INFINITY ? most : 0.f;
+        for (int b = 0; b < DB; ++b)
 #pragma unroll
-            for (int x = 1; x < 64; x *= 2) most = fmaxf(most, __shfl_xor(most, x, 64));
-            const float to = pick_scale(most), f2 = sc == 0.f ? 1.f : to / sc;
-#pragma unroll
-            for (int b = 0; b < DB; ++b)
-#pragma unroll
-              for (int r = 0; r < 16; ++r) gk[b][r] *= f2;
-            sc = to;
+          for (int r = 0; r < 16; ++r) {
+            st.gk[b][r] += at[(b * 16 + r) * 64];
+            st.gv[b][r] += at[(DB * 16 + b * 16 + r) * 64];
           }
-          const float mul = sc == 0.f ? 1.f : sc;
-#pragma unroll
-          for (int r = 0; r < 16; ++r) g[r] *= mul;
-        }
-#pragma unroll
-        for (int k2 = 0; k2 < 2; ++k2) {
-          const v8 pf = acc_frag<T>(s, k2 * 8), df = acc_frag<T>(g, k2 * 8);
-#pragma unroll
-          for (int b = 0; b < DB; ++b) {
-            gv[b] = Elem<T>::mma(col_frag<T, NC>(o_lds, u * 32 + k2 * 16, b, lane), pf, gv[b]);
-            gk[b] = Elem<T>::mma(col_frag<T, NC>(q_lds, u * 32 + k2 * 16, b, lane), df, gk[b]);
-          }
-        }
       }
     }
-    if (t + 1 < nt) land((t + 1) & 1);
+    if (rw != 0) return;
   }
   if (!live) return;
-  const float k_out = p.scale / (sc == 0.f ? 1.f : sc), v_out = Elem<T>::kNarrow ? 0x1p-14f : 1.f;
   char* kp = p.dk + ((int64_t)(it.k0 + key) * p.dk_ts + (int64_t)hk * p.dk_hs) * 2;
   char* vp = p.dv + ((int64_t)(it.k0 + key) * p.dv_ts + (int64_t)hk * p.dv_hs) * 2;
 #pragma unroll
@@ -223,17 +308,75 @@ __global__ __launch_bounds__(NW * 64, DP > 64 ? 1 : 2) void attn_dkv_kernel(Para
     for (int x = 0; x < 4; ++x) {
       const int d = b * 32 + x * 8 + h * 4;
       if (DP == dim || d < dim) {
-        store4<T>(kp + d * 2, gk[b][4 * x] * k_out, gk[b][4 * x + 1] * k_out, gk[b][4 * x + 2] * k_out, gk[b][4 * x + 3] * k_out);
-        store4<T>(vp + d * 2, gv[b][4 * x] * v_out, gv[b][4 * x + 1] * v_out, gv[b][4 * x + 2] * v_out, gv[b][4 * x + 3] * v_out);
+        const f32x16 &a = st.gk[b], &e = st.gv[b];
+        store4<T>(kp + d * 2, a[4 * x] * k_out, a[4 * x + 1] * k_out, a[4 * x + 2] * k_out, a[4 * x + 3] * k_out);
+        store4<T>(vp + d * 2, e[4 * x] * v_out, e[4 * x + 1] * v_out, e[4 * x + 2] * v_out, e[4 * x + 3] * v_out);
       }
     }
 }
 
-// dq of the rows of one item (32 rows a wave), transposed as in the forward pass
+// ---- dq ----------------------------------------------------------------------------------------
+
+template <typename T, int DP>
+struct RowState {
+  typename Elem<T>::v8 qf[DP / 16], of[DP / 16];
+  f32x16 acc[DP / 32];
+  float lse, delta, sc;
+};
+
+// One staged tile of keys and values for one wave's rows, transposed as in the forward pass.
+template <typename T, int DP>
+__device__ __forceinline__ void row_tile(const char* __restrict__ cur, RowState<T, DP>& st, bool cut, int mine, float c, int lane) {
+  typedef typename Elem<T>::v8 v8;
+  constexpr int NC = DP / 8, KS = DP / 16, DB = DP / 32;
+  constexpr int kTile = kKeys * DP * 2;
+  const int h = lane >> 5, n = lane & 31;
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    f32x16 s, g;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s[r] = g[r] = 0.f;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) s = Elem<T>::mma(row_frag<T, NC>(cur, u * 32 + n, ks, h), st.qf[ks], s);
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) g = Elem<T>::mma(row_frag<T, NC>(cur + kTile, u * 32 + n, ks, h), st.of[ks], g);
+#pragma unroll
+    for (int r = 0; r < 16; ++r) g[r] = ex2(fmaf(s[r], c, -st.lse)) * (g[r] - st.delta);
+    if (cut) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) g[r] = u * 32 + acc_row(r, h) < mine ? g[r] : 0.f;
+    }
+    if constexpr (Elem<T>::kNarrow) scale_ds<DB, true>(g, st.acc, st.sc);
+#pragma unroll
+    for (int k2 = 0; k2 < 2; ++k2) {
+      const v8 df = acc_frag<T>(g, k2 * 8);
+#pragma unroll
+      for (int b = 0; b < DB; ++b) st.acc[b] = Elem<T>::mma(col_frag<T, NC>(cur, u * 32 + k2 * 16, b, lane), df, st.acc[b]);
+    }
+  }
+}
+
+template <typename T, int DP, int NW>
+__device__ __forceinline__ void row_step(const char* __restrict__ cur, char* __restrict__ nxt, RowState<T, DP>& st,
+                                         const Stager<DP / 8, NW, kKeys>& stager, const Params& p, const RowItem& it, int hk, int t, int nt,
+                                         bool wave_live, int lim, int lim_lo, int lim_hi, int lane) {
+  if (t + 1 < nt) {
+    const int kt = (t + 1) * kKeys;
+    const int64_t at = (int64_t)it.k0 + kt;
+    stage_kv<DP, NW>(nxt, stager, p.k + (at * p.k_ts + (int64_t)hk * p.k_hs) * 2, p.v + (at * p.v_ts + (int64_t)hk * p.v_hs) * 2, p.k_ts, p.v_ts,
+                     min(kKeys, it.ke - kt), p.dim);
+  }
+  if (t < 0) return;
+  const int kt = t * kKeys;
+  if (!wave_live || kt >= lim_hi) return;
+  row_tile<T, DP>(cur, st, kt + kKeys > it.ke || kt + kKeys > lim_lo, min(lim, it.ke) - kt, p.scale_log2, lane);
+}
+
+// dq of the rows of one item, 32 a wave
 template <typename T, int DP, int NW>
 __global__ __launch_bounds__(NW * 64, 2) void attn_dq_kernel(Params p) {
   typedef typename Elem<T>::v8 v8;
-  constexpr int NC = DP / 8, KS = DP / 16, DB = DP / 32;
+  constexpr int KS = DP / 16, DB = DP / 32;
   constexpr int kTile = kKeys * DP * 2;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int lane = threadIdx.x & 63, h = lane >> 5, n = lane & 31;
@@ -252,7 +395,10 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_dq_kernel(Params p) {
   const int head = hk * p.group + (live ? row - tok * p.group : 0);
   const int lim = live ? (p.causal ? min(it.klen, it.koff + tok + 1) : it.klen) : 0;
   const bool wave_live = wave * 32 < n_rows;
-  v8 qf[KS], of[KS];
+  const int first = (wave * 32 * p.group_inv) >> 16, last = ((min(wave * 32 + 32, n_rows) - 1) * p.group_inv) >> 16;
+  const int lim_lo = p.causal ? min(it.klen, it.koff + first + 1) : it.klen;
+  const int lim_hi = p.causal ? min(it.klen, it.koff + last + 1) : it.klen;
+  RowState<T, DP> st;
   {
     const char* qp = p.q + ((int64_t)(it.q0 + tok) * p.q_ts + (int64_t)head * p.q_hs) * 2;
     const char* op = p.d_o + ((int64_t)(it.q0 + tok) * p.do_ts + (int64_t)head * p.do_hs) * 2;
@@ -261,110 +407,52 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_dq_kernel(Params p) {
       const int d = (2 * ks + h) * 8;
       const v8 z = {};
       const bool in = live && (DP == dim || d < dim);
-      qf[ks] = in ? *reinterpret_cast<const v8*>(qp + d * 2) : z;
-      of[ks] = in ? *reinterpret_cast<const v8*>(op + d * 2) : z;
+      st.qf[ks] = in ? *reinterpret_cast<const v8*>(qp + d * 2) : z;
+      st.of[ks] = in ? *reinterpret_cast<const v8*>(op + d * 2) : z;
     }
   }
   const int64_t li = (int64_t)(it.q0 + tok) * p.heads + head;
-  const float lse = live ? p.lse[li] : 0.f, delta = live ? p.delta[li] : 0.f;
-  int lim_lo, lim_hi;
-  {
-    const int first = (wave * 32 * p.group_inv) >> 16, last = ((min(wave * 32 + 32, n_rows) - 1) * p.group_inv) >> 16;
-    lim_lo = p.causal ? min(it.klen, it.koff + first + 1) : it.klen;
-    lim_hi = p.causal ? min(it.klen, it.koff + last + 1) : it.klen;
-  }
-  f32x16 acc[DB];
+  st.lse = live ? p.lse[li] : 0.f;
+  st.delta = live ? p.delta[li] : 0.f;
+  st.sc = Elem<T>::kNarrow ? 0.f : 1.f;
 #pragma unroll
   for (int b = 0; b < DB; ++b)
 #pragma unroll
-    for (int r = 0; r < 16; ++r) acc[b][r] = 0.f;
-  const float c = p.scale_log2;
-  float sc = Elem<T>::kNarrow ? 0.f : 1.f;  // factor of ds in acc, one for each row (0: none chosen yet)
+    for (int r = 0; r < 16; ++r) st.acc[b][r] = 0.f;
 
-  const Stager<NC, NW, kKeys> stager(wave, lane);
+  const Stager<DP / 8, NW, kKeys> stager(wave, lane);
   const int nt = (it.ke + kKeys - 1) / kKeys;
-  auto stage = [&](int t, int buf) {
-    const int kt = t * kKeys, have = min(kKeys, it.ke - kt);
-    const int kst = (int)p.k_ts * 2, vst = (int)p.v_ts * 2;
-    const __amdgpu_buffer_rsrc_t kr = dense::tile_rsrc_u(p.k + ((int64_t)(it.k0 + kt) * p.k_ts + (int64_t)hk * p.k_hs) * 2,
-                                                         (uint32_t)((have - 1) * kst + dim * 2));
-    const __amdgpu_buffer_rsrc_t vr = dense::tile_rsrc_u(p.v + ((int64_t)(it.k0 + kt) * p.v_ts + (int64_t)hk * p.v_hs) * 2,
-                                                         (uint32_t)((have - 1) * vst + dim * 2));
-    char* tile = smem + buf * 2 * kTile;
-    stager.load(kr, tile, dim, [&](int r) { return min(r, have - 1) * kst; });
-    stager.load(vr, tile + kTile, dim, [&](int r) { return min(r, have - 1) * vst; });
-  };
-  if (nt > 0) stage(0, 0);
-  for (int t = 0; t < nt; ++t) {
-    __syncthreads();
-    if (t + 1 < nt) stage(t + 1, (t + 1) & 1);
-    const int kt = t * kKeys;
-    if (!wave_live || kt >= min(it.ke, lim_hi)) continue;
-    const char* kt_lds = smem + (t & 1) * 2 * kTile;
-    const char* vt_lds = kt_lds + kTile;
-    const bool cut = kt + kKeys > it.ke || kt + kKeys > lim_lo;
-    const int mine = min(lim, it.ke) - kt;
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      f32x16 s, g;
-#pragma unroll
-      for (int r = 0; r < 16; ++r) s[r] = g[r] = 0.f;
-#pragma unroll
-      for (int ks = 0; ks < KS; ++ks) s = Elem<T>::mma(row_frag<T, NC>(kt_lds, u * 32 + n, ks, h), qf[ks], s);
-#pragma unroll
-      for (int ks = 0; ks < KS; ++ks) g = Elem<T>::mma(row_frag<T, NC>(vt_lds, u * 32 + n, ks, h), of[ks], g);
-#pragma unroll
-      for (int r = 0; r < 16; ++r) g[r] = ex2(fmaf(s[r], c, -lse)) * (g[r] - delta);
-      if (cut) {
-#pragma unroll
-        for (int r = 0; r < 16; ++r) g[r] = u * 32 + acc_row(r, h) < mine ? g[r] : 0.f;
-      }
-      if constexpr (Elem<T>::kNarrow) {
-        float most = 0.f;
-#pragma unroll
-        for (int r = 0; r < 16; ++r) most = fmaxf(most, fabsf(g[r]));
-        most = fmaxf(most, other_half(most));
-        const bool grow = (most * sc > kWide || (sc == 0.f && most > 0.f)) && most < INFINITY;
-        if (__any(grow)) {
-          const float to = grow ? pick_scale(most) : sc, f2 = grow && sc != 0.f ? to / sc : 1.f;
-#pragma unroll
-          for (int b = 0; b < DB; ++b)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) acc[b][r] *= f2;
-          sc = to;
-        }
-        const float mul = sc == 0.f ? 1.f : sc;
-#pragma unroll
-        for (int r = 0; r < 16; ++r) g[r] *= mul;
-      }
-#pragma unroll
-      for (int k2 = 0; k2 < 2; ++k2) {
-        const v8 df = acc_frag<T>(g, k2 * 8);
-#pragma unroll
-        for (int b = 0; b < DB; ++b)
-          acc[b] = Elem<T>::mma(col_frag<T, NC>(kt_lds, u * 32 + k2 * 16, b, lane), df, acc[b]);
-      }
+  if (nt > 0) {
+    row_step<T, DP, NW>(smem, smem, st, stager, p, it, hk, -1, nt, false, 0, 0, 0, lane);
+    for (int t = 0; t < nt; ++t) {
+      tile_barrier();
+      row_step<T, DP, NW>(smem + (t & 1) * 2 * kTile, smem + ((t + 1) & 1) * 2 * kTile, st, stager, p, it, hk, t, nt, wave_live, lim, lim_lo,
+                          lim_hi, lane);
     }
   }
   if (!live) return;
-  const float q_out = p.scale / (sc == 0.f ? 1.f : sc);
+  const float q_out = p.scale / (st.sc == 0.f ? 1.f : st.sc);
   char* qp = p.dq + ((int64_t)(it.q0 + tok) * p.dq_ts + (int64_t)head * p.dq_hs) * 2;
 #pragma unroll
   for (int b = 0; b < DB; ++b)
 #pragma unroll
     for (int x = 0; x < 4; ++x) {
       const int d = b * 32 + x * 8 + h * 4;
-      if (DP == dim || d < dim)
-        store4<T>(qp + d * 2, acc[b][4 * x] * q_out, acc[b][4 * x + 1] * q_out, acc[b][4 * x + 2] * q_out, acc[b][4 * x + 3] * q_out);
+      if (DP == dim || d < dim) {
+        const f32x16& a = st.acc[b];
+        store4<T>(qp + d * 2, a[4 * x] * q_out, a[4 * x + 1] * q_out, a[4 * x + 2] * q_out, a[4 * x + 3] * q_out);
+      }
     }
 }
 
-template <typename T, int DP, int NW>
+template <typename T, int DP, int KW, int RW>
 static int launch_dkv(const Params& p, hipStream_t s) {
-  constexpr int lds = 2 * (2 * kRowsB * DP * 2 + 2 * kRowsB * 4);
+  constexpr int tiles = 2 * KeyCfg<T, DP, RW>::kBuf, sums = RW > 1 ? KW * DP * 32 * 2 * 4 : 0;
+  constexpr int lds = tiles > sums ? tiles : sums;
+  static_assert(lds <= 160 * 1024, "LDS of one workgroup");
   static std::atomic<uint64_t> done{0};
-  ensure_lds_attr(done, reinterpret_cast<const void*>(attn_dkv_kernel<T, DP, NW>), lds);
-  attn_dkv_kernel<T, DP, NW><<<dim3((unsigned)(p.n_keys * p.kv_heads)), NW * 64, lds, s>>>(p);
+  ensure_lds_attr(done, reinterpret_cast<const void*>(attn_dkv_kernel<T, DP, KW, RW>), lds);
+  attn_dkv_kernel<T, DP, KW, RW><<<dim3((unsigned)(p.n_keys * p.kv_heads)), KW * RW * 64, lds, s>>>(p);
   AHR_HIP(hipGetLastError());
   return AHR_OK;
 }
@@ -383,9 +471,9 @@ template <typename T, int DP>
 static int launch_bwd_d(const ahr_attn_plan& pl, const Params& p, hipStream_t s) {
   int st = AHR_OK;
   if (p.n_keys) {
-    if (pl.key_waves == 1) st = launch_dkv<T, DP, 1>(p, s);
-    else if (pl.key_waves == 2) st = launch_dkv<T, DP, 2>(p, s);
-    else st = launch_dkv<T, DP, 4>(p, s);
+    if (pl.key_waves == 1) st = launch_dkv<T, DP, 1, 4>(p, s);
+    else if (pl.key_waves == 2) st = launch_dkv<T, DP, 2, 2>(p, s);
+    else st = launch_dkv<T, DP, 4, 1>(p, s);
     if (st != AHR_OK) return st;
   }
   if (p.n_rows) {

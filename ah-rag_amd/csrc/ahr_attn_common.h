@@ -83,6 +83,15 @@ __device__ __forceinline__ typename Elem<T>::v8 acc_frag(const f32x16& x, int o)
   return f;
 }
 
+// Before a tile that LDS-DMA fills is read: this wave's loads have landed, then every wave's (the
+// compiler's own barrier does not wait for LDS-DMA). All waves of the workgroup pass here once per tile,
+// whether or not they have work in it.
+__device__ __forceinline__ void tile_barrier() {
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
 // row of a 32x32 accumulator register r in lane half h
 __device__ __forceinline__ int acc_row(int r, int h) { return (r & 3) + 8 * (r >> 2) + 4 * h; }
 
@@ -110,15 +119,32 @@ struct Stager {
   // valid one: every load stays inside the tensors). Chunks past dim are left alone (zeroed once).
   template <typename F>
   __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t r, char* tile, int dim, F off) const {
+if (dim == NC * 8) {
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      const int ci = (i * NW + wave) * 64 + lane;
-      const int row = ci / NC, c = (ci % NC) ^ swz<NC>(row);
-      if (NC * 8 == dim || c * 8 < dim)
+      for (int i = 0; i < kPer; ++i) {
+        const int ci = (i * NW + wave) * 64 + lane, row = ci / NC, c = (ci % NC) ^ swz<NC>(row);
         dense::blds16(r, (uint32_t)(off(row) + c * 16), tile + (i * NW + wave) * 1024);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        const int ci = (i * NW + wave) * 64 + lane, row = ci / NC, c = (ci % NC) ^ swz<NC>(row);
+        if (c * 8 < dim) dense::blds16(r, (uint32_t)(off(row) + c * 16), tile + (i * NW + wave) * 1024);
+      }
     }
   }
 };
+
+// Keys and values [kt, kt + have) of one key head into a buffer.
+template <int DP, int NW>
+__device__ __forceinline__ void stage_kv(char* __restrict__ nxt, const Stager<DP / 8, NW, kKeys>& stager, const char* k, const char* v,
+                                         int64_t kts, int64_t vts, int have, int dim) {
+  const int kst = (int)kts * 2, vst = (int)vts * 2;
+  const __amdgpu_buffer_rsrc_t kr = dense::tile_rsrc_u(k, (uint32_t)((have - 1) * kst + dim * 2));
+  const __amdgpu_buffer_rsrc_t vr = dense::tile_rsrc_u(v, (uint32_t)((have - 1) * vst + dim * 2));
+  stager.load(kr, nxt, dim, [&](int r) { return min(r, have - 1) * kst; });
+  stager.load(vr, nxt + kKeys * DP * 2, dim, [&](int r) { return min(r, have - 1) * vst; });
+}
 
 }  // namespace attn
 }  // namespace ahr
