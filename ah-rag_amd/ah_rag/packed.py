@@ -28,7 +28,8 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
-import math
+import struct
+from types import SimpleNamespace
 from typing import Dict, Optional, Sequence, Tuple, Union
 
 import numpy as np
@@ -73,6 +74,7 @@ class PackedLayout:
             raise ValueError("a PackedLayout serves a ROCm GPU")
         if self.device.index is None:
             self.device = torch.device("cuda", torch.cuda.current_device())
+        self._index = self.device.index
         self.tokens = int(self.lengths.sum(dtype=np.int64))
         self.key_tokens = int(self.key_lengths.sum(dtype=np.int64))
         self._plans: Dict[tuple, Tuple[nat.AttnPlan, Optional[torch.Tensor]]] = {}
@@ -88,7 +90,9 @@ class PackedLayout:
                 raise RuntimeError("a layout's first call for a shape copies its work lists to the device: make it "
                                    "before the capture")
             # a blocking copy: the lists are complete for every stream
-            return torch.from_numpy(host).to(self.device)
+            t = torch.from_numpy(host).to(self.device)
+            t.ahr_stream = nat.stream_ptr(device_index=self._index)
+            return t
 
     def positions(self) -> torch.Tensor:
         """int32 [tokens] on the device: each token's position among its sequence's keys (0, 1, ... where
@@ -133,13 +137,15 @@ class PackedLayout:
 # ---- shared checks ---------------------------------------------------------------------------
 
 
-def _heads(t: torch.Tensor, what: str, like: Optional[torch.Tensor] = None, tokens: Optional[int] = None) -> None:
+def _heads(t: torch.Tensor, what: str) -> None:
     if not isinstance(t, torch.Tensor) or t.dim() != 3:
         raise ValueError(f"{what} must be a [tokens, heads, head_dim] tensor")
-    if like is not None and (t.dtype != like.dtype or t.device != like.device or t.shape[2] != like.shape[2]):
+
+
+def _like(t: torch.Tensor, what: str, q: torch.Tensor) -> None:
+    _heads(t, what)
+    if t.dtype != q.dtype or t.device != q.device or t.shape[2] != q.shape[2]:
         raise ValueError(f"{what} must have q's dtype, device and head_dim")
-    if tokens is not None and t.shape[0] != tokens:
-        raise ValueError(f"{what} has {t.shape[0]} tokens, the layout {tokens}")
 
 
 def _on_device(device: torch.device, *tensors: Optional[torch.Tensor]) -> None:
@@ -149,31 +155,50 @@ def _on_device(device: torch.device, *tensors: Optional[torch.Tensor]) -> None:
 
 
 def _aligned(t: torch.Tensor) -> torch.Tensor:
-    """t, or a copy whose rows start at multiples of 16 bytes and are contiguous."""
-    per = 16 // t.element_size()
+    """t, or a copy whose rows start at multiples of 16 bytes and are contiguous (16-bit types)."""
     n, h, d = t.shape
     ts, hs, es = t.stride()
-    if ((es == 1 or d == 1) and t.data_ptr() % 16 == 0 and (n < 2 or (ts % per == 0 and ts <= 1 << 23))
-            and (h < 2 or (hs % per == 0 and hs * h <= 1 << 29))):
+    if ((es == 1 or d == 1) and t.data_ptr() % 16 == 0 and (n < 2 or (ts % 8 == 0 and ts <= 1 << 23))
+            and (h < 2 or (hs % 8 == 0 and hs * h <= 1 << 29))):
         return t
     t = t.contiguous()
     return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
-def _tensor3(to: nat.Tensor3, t: torch.Tensor) -> None:
-    to.p = t.data_ptr()
-    # (the stride of an axis of one element is arbitrary)
-    to.ts = t.stride(0) if t.shape[0] > 1 else 0
-    to.hs = t.stride(1) if t.shape[1] > 1 else 0
+def _rows(t: Optional[torch.Tensor]) -> Tuple[int, int, int]:
+    """A struct ahr_tensor3: address and strides of tokens and heads (of an axis of one element arbitrary)."""
+    if t is None:
+        return 0, 0, 0
+    n, h, _ = t.shape
+    ts, hs, _ = t.stride()
+    return t.data_ptr(), ts if n > 1 else 0, hs if h > 1 else 0
+
+
+def _calls() -> SimpleNamespace:
+    """The entry points that take an argument struct, as (bytes, stream) -> status."""
+    global _CALLS
+    if _CALLS is None:
+        lib = nat.lib()
+        kind = ctypes.CFUNCTYPE(ctypes.c_int, ctypes.c_char_p, ctypes.c_void_p)
+        _CALLS = SimpleNamespace(**{n: kind((f, lib)) for n, f in (
+            ("attn_forward", "ahr_attn_forward"), ("attn_backward", "ahr_attn_backward"), ("rope", "ahr_qk_norm_rope"),
+            ("rope_backward", "ahr_qk_norm_rope_backward"))})
+    return _CALLS
+
+
+_CALLS: Optional[SimpleNamespace] = None
+
+# The argument structs of include/ahr.h, packed in one step (field by field through ctypes costs more than
+# a small kernel).
+_ATTN_ARGS = struct.Struct("@PPfi 3q3q3q 3q3q 3q P 3q3q3q3q Pq".replace(" ", ""))
+_ROPE_ARGS = struct.Struct("@iiiiii qqfi 3q3q 3q3q 3q3q PPPPP PP Pq".replace(" ", ""))
+assert _ATTN_ARGS.size == ctypes.sizeof(nat.AttnArgs) and _ROPE_ARGS.size == ctypes.sizeof(nat.RopeArgs)
 
 
 @contextlib.contextmanager
-def _on(stream: Optional[torch.cuda.Stream], device: torch.device, *tensors: Optional[torch.Tensor]):
-    """Run on the tensors' device and, if given, on `stream`, after the current stream's work."""
+def _side(stream: torch.cuda.Stream, device: torch.device, *tensors: Optional[torch.Tensor]):
+    """Run on `stream`, after the current stream's work."""
     with torch.cuda.device(device):
-        if stream is None or stream == torch.cuda.current_stream(device):
-            yield
-            return
         stream.wait_stream(torch.cuda.current_stream(device))
         for t in tensors:
             if t is not None:
@@ -182,37 +207,47 @@ def _on(stream: Optional[torch.cuda.Stream], device: torch.device, *tensors: Opt
             yield
 
 
-def _keep(lists: Optional[torch.Tensor], device: torch.device) -> None:
-    """The layout may be dropped while the current stream still reads its lists."""
-    if lists is not None and not torch.cuda.is_current_stream_capturing():
+def _elsewhere(stream: Optional[torch.cuda.Stream], device: torch.device) -> bool:
+    """Whether the call has to leave the current device or stream."""
+    return stream is not None or torch.cuda.current_device() != device.index
+
+
+def _on(stream: Optional[torch.cuda.Stream], device: torch.device, *tensors: Optional[torch.Tensor]):
+    return torch.cuda.device(device) if stream is None else _side(stream, device, *tensors)
+
+
+def _keep(lists: Optional[torch.Tensor], stream: int, device: torch.device) -> None:
+    """The layout may be dropped while another stream than the one that made its lists still reads them."""
+    if lists is not None and lists.ahr_stream != stream and not torch.cuda.is_current_stream_capturing():
         lists.record_stream(torch.cuda.current_stream(device))
 
 
 # ---- attention -------------------------------------------------------------------------------
 
 
+def _workspace(plan: nat.AttnPlan, device: torch.device) -> Optional[torch.Tensor]:
+    return torch.empty(plan.ws_bytes, dtype=torch.uint8, device=device) if plan.ws_bytes else None
+
+
+def _launch_attention(call, name, plan, lists, scale, q, k, v, pk, pv, o, lse, d_o, dq, dk, dv) -> None:
+    ws = _workspace(plan, q.device)
+    stream = nat.stream_ptr(device_index=q.device.index)
+    args = _ATTN_ARGS.pack(ctypes.addressof(plan), 0 if lists is None else lists.data_ptr(), scale, 0, *_rows(q), *_rows(k), *_rows(v),
+                           *_rows(pk), *_rows(pv), *_rows(o), 0 if lse is None else lse.data_ptr(), *_rows(d_o), *_rows(dq), *_rows(dk),
+                           *_rows(dv), 0 if ws is None else ws.data_ptr(), plan.ws_bytes)
+    if call(args, stream):
+        nat.check(-1, name)
+    _keep(lists, stream, q.device)
+
+
 def _attention(q, k, v, layout, causal, scale, lse, prefix_k=None, prefix_v=None, out=None) -> torch.Tensor:
     q, k, v = _aligned(q), _aligned(k), _aligned(v)
-    tokens, heads, dim = q.shape
-    plan, lists = layout._plan(_CODES[q.dtype], heads, k.shape[1], dim, causal, False,
-                               0 if prefix_k is None else prefix_k.shape[0])
-    o = torch.empty((tokens, heads, dim), dtype=q.dtype, device=q.device) if out is None else out
-    a = nat.AttnArgs()
-    a.plan = ctypes.pointer(plan)
-    a.lists = nat.ptr(lists)
-    a.scale = scale
-    for to, t in ((a.q, q), (a.k, k), (a.v, v), (a.o, o)):
-        _tensor3(to, t)
+    shape = q.shape
     if prefix_k is not None:
         prefix_k, prefix_v = _aligned(prefix_k), _aligned(prefix_v)
-        _tensor3(a.prefix_k, prefix_k)
-        _tensor3(a.prefix_v, prefix_v)
-    a.lse = nat.ptr(lse)
-    if plan.ws_bytes:
-        ws = torch.empty(plan.ws_bytes, dtype=torch.uint8, device=q.device)
-        a.ws, a.ws_bytes = ws.data_ptr(), plan.ws_bytes
-    nat.check(nat.lib().ahr_attn_forward(ctypes.byref(a), nat.stream_ptr(device_index=q.device.index)), "ahr_attn_forward")
-    _keep(lists, q.device)
+    plan, lists = layout._plan(_CODES[q.dtype], shape[1], k.shape[1], shape[2], causal, False, 0 if prefix_k is None else prefix_k.shape[0])
+    o = torch.empty(shape, dtype=q.dtype, device=q.device) if out is None else out
+    _launch_attention(_calls().attn_forward, "ahr_attn_forward", plan, lists, scale, q, k, v, prefix_k, prefix_v, o, lse, None, None, None, None)
     return o
 
 
@@ -234,40 +269,32 @@ class _PackedAttention(torch.autograd.Function):
         q, k, v, o, lse = ctx.saved_tensors
         with torch.cuda.device(q.device):
             plan, lists = ctx.layout._plan(_CODES[q.dtype], q.shape[1], k.shape[1], q.shape[2], ctx.causal, True, 0)
-            d_o, o = _aligned(d_o), _aligned(o)
             dq, dk, dv = (torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in (q, k, v))
-            a = nat.AttnArgs()
-            a.plan = ctypes.pointer(plan)
-            a.lists = nat.ptr(lists)
-            a.scale = ctx.scale
-            for to, t in ((a.q, q), (a.k, k), (a.v, v), (a.o, o), (a.d_o, d_o), (a.dq, dq), (a.dk, dk), (a.dv, dv)):
-                _tensor3(to, t)
-            a.lse = lse.data_ptr()
-            if plan.ws_bytes:
-                ws = torch.empty(plan.ws_bytes, dtype=torch.uint8, device=q.device)
-                a.ws, a.ws_bytes = ws.data_ptr(), plan.ws_bytes
-            nat.check(nat.lib().ahr_attn_backward(ctypes.byref(a), nat.stream_ptr(device_index=q.device.index)),
-                      "ahr_attn_backward")
-            _keep(lists, q.device)
+            _launch_attention(_calls().attn_backward, "ahr_attn_backward", plan, lists, ctx.scale, q, k, v, None, None, _aligned(o), lse,
+                              _aligned(d_o), dq, dk, dv)
         return dq, dk, dv, None, None, None
 
 
 def _check_attention(q, k, v, layout, scale) -> float:
-    _heads(q, "q", tokens=layout.tokens)
-    _heads(k, "k", q, layout.key_tokens)
-    _heads(v, "v", q, layout.key_tokens)
+    _heads(q, "q")
+    _like(k, "k", q)
+    _like(v, "v", q)
+    tokens, heads, dim = q.shape
+    keys, kv_heads, _ = k.shape
+    if tokens != layout.tokens or keys != layout.key_tokens:
+        raise ValueError(f"q has {tokens} and k {keys} tokens, the layout {layout.tokens} and {layout.key_tokens}")
     if v.shape != k.shape:
         raise ValueError("v must have k's shape")
     if q.dtype not in (torch.float16, torch.bfloat16):
         raise ValueError(f"attention takes float16 and bfloat16, got {q.dtype}")
-    if k.shape[1] < 1 or q.shape[1] < 1 or q.shape[1] % k.shape[1] or q.shape[1] // k.shape[1] > 128:
-        raise ValueError(f"{q.shape[1]} query heads do not share {k.shape[1]} key heads (a multiple, at most 128 each)")
-    dim = q.shape[2]
+    if kv_heads < 1 or heads < 1 or heads % kv_heads or heads // kv_heads > 128:
+        raise ValueError(f"{heads} query heads do not share {kv_heads} key heads (a multiple, at most 128 each)")
     if dim < 8 or dim % 8 or dim > 128:
         raise ValueError(f"head_dim must be a multiple of 8, at most 128, got {dim}")
-    _on_device(layout.device, q, k, v)
+    if q.device != layout.device:
+        raise ValueError(f"tensors must be on {layout.device}, got one on {q.device}")
     scale = dim ** -0.5 if scale is None else float(scale)
-    if not (scale > 0 and math.isfinite(scale)):
+    if not 0 < scale < 3e38:
         raise ValueError("scale must be positive and finite")
     return scale
 
@@ -302,10 +329,12 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, layout: 
     grad = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)
     if grad and out is not None:
         raise ValueError("out cannot be given where a gradient is wanted")
-    with _on(stream, layout.device, q, k, v, out):
-        if grad:
-            return _PackedAttention.apply(q, k, v, layout, bool(causal), scale)
-        return _attention(q, k, v, layout, bool(causal), scale, None, out=out)
+    if _elsewhere(stream, layout.device):
+        with _on(stream, layout.device, q, k, v, out):
+            return packed_attention(q, k, v, layout, causal, scale, None, out)
+    if grad:
+        return _PackedAttention.apply(q, k, v, layout, bool(causal), scale)
+    return _attention(q, k, v, layout, bool(causal), scale, None, out=out)
 
 
 def prefix_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, prefix_k: torch.Tensor, prefix_v: torch.Tensor,
@@ -320,15 +349,16 @@ def prefix_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, prefix_k
     enabled."""
     scale = _check_attention(q, k, v, layout, scale)
     _check_out(out, q)
-    _heads(prefix_k, "prefix_k", q)
-    _heads(prefix_v, "prefix_v", q)
+    _like(prefix_k, "prefix_k", q)
+    _like(prefix_v, "prefix_v", q)
     if prefix_k.shape != prefix_v.shape or prefix_k.shape[1] != k.shape[1]:
         raise ValueError("prefix_k and prefix_v must have the same shape and k's heads")
-    _on_device(layout.device, prefix_k, prefix_v)
     if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, prefix_k, prefix_v)):
         raise ValueError("prefix_attention has no gradient")
-    with _on(stream, layout.device, q, k, v, prefix_k, prefix_v, out):
-        return _attention(q, k, v, layout, bool(causal), scale, None, prefix_k, prefix_v, out)
+    if _elsewhere(stream, layout.device):
+        with _on(stream, layout.device, q, k, v, prefix_k, prefix_v, out):
+            return prefix_attention(q, k, v, prefix_k, prefix_v, layout, causal, scale, None, out)
+    return _attention(q, k, v, layout, bool(causal), scale, None, prefix_k, prefix_v, out)
 
 
 # ---- q/k norm with rotation ------------------------------------------------------------------
@@ -345,24 +375,21 @@ def rotary_table(n_positions: int, dim: int, base: float = 10000.0,
     return angle.cos().float().to(device), angle.sin().float().to(device)
 
 
-def _rope_args(q, k, cos, sin, positions, eps, interleaved, wq, wk) -> nat.RopeArgs:
-    a = nat.RopeArgs()
-    a.dtype, a.heads, a.kv_heads, a.head_dim = _CODES[q.dtype], q.shape[1], k.shape[1], q.shape[2]
-    a.rot, a.interleaved = 2 * cos.shape[1], int(interleaved)
-    a.tokens, a.n_pos, a.eps = q.shape[0], cos.shape[0], eps
-    _tensor3(a.q, q)
-    _tensor3(a.k, k)
-    a.wq, a.wk = nat.ptr(wq), nat.ptr(wk)
-    a.cos, a.sin, a.positions = cos.data_ptr(), sin.data_ptr(), positions.data_ptr()
-    return a
+def _launch_rope(call, name, q, k, cos, sin, positions, eps, interleaved, wq, wk, yq, yk, dq=None, dk=None, dw=None, ws=None) -> None:
+    tokens, heads, dim = q.shape
+    n_pos, half = cos.shape
+    dwq, dwk = (0, 0) if dw is None else (dw.data_ptr(), dw.data_ptr() + 4 * dim)
+    args = _ROPE_ARGS.pack(_CODES[q.dtype], heads, k.shape[1], dim, 2 * half, interleaved, tokens, n_pos, eps, 0, *_rows(q), *_rows(k),
+                           *_rows(yq), *_rows(yk), *_rows(dq), *_rows(dk), 0 if wq is None else wq.data_ptr(),
+                           0 if wk is None else wk.data_ptr(), cos.data_ptr(), sin.data_ptr(), positions.data_ptr(), dwq, dwk,
+                           0 if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel())
+    if call(args, nat.stream_ptr(device_index=q.device.index)):
+        nat.check(-1, name)
 
 
 def _rope_forward(q, k, wq, wk, cos, sin, positions, eps, interleaved):
-    yq, yk = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k))
-    a = _rope_args(q, k, cos, sin, positions, eps, interleaved, wq, wk)
-    _tensor3(a.yq, yq)
-    _tensor3(a.yk, yk)
-    nat.check(nat.lib().ahr_qk_norm_rope(ctypes.byref(a), nat.stream_ptr(device_index=q.device.index)), "ahr_qk_norm_rope")
+    yq, yk = torch.empty(q.shape, dtype=q.dtype, device=q.device), torch.empty(k.shape, dtype=k.dtype, device=k.device)
+    _launch_rope(_calls().rope, "ahr_qk_norm_rope", q, k, cos, sin, positions, eps, interleaved, wq, wk, yq, yk)
     return yq, yk
 
 
@@ -370,34 +397,36 @@ def _unit(t: torch.Tensor) -> torch.Tensor:
     return t if t.stride(2) == 1 or t.shape[2] == 1 else t.contiguous()
 
 
+def _weight(w: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+    if w is None or (w.dtype == torch.float32 and w.is_contiguous()):
+        return w
+    return w.detach().float().contiguous()
+
+
 class _QkNormRope(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, wq, wk, cos, sin, positions, eps, interleaved):
-        w = [None if x is None else x.detach().float().contiguous() for x in (wq, wk)]
-        ctx.save_for_backward(q, k, w[0], w[1], cos, sin, positions)
+    def forward(ctx, q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved):
+        wq, wk = _weight(q_weight), _weight(k_weight)
+        ctx.save_for_backward(q, k, wq, wk, cos, sin, positions)
         ctx.eps, ctx.interleaved = eps, interleaved
-        ctx.w_dtype = None if wq is None else (wq.dtype, wk.dtype)
-        return _rope_forward(q, k, w[0], w[1], cos, sin, positions, eps, interleaved)
+        ctx.w_dtype = None if wq is None else (q_weight.dtype, k_weight.dtype)
+        return _rope_forward(q, k, wq, wk, cos, sin, positions, eps, interleaved)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dyq, dyk):
         q, k, wq, wk, cos, sin, positions = ctx.saved_tensors
         with torch.cuda.device(q.device):
-            dyq, dyk = _unit(dyq), _unit(dyk)
-            dq, dk = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k))
-            a = _rope_args(q, k, cos, sin, positions, ctx.eps, ctx.interleaved, wq, wk)
-            for to, t in ((a.yq, dyq), (a.yk, dyk), (a.dq, dq), (a.dk, dk)):
-                _tensor3(to, t)
-            dw = None
+            dim = q.shape[2]
+            dq, dk = torch.empty(q.shape, dtype=q.dtype, device=q.device), torch.empty(k.shape, dtype=k.dtype, device=k.device)
+            dw = ws = None
             if wq is not None:
                 n = ctypes.c_int64()
-                nat.check(nat.lib().ahr_rope_ws_bytes(q.shape[0], q.shape[2], ctypes.byref(n)), "ahr_rope_ws_bytes")
+                nat.check(nat.lib().ahr_rope_ws_bytes(q.shape[0], dim, ctypes.byref(n)), "ahr_rope_ws_bytes")
                 ws = torch.empty(n.value, dtype=torch.uint8, device=q.device)
-                dw = torch.empty((2, q.shape[2]), dtype=torch.float32, device=q.device)
-                a.dwq, a.dwk, a.ws, a.ws_bytes = dw[0].data_ptr(), dw[1].data_ptr(), ws.data_ptr(), n.value
-            nat.check(nat.lib().ahr_qk_norm_rope_backward(ctypes.byref(a), nat.stream_ptr(device_index=q.device.index)),
-                      "ahr_qk_norm_rope_backward")
+                dw = torch.empty((2, dim), dtype=torch.float32, device=q.device)
+            _launch_rope(_calls().rope_backward, "ahr_qk_norm_rope_backward", q, k, cos, sin, positions, ctx.eps, ctx.interleaved, wq, wk,
+                         _unit(dyq), _unit(dyk), dq, dk, dw, ws)
         gq, gk = (None, None) if dw is None else (dw[0].to(ctx.w_dtype[0]), dw[1].to(ctx.w_dtype[1]))
         return dq, dk, gq, gk, None, None, None, None, None
 
@@ -415,13 +444,15 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: Optional[torch.Tens
     2 i + 1. head_dim even, at most 512. Computed in fp32, rounded once. Differentiable in q, k and the
     weights (whose gradients are summed in a fixed order)."""
     _heads(q, "q")
-    _heads(k, "k", q, q.shape[0])
+    _like(k, "k", q)
     if q.dtype not in _CODES:
         raise ValueError(f"qk_norm_rope takes float32, float16 and bfloat16, got {q.dtype}")
-    dim = q.shape[2]
+    tokens, heads, dim = q.shape
+    if k.shape[0] != tokens:
+        raise ValueError("q and k must have the same tokens")
     if dim < 2 or dim % 2 or dim > 512:
         raise ValueError(f"head_dim must be even, at most 512, got {dim}")
-    if q.shape[1] < 1 or k.shape[1] < 1:
+    if heads < 1 or k.shape[1] < 1:
         raise ValueError("q and k need a head each")
     if (q_weight is None) != (k_weight is None):
         raise ValueError("one norm weight without the other")
@@ -430,25 +461,27 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: Optional[torch.Tens
             raise ValueError("a norm weight must be a floating [head_dim] tensor")
     if cos.dim() != 2 or cos.shape != sin.shape or cos.dtype != torch.float32 or sin.dtype != torch.float32:
         raise ValueError("cos and sin must be float32 tensors of the same [positions, rot / 2]")
-    if cos.shape[1] < 1 or 2 * cos.shape[1] > dim or (cos.shape[0] < 1 and q.shape[0] > 0):
+    n_pos, half = cos.shape
+    if half < 1 or 2 * half > dim or (n_pos < 1 and tokens > 0):
         raise ValueError("the table must have a row, and at most head_dim / 2 columns")
-    if positions.shape != (q.shape[0],) or positions.dtype not in (torch.int32, torch.int64):
+    if positions.shape != (tokens,) or positions.dtype not in (torch.int32, torch.int64):
         raise ValueError("positions must be int32 or int64 [tokens]")
-    if not (eps >= 0 and math.isfinite(eps)):
+    if not 0 <= eps < 3e38:
         raise ValueError("eps must be finite and not negative")
-    if q.device.type != "cuda":
+    device = q.device
+    if device.type != "cuda":
         raise nat.NativeLibraryError("qk_norm_rope needs tensors on a ROCm GPU")
-    _on_device(q.device, k, q_weight, k_weight, cos, sin, positions)
-    grad = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, q_weight, k_weight))
-    with _on(stream, q.device, q, k, q_weight, k_weight, cos, sin, positions):
-        if positions.dtype == torch.int64:  # (a position beyond 32 bits must not wrap into the table)
-            positions = positions.clamp(-1, 2 ** 31 - 1).to(torch.int32)
-        cos, sin, positions = cos.contiguous(), sin.contiguous(), positions.contiguous()
-        q, k = _unit(q), _unit(k)
-        if grad:
-            return _QkNormRope.apply(q, k, q_weight, k_weight, cos, sin, positions, float(eps), bool(interleaved))
-        w = [None if x is None else x.detach().float().contiguous() for x in (q_weight, k_weight)]
-        return _rope_forward(q, k, w[0], w[1], cos, sin, positions, float(eps), bool(interleaved))
+    _on_device(device, q_weight, k_weight, cos, sin, positions)
+    if _elsewhere(stream, device):
+        with _on(stream, device, q, k, q_weight, k_weight, cos, sin, positions):
+            return qk_norm_rope(q, k, q_weight, k_weight, cos, sin, positions, eps, interleaved)
+    if positions.dtype == torch.int64:  # (a position beyond 32 bits must not wrap into the table)
+        positions = positions.clamp(-1, 2 ** 31 - 1).to(torch.int32)
+    cos, sin, positions = cos.contiguous(), sin.contiguous(), positions.contiguous()
+    q, k = _unit(q), _unit(k)
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or (q_weight is not None and (q_weight.requires_grad or k_weight.requires_grad))):
+        return _QkNormRope.apply(q, k, q_weight, k_weight, cos, sin, positions, float(eps), bool(interleaved))
+    return _rope_forward(q, k, _weight(q_weight), _weight(k_weight), cos, sin, positions, float(eps), bool(interleaved))
 
 
 # ---- mean pooling ----------------------------------------------------------------------------
@@ -459,10 +492,10 @@ def _pool_forward(rows, layout, normalize, norm):
     n, width = len(layout), rows.shape[1]
     out = torch.empty((n, width), dtype=torch.float32, device=rows.device)
     ws = torch.empty(max(1, n_chunks * width), dtype=torch.float32, device=rows.device)
+    stream = nat.stream_ptr(device_index=rows.device.index)
     nat.check(nat.lib().ahr_pool_mean(_CODES[rows.dtype], rows.data_ptr(), rows.stride(0), width, lists.data_ptr(), n_chunks, n,
-                                      int(normalize), out.data_ptr(), nat.ptr(norm), ws.data_ptr(), ws.numel() * 4,
-                                      nat.stream_ptr(device_index=rows.device.index)), "ahr_pool_mean")
-    _keep(lists, rows.device)
+                                      int(normalize), out.data_ptr(), nat.ptr(norm), ws.data_ptr(), ws.numel() * 4, stream), "ahr_pool_mean")
+    _keep(lists, stream, rows.device)
     return out
 
 
@@ -483,12 +516,11 @@ class _PackedMeanPool(torch.autograd.Function):
             n_chunks, lists = ctx.layout._pool_lists()
             d_out = d_out.contiguous()
             d_rows = torch.empty(ctx.shape, dtype=ctx.dtype, device=out.device)
+            stream = nat.stream_ptr(device_index=out.device.index)
             nat.check(nat.lib().ahr_pool_mean_backward(_CODES[ctx.dtype], d_rows.data_ptr(), ctx.shape[1], lists.data_ptr(),
                                                        n_chunks, len(ctx.layout), int(ctx.normalize), d_out.data_ptr(),
-                                                       out.data_ptr(), norm.data_ptr(),
-                                                       nat.stream_ptr(device_index=out.device.index)),
-                      "ahr_pool_mean_backward")
-            _keep(lists, out.device)
+                                                       out.data_ptr(), norm.data_ptr(), stream), "ahr_pool_mean_backward")
+            _keep(lists, stream, out.device)
         return d_rows, None, None
 
 
@@ -504,9 +536,11 @@ def packed_mean_pool(rows: torch.Tensor, layout: PackedLayout, normalize: bool =
     if rows.shape[0] != layout.tokens:
         raise ValueError(f"rows has {rows.shape[0]} tokens, the layout {layout.tokens}")
     _on_device(layout.device, rows)
-    with _on(stream, layout.device, rows):
-        if rows.stride(1) != 1 and rows.shape[1] > 1:
-            rows = rows.contiguous()
-        if torch.is_grad_enabled() and rows.requires_grad:
-            return _PackedMeanPool.apply(rows, layout, bool(normalize))
-        return _pool_forward(rows, layout, bool(normalize), None)
+    if _elsewhere(stream, layout.device):
+        with _on(stream, layout.device, rows):
+            return packed_mean_pool(rows, layout, normalize)
+    if rows.stride(1) != 1 and rows.shape[1] > 1:
+        rows = rows.contiguous()
+    if torch.is_grad_enabled() and rows.requires_grad:
+        return _PackedMeanPool.apply(rows, layout, bool(normalize))
+    return _pool_forward(rows, layout, bool(normalize), None)

@@ -9,6 +9,8 @@ namespace ahr {
 namespace attn {
 
 constexpr int kKeys = 64;     // keys of one staged tile
+constexpr int kWaves = 4;     // waves of a workgroup
+constexpr int kRows = 128;    // rows of a row tile: 32 a wave
 constexpr int kMaxDim = 128;  // head dimensions: multiples of 8 up to this
 constexpr int kMaxGroup = 128;  // query heads that share a key head
 

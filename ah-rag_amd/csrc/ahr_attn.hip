@@ -94,9 +94,9 @@ __device__ __forceinline__ void fwd_tile(const char* __restrict__ cur, FwdState<
   }
 }
 
-template <typename T, int DP, int NW>
+template <typename T, int DP>
 __device__ __forceinline__ void fwd_step(const char* __restrict__ cur, char* __restrict__ nxt, FwdState<T, DP>& st,
-                                         const Stager<DP / 8, NW, kKeys>& stager, const Params& p, const RowItem& it, int hk, int t, int np,
+                                         const Stager<DP / 8, kWaves, kKeys>& stager, const Params& p, const RowItem& it, int hk, int t, int np,
                                          int nt, bool wave_live, int lim, int lim_lo, int lim_hi, int lane) {
   auto stage = [&](int t) {
     const bool pre = t < np;
@@ -104,7 +104,7 @@ __device__ __forceinline__ void fwd_step(const char* __restrict__ cur, char* __r
     const int have = min(kKeys, (pre ? it.pe : it.ke) - kt);
     const int64_t at = pre ? kt : (int64_t)it.k0 + kt;
     const int64_t kts = pre ? p.pk_ts : p.k_ts, vts = pre ? p.pv_ts : p.v_ts;
-    stage_kv<DP, NW>(nxt, stager, (pre ? p.pk : p.k) + (at * kts + hk * (pre ? p.pk_hs : p.k_hs)) * 2,
+    stage_kv<DP>(nxt, stager, (pre ? p.pk : p.k) + (at * kts + hk * (pre ? p.pk_hs : p.k_hs)) * 2,
                      (pre ? p.pv : p.v) + (at * vts + hk * (pre ? p.pv_hs : p.v_hs)) * 2, kts, vts, have, p.dim);
   };
   if (t + 1 < nt) stage(t + 1);
@@ -116,8 +116,8 @@ __device__ __forceinline__ void fwd_step(const char* __restrict__ cur, char* __r
   fwd_tile<T, DP>(cur, st, kt + kKeys > stop || (!pre && kt + kKeys > lim_lo), (pre ? stop : min(lim, stop)) - kt, p.scale_log2, lane);
 }
 
-template <typename T, int DP, int NW>
-__global__ __launch_bounds__(NW * 64, 2) void attn_fwd_kernel(Params p) {
+template <typename T, int DP>
+__global__ __launch_bounds__(kWaves * 64, 2) void attn_fwd_kernel(Params p) {
   typedef typename Elem<T>::v8 v8;
   constexpr int KS = DP / 16, DB = DP / 32;
   constexpr int kTile = kKeys * DP * 2;
@@ -129,7 +129,7 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_fwd_kernel(Params p) {
   const int dim = p.dim;
 
   if (DP != dim) {  // the chunks past dim are never loaded
-    for (int i = threadIdx.x; i < 4 * kTile / 16; i += NW * 64) reinterpret_cast<f32x4*>(smem)[i] = f32x4{0, 0, 0, 0};
+    for (int i = threadIdx.x; i < 4 * kTile / 16; i += kWaves * 64) reinterpret_cast<f32x4*>(smem)[i] = f32x4{0, 0, 0, 0};
     __syncthreads();
   }
 
@@ -163,14 +163,14 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_fwd_kernel(Params p) {
   st.m = -INFINITY;
   st.l = 0.f;
 
-  const Stager<DP / 8, NW, kKeys> stager(wave, lane);
+  const Stager<DP / 8, kWaves, kKeys> stager(wave, lane);
   const int np = (it.pe - it.pb + kKeys - 1) / kKeys;
   const int nt = np + (it.ke - it.kb + kKeys - 1) / kKeys;
   if (nt > 0) {
-    fwd_step<T, DP, NW>(smem, smem, st, stager, p, it, hk, -1, np, nt, false, 0, 0, 0, lane);  // the first tile's loads
+    fwd_step<T, DP>(smem, smem, st, stager, p, it, hk, -1, np, nt, false, 0, 0, 0, lane);  // the first tile's loads
     for (int t = 0; t < nt; ++t) {
       tile_barrier();  // tile t has landed, tile t - 1 is no longer read
-      fwd_step<T, DP, NW>(smem + (t & 1) * 2 * kTile, smem + ((t + 1) & 1) * 2 * kTile, st, stager, p, it, hk, t, np, nt, wave_live, lim,
+      fwd_step<T, DP>(smem + (t & 1) * 2 * kTile, smem + ((t + 1) & 1) * 2 * kTile, st, stager, p, it, hk, t, np, nt, wave_live, lim,
                           lim_lo, lim_hi, lane);
     }
   }
@@ -207,40 +207,47 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_fwd_kernel(Params p) {
     }
 }
 
-// Joins partial results: o = sum_i 2^(lse_i - max) o_i / sum_i 2^(lse_i - max). One wave per row;
-// each plane is read once.
+// Joins partial results: o = sum_i 2^(lse_i - max) o_i / sum_i 2^(lse_i - max). dim / 4 lanes (a power of
+// two or, with idle lanes, the next) take a row, 4 elements each; every partial value is read once.
 template <typename T>
-__global__ __launch_bounds__(256) void attn_join_kernel(Params p) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const JoinItem it = p.join[blockIdx.x / p.heads];
-  const int head = blockIdx.x % p.heads;
-  const int64_t plane = p.prows * p.heads;
-  for (int i = wave; i < it.nq; i += 4) {
-    const int64_t at = (int64_t)(it.prow + i) * p.heads + head;
-    float top = -INFINITY;
-    for (int j = lane; j < it.np; j += 64) top = fmaxf(top, p.part_l[at + j * plane]);
+__global__ __launch_bounds__(256) void attn_join_kernel(Params p, int lanes) {
+  const JoinItem it = p.join[blockIdx.x];
+  const int per = 256 / lanes;  // rows of a workgroup
+  const int r = blockIdx.y * per + threadIdx.x / lanes, d = (threadIdx.x % lanes) * 4;
+  if (r >= it.nq * p.heads || d >= p.dim) return;
+  const int i = r / p.heads, head = r - i * p.heads;
+  const int64_t plane = p.prows * p.heads, at = (int64_t)(it.prow + i) * p.heads + head;
+  const float* pl = p.part_l + at;
+  const float* po = p.part_o + at * p.dim + d;
+  float m = -INFINITY, sum = 0.f;
+  f32x4 a = {0, 0, 0, 0};
+  for (int j0 = 0; j0 < it.np; j0 += 8) {  // the loads of 8 planes are in flight together
+    float l[8];
+    f32x4 x[8];
 #pragma unroll
-    for (int x = 1; x < 64; x *= 2) top = fmaxf(top, __shfl_xor(top, x, 64));
-    const float ref = top == -INFINITY ? 0.f : top;
-    float sum = 0.f, a = 0.f, b = 0.f;
-    const bool have = lane * 2 < p.dim;
-    for (int j = 0; j < it.np; ++j) {
-      const float w = ex2(p.part_l[at + j * plane] - ref);
+    for (int j = 0; j < 8; ++j) {
+      const int64_t o = min(j0 + j, it.np - 1) * plane;
+      l[j] = j0 + j < it.np ? pl[o] : -INFINITY;
+      x[j] = *reinterpret_cast<const f32x4*>(po + o * p.dim);
+    }
+    float to = m;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) to = fmaxf(to, l[j]);
+    const float ref = to == -INFINITY ? 0.f : to, f = ex2(m - ref);
+    sum *= f;
+    a *= f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float w = ex2(l[j] - ref);
+      if (j0 + j >= it.np) break;
       sum += w;
-      if (have) {
-        const float2 x = *reinterpret_cast<const float2*>(p.part_o + (at + j * plane) * p.dim + lane * 2);
-        a = fmaf(w, x.x, a);
-        b = fmaf(w, x.y, b);
-      }
+      a += w * x[j];
     }
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    if (p.lse && lane == 0) p.lse[(int64_t)(it.q0 + i) * p.heads + head] = sum == 0.f ? -INFINITY : ref + __log2f(sum);
-    if (have) {
-      T* o = reinterpret_cast<T*>(p.o) + (int64_t)(it.q0 + i) * p.o_ts + (int64_t)head * p.o_hs + lane * 2;
-      o[0] = (T)(a * inv);
-      o[1] = (T)(b * inv);
-    }
+    m = to;
   }
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  if (p.lse && d == 0) p.lse[(int64_t)(it.q0 + i) * p.heads + head] = sum == 0.f ? -INFINITY : m + __log2f(sum);
+  store4<T>(p.o + ((int64_t)(it.q0 + i) * p.o_ts + (int64_t)head * p.o_hs + d) * 2, a[0] * inv, a[1] * inv, a[2] * inv, a[3] * inv);
 }
 
 // ---- host: plans ---------------------------------------------------------------------------
@@ -251,7 +258,7 @@ struct Lists {
   std::vector<RowItem> rows;
   std::vector<KeyItem> keys;
   std::vector<JoinItem> join;
-  int waves = 4, key_waves = 4, planes = 0;
+  int key_waves = 4, planes = 0, join_tokens = 0;
   int64_t prows = 0;
 };
 
@@ -266,34 +273,22 @@ static int keys_of(const Seq& s, bool causal, int t, int n) {
   return (int)std::max<int64_t>(0, std::min<int64_t>(s.klen, (int64_t)s.klen - s.qlen + t + n));
 }
 
-// Forward lists. A tile takes `rows` rows; where there are fewer workgroups than fill the chip the key
-// ranges are cut and joined.
+// Row lists: a tile takes the rows of as many tokens of one sequence as fit. Where there are fewer
+// workgroups than fill the chip, key ranges are cut into pieces and joined; a shared prefix is read
+// within each sequence's tiles or, where those are mostly empty, by tiles over all tokens, and joined.
 static void plan_rows(const std::vector<Seq>& seqs, const ahr_attn_shape& sh, int64_t prefix, bool may_split, Lists& L) {
   const int G = sh.heads / sh.kv_heads;
-  int64_t total = 0;
-  for (const Seq& s : seqs) total += s.qlen;
-  auto tiles_at = [&](int rows) {  // row tiles when a tile holds whole tokens of one sequence
-    const int per = std::max(1, rows / G);
-    int64_t n = 0;
-    for (const Seq& s : seqs) n += up(s.qlen, per);
-    return n;
-  };
-  int waves = 4;
-  const int least = (G + 31) / 32 <= 1 ? 1 : ((G + 31) / 32 <= 2 ? 2 : 4);
-  while (waves > least && (tiles_at(waves * 32) * sh.kv_heads < 512 ||
-                           tiles_at(waves * 32) * waves > tiles_at(least * 32) * least * 5 / 4))
-    waves /= 2;
-  L.waves = waves;
-  const int per = std::max(1, waves * 32 / G);  // tokens of a tile
-
-  // the shared prefix: read within each sequence's tiles, or by tiles over all tokens and joined
-  const int64_t ptiles = up(prefix, kKeys);
-  bool apart = false;
-  if (prefix > 0) {
-    const int64_t within = tiles_at(waves * 32), across = up(total, per);
-    apart = may_split && (across * 5 < within * 4 || within * sh.kv_heads < 512);
+  const int per = kRows / G;  // tokens of a tile
+  int64_t total = 0, tiles = 0, waves = 0;
+  for (const Seq& s : seqs) {
+    total += s.qlen;
+    tiles += up(s.qlen, per);
+    waves += up((int64_t)s.qlen * G, 32);
   }
-  struct Part { size_t item; int pieces; };
+  const int64_t ptiles = up(prefix, kKeys), across = up(total, per);
+  // (prefix 4000, 64 sequences of 10 tokens, 32/8 heads of 64: within 94 us, apart 49; 64 of 57 tokens,
+  // 16/8 heads, prefix 900: within 33, apart 42; equal where the waves of the former hold 1.5 times the rows)
+  const bool apart = prefix > 0 && may_split && 2 * waves > 3 * up(total * G, 32);
   std::vector<RowItem> base;
   std::vector<int> load;
   for (const Seq& s : seqs)
@@ -311,15 +306,19 @@ static void plan_rows(const std::vector<Seq>& seqs, const ahr_attn_shape& sh, in
       base.push_back(r);
       load.push_back((int)(up(r.ke, kKeys) + (apart ? 0 : ptiles)));
     }
-  const int64_t prow_all = apart ? total : 0;
   int64_t work = 0;
   for (int x : load) work += x;
-  const int64_t ptl = apart ? up(total, per) : 0;  // prefix row tiles
+  const int64_t ptl = apart ? across : 0;  // prefix row tiles
   work += ptl * ptiles;
   const int64_t blocks = ((int64_t)base.size() + ptl) * sh.kv_heads;
-  // pieces of about `chunk` key tiles, at least four (256 keys), so that about 1024 workgroups run
+  // Pieces of about `chunk` key tiles, at least four (256 keys). Tiles of one wave's rows stream their
+  // keys from memory and gain from many workgroups (24 sequences of one token over 1k-33k keys, 8 key heads
+  // of 128: 512 / 1024 / 2048 / 4096 pieces 295 / 279 / 258 / 278 us); fuller ones compute, and take one
+  // round of resident workgroups (200 tokens, 32/8 heads, prefix 16000: 256 / 512 / 1024 / 2048 110 / 93 /
+  // 100 / 120 us).
+  const int64_t want = !apart && waves <= tiles ? 2048 : 512;
   int64_t chunk = INT32_MAX;
-  if (may_split && (blocks < 512 || apart)) chunk = std::max<int64_t>(4, up(work * sh.kv_heads, 1024));
+  if (may_split && (blocks < 512 || apart)) chunk = std::max<int64_t>(4, up(work * sh.kv_heads, want));
 
   int prefix_pieces = 0;
   if (apart) {
@@ -339,7 +338,7 @@ static void plan_rows(const std::vector<Seq>& seqs, const ahr_attn_shape& sh, in
         L.rows.push_back(r);
       }
     L.planes = prefix_pieces;
-    L.prows = prow_all;
+    L.prows = total;
   }
   for (size_t b = 0; b < base.size(); ++b) {
     RowItem r = base[b];
@@ -368,6 +367,7 @@ static void plan_rows(const std::vector<Seq>& seqs, const ahr_attn_shape& sh, in
     L.planes = std::max(L.planes, made);
     if (!apart) L.prows += r.nq;
     L.join.push_back(JoinItem{r.q0, r.nq, (int32_t)prow, made});
+    L.join_tokens = std::max(L.join_tokens, r.nq);
   }
   std::stable_sort(L.rows.begin(), L.rows.end(), [](const RowItem& a, const RowItem& b) {
     return (a.pe - a.pb) + (a.ke - a.kb) > (b.pe - b.pb) + (b.ke - b.kb);  // longest first
@@ -381,8 +381,7 @@ static void plan_keys(const std::vector<Seq>& seqs, const ahr_attn_shape& sh, Li
     return n;
   };
   int waves = 4;
-  while (waves > 1 && (tiles_at(waves * 32) * sh.kv_heads < 512 || tiles_at(waves * 32) * waves > tiles_at(32) * 5 / 4))
-    waves /= 2;
+  while (waves > 1 && tiles_at(waves * 32) * sh.kv_heads < 512) waves /= 2;
   L.key_waves = waves;
   const int per = waves * 32;
   for (const Seq& s : seqs)
@@ -437,7 +436,7 @@ static int build(const int32_t* q_len, const int32_t* k_len, int n, const ahr_at
   plan->n_rows = (int32_t)L.rows.size();
   plan->n_keys = (int32_t)L.keys.size();
   plan->n_join = (int32_t)L.join.size();
-  plan->waves = L.waves;
+  plan->join_tokens = L.join_tokens;
   plan->key_waves = L.key_waves;
   plan->planes = L.planes;
   plan->part_rows = L.prows;
@@ -518,33 +517,27 @@ static int fill(const ahr_attn_args* a, bool backward, Params* out) {
   return AHR_OK;
 }
 
-template <typename T, int DP, int NW>
-static int launch_fwd(const Params& p, hipStream_t s) {
+template <typename T, int DP>
+static int launch_fwd(const Params& p, int join_tokens, hipStream_t s) {
   constexpr int lds = 4 * kKeys * DP * 2;
   static std::atomic<uint64_t> done{0};
-  ensure_lds_attr(done, reinterpret_cast<const void*>(attn_fwd_kernel<T, DP, NW>), lds);
-  attn_fwd_kernel<T, DP, NW><<<dim3((unsigned)(p.n_rows * p.kv_heads)), NW * 64, lds, s>>>(p);
+  ensure_lds_attr(done, reinterpret_cast<const void*>(attn_fwd_kernel<T, DP>), lds);
+  attn_fwd_kernel<T, DP><<<dim3((unsigned)(p.n_rows * p.kv_heads)), kWaves * 64, lds, s>>>(p);
   AHR_HIP(hipGetLastError());
   if (p.n_join) {
-    attn_join_kernel<T><<<dim3((unsigned)(p.n_join * p.heads)), 256, 0, s>>>(p);
+    const int lanes = p.dim <= 32 ? 8 : (p.dim <= 64 ? 16 : 32), per = 256 / lanes;
+    attn_join_kernel<T><<<dim3((unsigned)p.n_join, (unsigned)((join_tokens * p.heads + per - 1) / per)), 256, 0, s>>>(p, lanes);
     AHR_HIP(hipGetLastError());
   }
   return AHR_OK;
 }
 
-template <typename T, int DP>
-static int launch_fwd_w(const Params& p, int waves, hipStream_t s) {
-  if (waves == 1) return launch_fwd<T, DP, 1>(p, s);
-  if (waves == 2) return launch_fwd<T, DP, 2>(p, s);
-  return launch_fwd<T, DP, 4>(p, s);
-}
-
 template <typename T>
-static int launch_fwd_d(const Params& p, int waves, hipStream_t s) {
-  if (p.dim <= 32) return launch_fwd_w<T, 32>(p, waves, s);
-  if (p.dim <= 64) return launch_fwd_w<T, 64>(p, waves, s);
-  if (p.dim <= 96) return launch_fwd_w<T, 96>(p, waves, s);
-  return launch_fwd_w<T, 128>(p, waves, s);
+static int launch_fwd_d(const Params& p, int join_tokens, hipStream_t s) {
+  if (p.dim <= 32) return launch_fwd<T, 32>(p, join_tokens, s);
+  if (p.dim <= 64) return launch_fwd<T, 64>(p, join_tokens, s);
+  if (p.dim <= 96) return launch_fwd<T, 96>(p, join_tokens, s);
+  return launch_fwd<T, 128>(p, join_tokens, s);
 }
 
 }  // namespace attn
@@ -572,8 +565,8 @@ int ahr_attn_forward(const ahr_attn_args* a, void* stream) {
   if (st != AHR_OK) return st;
   if (p.n_rows == 0) return AHR_OK;
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  if (a->plan->shape.dtype == AHR_BF16) return attn::launch_fwd_d<__bf16>(p, a->plan->waves, s);
-  return attn::launch_fwd_d<_Float16>(p, a->plan->waves, s);
+  if (a->plan->shape.dtype == AHR_BF16) return attn::launch_fwd_d<__bf16>(p, a->plan->join_tokens, s);
+  return attn::launch_fwd_d<_Float16>(p, a->plan->join_tokens, s);
 }
 
 int ahr_attn_backward(const ahr_attn_args* a, void* stream) {

@@ -23,26 +23,6 @@ __device__ __forceinline__ float pick_scale(float largest) {
 }
 // (p <= 1 is held times 2^14 for dv.)
 
-// delta[t][head] = sum_d do o: 8 elements a lane, 16 lanes a row
-template <typename T>
-__global__ __launch_bounds__(256) void attn_delta_kernel(Params p, int64_t rows) {
-  typedef typename Elem<T>::v8 v8;
-  const int64_t r = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4);
-  const int d = (threadIdx.x & 15) * 8;
-  float x = 0.f;
-  if (r < rows && d < p.dim) {
-    const int64_t t = r / p.heads;
-    const int hd = (int)(r - t * p.heads);
-    const v8 a = *reinterpret_cast<const v8*>(p.o + (t * p.o_ts + hd * p.o_hs + d) * 2);
-    const v8 b = *reinterpret_cast<const v8*>(p.d_o + (t * p.do_ts + hd * p.do_hs + d) * 2);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x = fmaf((float)a[i], (float)b[i], x);
-  }
-#pragma unroll
-  for (int i = 1; i < 16; i *= 2) x += __shfl_xor(x, i, 64);
-  if (r < rows && d == 0) p.delta[r] = x;
-}
-
 // f16: ds of the tile times the state's factor, which is chosen and lowered here (ROW: one factor for each
 // row, held by its lane; else one for the wave). acc: the accumulators that hold ds already.
 template <int DB, bool ROW>
@@ -356,14 +336,14 @@ __device__ __forceinline__ void row_tile(const char* __restrict__ cur, RowState<
   }
 }
 
-template <typename T, int DP, int NW>
+template <typename T, int DP>
 __device__ __forceinline__ void row_step(const char* __restrict__ cur, char* __restrict__ nxt, RowState<T, DP>& st,
-                                         const Stager<DP / 8, NW, kKeys>& stager, const Params& p, const RowItem& it, int hk, int t, int nt,
+                                         const Stager<DP / 8, kWaves, kKeys>& stager, const Params& p, const RowItem& it, int hk, int t, int nt,
                                          bool wave_live, int lim, int lim_lo, int lim_hi, int lane) {
   if (t + 1 < nt) {
     const int kt = (t + 1) * kKeys;
     const int64_t at = (int64_t)it.k0 + kt;
-    stage_kv<DP, NW>(nxt, stager, p.k + (at * p.k_ts + (int64_t)hk * p.k_hs) * 2, p.v + (at * p.v_ts + (int64_t)hk * p.v_hs) * 2, p.k_ts, p.v_ts,
+    stage_kv<DP>(nxt, stager, p.k + (at * p.k_ts + (int64_t)hk * p.k_hs) * 2, p.v + (at * p.v_ts + (int64_t)hk * p.v_hs) * 2, p.k_ts, p.v_ts,
                      min(kKeys, it.ke - kt), p.dim);
   }
   if (t < 0) return;
@@ -373,8 +353,8 @@ __device__ __forceinline__ void row_step(const char* __restrict__ cur, char* __r
 }
 
 // dq of the rows of one item, 32 a wave
-template <typename T, int DP, int NW>
-__global__ __launch_bounds__(NW * 64, 2) void attn_dq_kernel(Params p) {
+template <typename T, int DP>
+__global__ __launch_bounds__(kWaves * 64, 2) void attn_dq_kernel(Params p) {
   typedef typename Elem<T>::v8 v8;
   constexpr int KS = DP / 16, DB = DP / 32;
   constexpr int kTile = kKeys * DP * 2;
@@ -385,7 +365,7 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_dq_kernel(Params p) {
   const RowItem it = p.rows[blockIdx.x / p.kv_heads];
   const int dim = p.dim;
   if (DP != dim) {
-    for (int i = threadIdx.x; i < 4 * kTile / 16; i += NW * 64) reinterpret_cast<f32x4*>(smem)[i] = f32x4{0, 0, 0, 0};
+    for (int i = threadIdx.x; i < 4 * kTile / 16; i += kWaves * 64) reinterpret_cast<f32x4*>(smem)[i] = f32x4{0, 0, 0, 0};
     __syncthreads();
   }
   const int n_rows = it.nq * p.group;
@@ -413,20 +393,35 @@ __global__ __launch_bounds__(NW * 64, 2) void attn_dq_kernel(Params p) {
   }
   const int64_t li = (int64_t)(it.q0 + tok) * p.heads + head;
   st.lse = live ? p.lse[li] : 0.f;
-  st.delta = live ? p.delta[li] : 0.f;
+  // delta = sum_d do o of this lane's row, written for the dk/dv kernel that follows
+  {
+    const char* op = p.o + ((int64_t)(it.q0 + tok) * p.o_ts + (int64_t)head * p.o_hs) * 2;
+    float x = 0.f;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      const int d = (2 * ks + h) * 8;
+      if (live && (DP == dim || d < dim)) {
+        const v8 o = *reinterpret_cast<const v8*>(op + d * 2);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x = fmaf((float)o[i], (float)st.of[ks][i], x);
+      }
+    }
+    st.delta = x + other_half(x);
+    if (live && h == 0) p.delta[li] = st.delta;
+  }
   st.sc = Elem<T>::kNarrow ? 0.f : 1.f;
 #pragma unroll
   for (int b = 0; b < DB; ++b)
 #pragma unroll
     for (int r = 0; r < 16; ++r) st.acc[b][r] = 0.f;
 
-  const Stager<DP / 8, NW, kKeys> stager(wave, lane);
+  const Stager<DP / 8, kWaves, kKeys> stager(wave, lane);
   const int nt = (it.ke + kKeys - 1) / kKeys;
   if (nt > 0) {
-    row_step<T, DP, NW>(smem, smem, st, stager, p, it, hk, -1, nt, false, 0, 0, 0, lane);
+    row_step<T, DP>(smem, smem, st, stager, p, it, hk, -1, nt, false, 0, 0, 0, lane);
     for (int t = 0; t < nt; ++t) {
       tile_barrier();
-      row_step<T, DP, NW>(smem + (t & 1) * 2 * kTile, smem + ((t + 1) & 1) * 2 * kTile, st, stager, p, it, hk, t, nt, wave_live, lim, lim_lo,
+      row_step<T, DP>(smem + (t & 1) * 2 * kTile, smem + ((t + 1) & 1) * 2 * kTile, st, stager, p, it, hk, t, nt, wave_live, lim, lim_lo,
                           lim_hi, lane);
     }
   }
@@ -457,40 +452,30 @@ static int launch_dkv(const Params& p, hipStream_t s) {
   return AHR_OK;
 }
 
-template <typename T, int DP, int NW>
+template <typename T, int DP>
 static int launch_dq(const Params& p, hipStream_t s) {
   constexpr int lds = 4 * kKeys * DP * 2;
   static std::atomic<uint64_t> done{0};
-  ensure_lds_attr(done, reinterpret_cast<const void*>(attn_dq_kernel<T, DP, NW>), lds);
-  attn_dq_kernel<T, DP, NW><<<dim3((unsigned)(p.n_rows * p.kv_heads)), NW * 64, lds, s>>>(p);
+  ensure_lds_attr(done, reinterpret_cast<const void*>(attn_dq_kernel<T, DP>), lds);
+  attn_dq_kernel<T, DP><<<dim3((unsigned)(p.n_rows * p.kv_heads)), kWaves * 64, lds, s>>>(p);
   AHR_HIP(hipGetLastError());
   return AHR_OK;
 }
 
 template <typename T, int DP>
 static int launch_bwd_d(const ahr_attn_plan& pl, const Params& p, hipStream_t s) {
-  int st = AHR_OK;
-  if (p.n_keys) {
-    if (pl.key_waves == 1) st = launch_dkv<T, DP, 1, 4>(p, s);
-    else if (pl.key_waves == 2) st = launch_dkv<T, DP, 2, 2>(p, s);
-    else st = launch_dkv<T, DP, 4, 1>(p, s);
+  if (p.n_rows) {
+    const int st = launch_dq<T, DP>(p, s);  // writes delta, so it comes first
     if (st != AHR_OK) return st;
   }
-  if (p.n_rows) {
-    if (pl.waves == 1) st = launch_dq<T, DP, 1>(p, s);
-    else if (pl.waves == 2) st = launch_dq<T, DP, 2>(p, s);
-    else st = launch_dq<T, DP, 4>(p, s);
-  }
-  return st;
+  if (!p.n_keys) return AHR_OK;
+  if (pl.key_waves == 1) return launch_dkv<T, DP, 1, 4>(p, s);
+  if (pl.key_waves == 2) return launch_dkv<T, DP, 2, 2>(p, s);
+  return launch_dkv<T, DP, 4, 1>(p, s);
 }
 
 template <typename T>
 static int launch_bwd(const ahr_attn_plan& pl, const Params& p, hipStream_t s) {
-  const int64_t rows = pl.tokens * p.heads;
-  if (rows > 0) {
-    attn_delta_kernel<T><<<dim3((unsigned)((rows + 15) / 16)), 256, 0, s>>>(p, rows);
-    AHR_HIP(hipGetLastError());
-  }
   if (p.dim <= 32) return launch_bwd_d<T, 32>(pl, p, s);
   if (p.dim <= 64) return launch_bwd_d<T, 64>(pl, p, s);
   if (p.dim <= 96) return launch_bwd_d<T, 96>(pl, p, s);

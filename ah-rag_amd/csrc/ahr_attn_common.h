@@ -136,8 +136,8 @@ if (dim == NC * 8) {
 };
 
 // Keys and values [kt, kt + have) of one key head into a buffer.
-template <int DP, int NW>
-__device__ __forceinline__ void stage_kv(char* __restrict__ nxt, const Stager<DP / 8, NW, kKeys>& stager, const char* k, const char* v,
+template <int DP>
+__device__ __forceinline__ void stage_kv(char* __restrict__ nxt, const Stager<DP / 8, kWaves, kKeys>& stager, const char* k, const char* v,
                                          int64_t kts, int64_t vts, int have, int dim) {
   const int kst = (int)kts * 2, vst = (int)vts * 2;
   const __amdgpu_buffer_rsrc_t kr = dense::tile_rsrc_u(k, (uint32_t)((have - 1) * kst + dim * 2));

@@ -287,6 +287,7 @@ __global__ __launch_bounds__(256) void rope_dw_kernel(const float* part, int blo
   const int col = blockIdx.x * 16 + (threadIdx.x & 15), y = threadIdx.x >> 4;
   float s = 0.f;
   if (col < 2 * dim)
+#pragma unroll 8
     for (int b = y; b < blocks; b += 16) s += part[(int64_t)b * 2 * dim + col];
   acc[y][threadIdx.x & 15] = s;
   __syncthreads();

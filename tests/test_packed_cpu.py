@@ -62,7 +62,7 @@ def test_row_lists_cover_every_pair_once(case):
     pre = [np.zeros(prefix, int) for _ in range(T)]
     planes, final = [set() for _ in range(T)], np.zeros(T, int)
     for r in rows:
-        assert 0 < r["nq"] and r["nq"] * group <= plan.waves * 32
+        assert 0 < r["nq"] and r["nq"] * group <= 128
         assert 0 <= r["q0"] and r["q0"] + r["nq"] <= T
         assert 0 <= r["pb"] <= r["pe"] <= prefix and 0 <= r["kb"] <= r["ke"]
         if r["ke"] > r["kb"]:
