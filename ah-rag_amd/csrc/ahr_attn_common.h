@@ -109,28 +109,32 @@ __device__ __forceinline__ void store4(char* p, float a, float b, float c, float
   *reinterpret_cast<typename Elem<T>::v4*>(p) = x;
 }
 
-// LDS-DMA of tile rows: the NC * ROWS / 64 16-B-per-lane loads are dealt to the NW waves.
+// LDS-DMA of a tile of ROWS rows: its NC * ROWS / 64 loads of 16 B a lane are dealt to the NW waves. A
+// wave's loads are kStep rows apart; where the swizzle repeats after that many rows (all but NC = 12),
+// its lanes keep one row and chunk, and the step goes into the scalar offset.
 template <int NC, int NW, int ROWS>
 struct Stager {
   static constexpr int kPer = NC * ROWS / 64 / NW;
-  int wave, lane;
-  __device__ __forceinline__ Stager(int w, int l) : wave(w), lane(l) {}
-  // off(row) -> byte offset of the row from the descriptor's base (rows past the range repeat a
-  // valid one: every load stays inside the tensors). Chunks past dim are left alone (zeroed once).
+  static constexpr int kStep = NC == 12 ? 0 : NW * 64 / NC;
+  int wave, lane, row0, c0;
+  __device__ __forceinline__ Stager(int w, int l) : wave(w), lane(l) {
+    row0 = (w * 64 + l) / NC;
+    c0 = ((w * 64 + l) % NC) ^ swz<NC>(row0);
+  }
+  // a whole tile of NC * 8 = dim elements: row r lies at row_off (of row0) + (r - row0) / kStep * step
+  __device__ __forceinline__ void load_full(__amdgpu_buffer_rsrc_t r, char* tile, int row_off, int step) const {
+    const uint32_t v = (uint32_t)(row_off + c0 * 16);
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) dense::blds16_soff(r, v, (uint32_t)(i * step), tile + (i * NW + wave) * 1024);
+  }
+  // any: off(row) -> byte offset of the row from the descriptor's base (rows past the range repeat a valid
+  // one: every load stays inside the tensors). Chunks past dim are left alone (zeroed once).
   template <typename F>
   __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t r, char* tile, int dim, F off) const {
-if (dim == NC * 8) {
 #pragma unroll
-      for (int i = 0; i < kPer; ++i) {
-        const int ci = (i * NW + wave) * 64 + lane, row = ci / NC, c = (ci % NC) ^ swz<NC>(row);
-        dense::blds16(r, (uint32_t)(off(row) + c * 16), tile + (i * NW + wave) * 1024);
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < kPer; ++i) {
-        const int ci = (i * NW + wave) * 64 + lane, row = ci / NC, c = (ci % NC) ^ swz<NC>(row);
-        if (c * 8 < dim) dense::blds16(r, (uint32_t)(off(row) + c * 16), tile + (i * NW + wave) * 1024);
-      }
+    for (int i = 0; i < kPer; ++i) {
+      const int ci = (i * NW + wave) * 64 + lane, row = ci / NC, c = (ci % NC) ^ swz<NC>(row);
+      if (c * 8 < dim) dense::blds16(r, (uint32_t)(off(row) + c * 16), tile + (i * NW + wave) * 1024);
     }
   }
 };
@@ -142,8 +146,14 @@ __device__ __forceinline__ void stage_kv(char* __restrict__ nxt, const Stager<DP
   const int kst = (int)kts * 2, vst = (int)vts * 2;
   const __amdgpu_buffer_rsrc_t kr = dense::tile_rsrc_u(k, (uint32_t)((have - 1) * kst + dim * 2));
   const __amdgpu_buffer_rsrc_t vr = dense::tile_rsrc_u(v, (uint32_t)((have - 1) * vst + dim * 2));
-  stager.load(kr, nxt, dim, [&](int r) { return min(r, have - 1) * kst; });
-  stager.load(vr, nxt + kKeys * DP * 2, dim, [&](int r) { return min(r, have - 1) * vst; });
+  if (DP != 96 && dim == DP && have == kKeys) {
+    constexpr int step = Stager<DP / 8, kWaves, kKeys>::kStep;
+    stager.load_full(kr, nxt, __mul24(stager.row0, kst), step * kst);
+    stager.load_full(vr, nxt + kKeys * DP * 2, __mul24(stager.row0, vst), step * vst);
+  } else {
+    stager.load(kr, nxt, dim, [&](int r) { return __mul24(min(r, have - 1), kst); });
+    stager.load(vr, nxt + kKeys * DP * 2, dim, [&](int r) { return __mul24(min(r, have - 1), vst); });
+  }
 }
 
 }  // namespace attn

@@ -13,6 +13,8 @@
 namespace ahr {
 namespace packed {
 
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
 template <typename T, int N>
 __device__ __forceinline__ void load_f32(float* to, const T* from) {  // N consecutive, aligned to N * sizeof(T) or 16 B
   constexpr int W = (int)sizeof(T) * N >= 16 ? 16 / (int)sizeof(T) : N;
@@ -404,7 +406,7 @@ constexpr float kPoolEps = 1e-12f;
 
 // Sum of a chunk's rows: a workgroup per chunk and 64 * V columns, its four waves take every fourth row.
 template <typename T, int V>
-__global__ __launch_bounds__(256) void pool_sum_kernel(const T* rows, int64_t rs, int width, const int4* chunks, float* ws) {
+__global__ __launch_bounds__(256) void pool_sum_kernel(const T* rows, int64_t rs, int width, const int4* chunks, float* ws, int ld) {
   __shared__ float acc[4][64 * V];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int4 ch = chunks[blockIdx.x];
@@ -425,49 +427,70 @@ __global__ __launch_bounds__(256) void pool_sum_kernel(const T* rows, int64_t rs
 #pragma unroll
   for (int i = 0; i < V; ++i) acc[wave][i * 64 + lane] = s[i];
   __syncthreads();
-  float* o = ws + (int64_t)blockIdx.x * width + (int64_t)blockIdx.y * 64 * V;
+  float* o = ws + (int64_t)blockIdx.x * ld + (int64_t)blockIdx.y * 64 * V;
   for (int i = threadIdx.x; i < 64 * V; i += 256) {  // column i = lane' * V + part
     const int j = (i % V) * 64 + i / V;
-    if (blockIdx.y * 64 * V + i < width) o[i] = acc[0][j] + acc[1][j] + acc[2][j] + acc[3][j];
+    if (blockIdx.y * 64 * V + i < ld) o[i] = acc[0][j] + acc[1][j] + acc[2][j] + acc[3][j];  // (zeros past width)
   }
 }
 
+template <int WAVES>
 __device__ __forceinline__ float block_sum(float x, float* red) {
 #pragma unroll
   for (int m = 1; m < 64; m *= 2) x += __shfl_xor(x, m, 64);
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = x;
   __syncthreads();
-  x = red[0] + red[1] + red[2] + red[3];
+  x = 0.f;
+#pragma unroll
+  for (int i = 0; i < WAVES; ++i) x += red[i];
   __syncthreads();
   return x;
 }
 
-// mean and norm of a sequence: its chunks' sums in order
-__global__ __launch_bounds__(256) void pool_mean_kernel(const float* ws, int width, const int2* seqs, int normalize, float* out,
-                                                        float* norm) {
-  __shared__ float red[4];
-  const int2 sq = seqs[blockIdx.x];
-  const int n = (sq.x + AHR_POOL_CHUNK - 1) / AHR_POOL_CHUNK;
+// Mean and norm of a sequence: the sums of its chunks in a fixed order, four chunks at a time and 4
+// columns a thread (a long document's partial rows are all that one workgroup has to read: wide loads,
+// several in flight, 63 partial rows of 1024 in 7 us, 118 with one column a thread).
+__global__ __launch_bounds__(1024) void pool_mean_kernel(const float* ws, int ld, int width, const int4* seqs, int normalize, float* out,
+                                                         float* norm) {
+  __shared__ f32x4 part[4][256];
+  __shared__ float red[16];
+  const int4 sq = seqs[blockIdx.x];  // rows, first chunk, chunks
+  const int x = threadIdx.x & 255, y = threadIdx.x >> 8;
   float* o = out + (int64_t)blockIdx.x * width;
   float ss = 0.f;
-  for (int c = threadIdx.x; c < width; c += 256) {
-    float s = 0.f;
-    for (int i = 0; i < n; ++i) s += ws[(int64_t)(sq.y + i) * width + c];
-    s = sq.x > 0 ? s / (float)sq.x : 0.f;
-    o[c] = s;
-    ss = fmaf(s, s, ss);
+  for (int g0 = 0; g0 < ld / 4; g0 += 256) {
+    const int g = g0 + x;
+    f32x4 s = {0, 0, 0, 0};
+    if (g < ld / 4) {
+      const f32x4* p = reinterpret_cast<const f32x4*>(ws + (int64_t)sq.y * ld) + g;
+#pragma unroll 8
+      for (int i = y; i < sq.z; i += 4) s += p[(int64_t)i * (ld / 4)];
+    }
+    part[y][x] = s;
+    __syncthreads();
+    if (y == 0 && g < ld / 4) {
+      s = part[0][x] + part[1][x] + part[2][x] + part[3][x];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float v = sq.x > 0 ? s[i] / (float)sq.x : 0.f;
+        if (g * 4 + i < width) o[g * 4 + i] = v;
+        ss = fmaf(v, v, ss);  // (zeros past width)
+      }
+    }
+    __syncthreads();
   }
-  const float nm = sqrtf(block_sum(ss, red));
+  const float nm = sqrtf(block_sum<16>(ss, red));
   if (threadIdx.x == 0 && norm) norm[blockIdx.x] = nm;
-  if (!normalize) return;
+  if (!normalize || y != 0) return;
   const float d = fmaxf(nm, kPoolEps);
-  for (int c = threadIdx.x; c < width; c += 256) o[c] /= d;  // (each thread its own values)
+  for (int g = x; g < ld / 4; g += 256)
+    for (int c = g * 4; c < min(width, g * 4 + 4); ++c) o[c] /= d;  // (each thread its own values)
 }
 
 // Gradient of the rows: the same for every row of a sequence, (d_out - out (out . d_out)) / (norm rows),
 // written to the rows of one chunk.
 template <typename T, int V>
-__global__ __launch_bounds__(256) void pool_grad_kernel(T* d_rows, int width, const int4* chunks, const int2* seqs, int normalize,
+__global__ __launch_bounds__(256) void pool_grad_kernel(T* d_rows, int width, const int4* chunks, const int4* seqs, int normalize,
                                                         const float* d_out, const float* out, const float* norm) {
   __shared__ float red[4];
   const int4 ch = chunks[blockIdx.x];
@@ -479,7 +502,7 @@ __global__ __launch_bounds__(256) void pool_grad_kernel(T* d_rows, int width, co
     if (nm >= kPoolEps) {  // below it the division is by a constant
       for (int c = threadIdx.x; c < width; c += 256) dot = fmaf(dy[c], y[c], dot);
     }
-    dot = block_sum(dot, red);
+    dot = block_sum<4>(dot, red);
     d = fmaxf(nm, kPoolEps);
   }
   const float f = 1.f / (d * (float)seqs[ch.z].x);
@@ -493,18 +516,18 @@ __global__ __launch_bounds__(256) void pool_grad_kernel(T* d_rows, int width, co
 }
 
 template <typename T>
-static int pool_sum(const void* rows, int64_t rs, int width, const int4* chunks, int n_chunks, float* ws, hipStream_t s) {
+static int pool_sum(const void* rows, int64_t rs, int width, const int4* chunks, int n_chunks, float* ws, int ld, hipStream_t s) {
   constexpr int V = 16 / (int)sizeof(T);
   if (width % V == 0 && rs % V == 0 && reinterpret_cast<uintptr_t>(rows) % 16 == 0)
-    pool_sum_kernel<T, V><<<dim3(n_chunks, (width + 64 * V - 1) / (64 * V)), 256, 0, s>>>((const T*)rows, rs, width, chunks, ws);
+    pool_sum_kernel<T, V><<<dim3(n_chunks, (width + 64 * V - 1) / (64 * V)), 256, 0, s>>>((const T*)rows, rs, width, chunks, ws, ld);
   else
-    pool_sum_kernel<T, 1><<<dim3(n_chunks, (width + 63) / 64), 256, 0, s>>>((const T*)rows, rs, width, chunks, ws);
+    pool_sum_kernel<T, 1><<<dim3(n_chunks, (width + 63) / 64), 256, 0, s>>>((const T*)rows, rs, width, chunks, ws, ld);
   AHR_HIP(hipGetLastError());
   return AHR_OK;
 }
 
 template <typename T>
-static int pool_grad(void* d_rows, int width, const int4* chunks, int n_chunks, const int2* seqs, int normalize,
+static int pool_grad(void* d_rows, int width, const int4* chunks, int n_chunks, const int4* seqs, int normalize,
                      const float* d_out, const float* out, const float* norm, hipStream_t s) {
   constexpr int V = 16 / (int)sizeof(T);
   if (width % V == 0 && reinterpret_cast<uintptr_t>(d_rows) % 16 == 0)
@@ -533,28 +556,33 @@ int ahr_qk_norm_rope_backward(const ahr_rope_args* a, void* stream) { return ahr
 int ahr_pool_plan_build(const int32_t* lengths, int n, int32_t* buf, int64_t cap, int* n_chunks) {
   using namespace ahr;
   if (n < 0 || (n > 0 && !lengths) || !n_chunks) return fail(AHR_EINVAL, "null lengths or output");
-  int64_t count = 0, tokens = 0;
+  int64_t tokens = 0, count = 0;
   for (int i = 0; i < n; ++i) {
     if (lengths[i] < 0) return fail(AHR_EINVAL, "negative length");
-    count += ((int64_t)lengths[i] + AHR_POOL_CHUNK - 1) / AHR_POOL_CHUNK;
     tokens += lengths[i];
   }
   if (tokens > INT32_MAX / 2) return fail(AHR_EINVAL, "more than 2^30 packed tokens");
+  // rows of a chunk: as few as keep about 512 chunks (each of which leaves a partial row to be added)
+  int64_t rows = 64;
+  while (rows < 1024 && rows * 512 < tokens) rows *= 2;
+  for (int i = 0; i < n; ++i) count += (lengths[i] + rows - 1) / rows;
   *n_chunks = (int)count;
   if (!buf) return AHR_OK;
-  if (cap < count * 4 + (int64_t)n * 2) return fail(AHR_EINVAL, "buffer smaller than the lists");
-  int32_t* c = buf;
-  int32_t* s = buf + count * 4;
-  int32_t row = 0, made = 0;
-  for (int i = 0; i < n; ++i) {
-    s[2 * i] = lengths[i];
-    s[2 * i + 1] = made;
-    for (int32_t t = 0; t < lengths[i]; t += AHR_POOL_CHUNK, ++made, c += 4) {
-      c[0] = row + t;
-      c[1] = std::min<int32_t>(AHR_POOL_CHUNK, lengths[i] - t);
+  if (cap < (count + n) * 4) return fail(AHR_EINVAL, "buffer smaller than the lists");
+  int32_t *c = buf, *s = buf + count * 4;
+  int64_t row = 0;
+  int32_t made = 0;
+  for (int i = 0; i < n; ++i, s += 4) {
+    s[0] = lengths[i];
+    s[1] = made;
+    for (int64_t t = 0; t < lengths[i]; t += rows, ++made, c += 4) {
+      c[0] = (int32_t)(row + t);
+      c[1] = (int32_t)std::min<int64_t>(rows, lengths[i] - t);
       c[2] = i;
       c[3] = 0;
     }
+    s[2] = made - s[1];
+    s[3] = 0;
     row += lengths[i];
   }
   return AHR_OK;
@@ -575,17 +603,18 @@ int ahr_pool_mean(int dtype, const void* rows, int64_t rs, int width, const int3
   if (st != AHR_OK) return st;
   if (n == 0) return AHR_OK;
   if (!out || rs < 0 || (n_chunks > 0 && (!rows || !ws))) return fail(AHR_EINVAL, "null tensor or negative stride");
-  if (ws_bytes < (int64_t)n_chunks * width * 4) return fail(AHR_EINVAL, "workspace too small");
+  const int ld = (width + 3) / 4 * 4;
+  if (ws_bytes < (int64_t)n_chunks * ld * 4 || reinterpret_cast<uintptr_t>(ws) % 16) return fail(AHR_EINVAL, "workspace too small, or not aligned");
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   const int4* ch = reinterpret_cast<const int4*>(lists);
-  const int2* sq = reinterpret_cast<const int2*>(lists + (int64_t)n_chunks * 4);
+  const int4* sq = reinterpret_cast<const int4*>(lists + (int64_t)n_chunks * 4);
   if (n_chunks > 0) {
-    if (dtype == AHR_F32) st = packed::pool_sum<float>(rows, rs, width, ch, n_chunks, ws, s);
-    else if (dtype == AHR_F16) st = packed::pool_sum<_Float16>(rows, rs, width, ch, n_chunks, ws, s);
-    else st = packed::pool_sum<__bf16>(rows, rs, width, ch, n_chunks, ws, s);
+    if (dtype == AHR_F32) st = packed::pool_sum<float>(rows, rs, width, ch, n_chunks, ws, ld, s);
+    else if (dtype == AHR_F16) st = packed::pool_sum<_Float16>(rows, rs, width, ch, n_chunks, ws, ld, s);
+    else st = packed::pool_sum<__bf16>(rows, rs, width, ch, n_chunks, ws, ld, s);
     if (st != AHR_OK) return st;
   }
-  packed::pool_mean_kernel<<<n, 256, 0, s>>>(ws, width, sq, normalize, out, norm);
+  packed::pool_mean_kernel<<<n, 1024, 0, s>>>(ws, ld, width, sq, normalize, out, norm);
   AHR_HIP(hipGetLastError());
   return AHR_OK;
 }
@@ -599,7 +628,7 @@ int ahr_pool_mean_backward(int dtype, void* d_rows, int width, const int32_t* li
   if (!d_rows || !d_out || (normalize && (!out || !norm))) return fail(AHR_EINVAL, "null tensor");
   hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   const int4* ch = reinterpret_cast<const int4*>(lists);
-  const int2* sq = reinterpret_cast<const int2*>(lists + (int64_t)n_chunks * 4);
+  const int4* sq = reinterpret_cast<const int4*>(lists + (int64_t)n_chunks * 4);
   if (dtype == AHR_F32) return packed::pool_grad<float>(d_rows, width, ch, n_chunks, sq, normalize, d_out, out, norm, s);
   if (dtype == AHR_F16) return packed::pool_grad<_Float16>(d_rows, width, ch, n_chunks, sq, normalize, d_out, out, norm, s);
   return packed::pool_grad<__bf16>(d_rows, width, ch, n_chunks, sq, normalize, d_out, out, norm, s);

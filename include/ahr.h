@@ -445,14 +445,13 @@ int ahr_qk_norm_rope(const ahr_rope_args* a, void* stream);
 int ahr_qk_norm_rope_backward(const ahr_rope_args* a, void* stream);
 
 /* Mean over the rows of each sequence in fp32, then (normalize) division by max(L2 norm, 1e-12).
- * The work lists of a batch's lengths (host int32 [n]) are laid out once by ahr_pool_plan_build: chunks
- * of at most AHR_POOL_CHUNK rows, int32 [n_chunks][4], then int32 [n][2]; buf NULL: *n_chunks alone.
- * The caller copies them to the device (16-B aligned). */
-#define AHR_POOL_CHUNK 64
+ * The work lists of a batch's lengths (host int32 [n]) are laid out once by ahr_pool_plan_build: int32
+ * [n_chunks + n][4], {first row, rows, sequence, 0} of each chunk, {rows, first chunk, chunks, 0} of each
+ * sequence; buf NULL: *n_chunks alone. The caller copies them to the device (16-B aligned). */
 int ahr_pool_plan_build(const int32_t* lengths, int n, int32_t* buf, int64_t cap, int* n_chunks);
 /* rows [tokens][width] in dtype (AHR_F32 / F16 / BF16), row stride rs elements. out fp32 [n][width];
  * norm fp32 [n] (NULL: not wanted): the norm of the mean, for the backward pass. A sequence without
- * rows gives zeros. ws: n_chunks * width * 4 bytes. Capturable. */
+ * rows gives zeros. ws: n_chunks * (width rounded up to 4) * 4 bytes, 16-B aligned. Capturable. */
 int ahr_pool_mean(int dtype, const void* rows, int64_t rs, int width, const int32_t* lists, int n_chunks, int n,
                   int normalize, float* out, float* norm, float* ws, int64_t ws_bytes, void* stream);
 /* d_rows [tokens][width] (contiguous, dtype) from d_out, and out and norm of the forward pass, fp32. */

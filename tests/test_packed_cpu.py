@@ -177,19 +177,25 @@ def test_launch_refusals_without_a_device():
     assert lib.ahr_pool_mean(2, None, 0, 4, None, 0, 0, 0, None, None, None, 0, None) == nat.AHR_OK  # empty batch
 
 
-def test_pool_lists():
+@pytest.mark.parametrize("lens", [[0, 1, 64, 65, 0, 200], [0], [], [100000, 3, 0, 700]])
+def test_pool_lists(lens):
     from ah_rag import _native as nat
-    lens = np.asarray([0, 1, 64, 65, 0, 200], np.int32)
+    lens = np.asarray(lens, np.int32)
     n = ctypes.c_int()
-    buf = np.zeros(4 * 8 + 2 * len(lens), np.int32)
-    nat.check(nat.lib().ahr_pool_plan_build(lens.ctypes.data, len(lens), buf.ctypes.data, buf.size, ctypes.byref(n)))
-    assert n.value == 1 + 1 + 2 + 4
-    chunks, seqs = buf[:n.value * 4].reshape(-1, 4), buf[n.value * 4:].reshape(-1, 2)
-    assert chunks[:, 1].sum() == lens.sum() and (chunks[:, 0] == np.concatenate(([0], np.cumsum(chunks[:-1, 1])))).all()
+    nat.check(nat.lib().ahr_pool_plan_build(lens.ctypes.data, len(lens), None, 0, ctypes.byref(n)))
+    buf = np.full((n.value + len(lens)) * 4 + 1, -7, np.int32)
+    nat.check(nat.lib().ahr_pool_plan_build(lens.ctypes.data, len(lens), buf.ctypes.data, buf.size - 1, ctypes.byref(n)))
+    assert buf[-1] == -7
+    chunks, seqs = buf[:n.value * 4].reshape(-1, 4), buf[n.value * 4:-1].reshape(-1, 4)
+    assert chunks[:, 1].sum() == lens.sum() and (chunks[:, 1] > 0).all()
+    assert (chunks[:, 0] == np.concatenate(([0], np.cumsum(chunks[:, 1])))[:-1]).all()
     assert (seqs[:, 0] == lens).all()
     for i, m in enumerate(lens):
-        assert (chunks[seqs[i, 1]:seqs[i, 1] + (m + 63) // 64, 2] == i).all()
-    assert nat.lib().ahr_pool_plan_build(lens.ctypes.data, len(lens), buf.ctypes.data, 10, ctypes.byref(n)) == nat.AHR_EINVAL
+        mine = chunks[seqs[i, 1]:seqs[i, 1] + seqs[i, 2]]
+        assert (mine[:, 2] == i).all() and mine[:, 1].sum() == m
+    assert seqs[:, 2].sum() == n.value
+    if buf.size > 2:
+        assert nat.lib().ahr_pool_plan_build(lens.ctypes.data, len(lens), buf.ctypes.data, buf.size - 2, ctypes.byref(n)) == nat.AHR_EINVAL
 
 
 def test_layout_refusals():

@@ -276,14 +276,14 @@ def test_rows_outside_are_left_alone(cuda):
 def test_far_offsets(cuda):
     """Rows whose byte offsets pass 32 bits: the keys of the last sequence lie beyond 4 GiB."""
     from ah_rag.packed import PackedLayout, packed_attention
-    rows, wide = 300, 1 << 23  # 16 MiB from token to token: 4.7 GiB
+    rows, wide = 600, (1 << 22) - 64  # 8 MiB from token to token: 4.7 GiB
     buf = torch.empty(rows * wide, dtype=BF, device=cuda)
     g = torch.Generator().manual_seed(4)
     small = torch.randn(3, rows, 1, 64, generator=g).to(BF).to(cuda)
     views = [buf.view(rows, wide)[:, 64 * i:64 * i + 64].unsqueeze(1) for i in range(3)]
     for a, b in zip(views, small):
         a.copy_(b)
-    lay = PackedLayout([200, 100], device=cuda)
+    lay = PackedLayout([450, 150], device=cuda)
     leaves = [x.detach().requires_grad_() for x in views]
     dense = [x.detach().requires_grad_() for x in small]
     o, w = packed_attention(*leaves, lay, causal=True), packed_attention(*dense, lay, causal=True)
