@@ -51,6 +51,7 @@ __device__ __forceinline__ void fwd_tile(const char* __restrict__ cur, FwdState<
   for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
     for (int u = 0; u < 2; ++u) s[u] = Elem<T>::mma(row_frag<T, NC>(cur, u * 32 + n, ks, h), st.qf[ks], s[u]);
+  reads_ahead<2 * KS, 1>();
 
   if (cut) {  // keys that a row does not read: selected away, whatever their scores are
 #pragma unroll
@@ -92,6 +93,7 @@ __device__ __forceinline__ void fwd_tile(const char* __restrict__ cur, FwdState<
 #pragma unroll
     for (int b = 0; b < DB; ++b) st.acc[b] = Elem<T>::mma(col_frag<T, NC>(cur + kTile, g * 16, b, lane), pf, st.acc[b]);
   }
+  reads_ahead<4 * DB, 2>();
 }
 
 template <typename T, int DP>

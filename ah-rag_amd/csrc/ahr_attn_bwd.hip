@@ -76,6 +76,7 @@ __device__ __forceinline__ void key_tile(const char* __restrict__ q_lds, const c
   for (int ks = 0; ks < KS; ++ks) s = Elem<T>::mma(row_frag<T, NC>(q_lds, u0 + n, ks, h), st.kf[ks], s);
 #pragma unroll
   for (int ks = 0; ks < KS; ++ks) g = Elem<T>::mma(row_frag<T, NC>(o_lds, u0 + n, ks, h), st.vf[ks], g);
+  reads_ahead<2 * KS, 1>();
 #pragma unroll
   for (int r4 = 0; r4 < 4; ++r4) {
     const f32x4 ls = *reinterpret_cast<const f32x4*>(f + u0 + r4 * 8 + h * 4);
@@ -110,12 +111,22 @@ __device__ __forceinline__ void key_tile(const char* __restrict__ q_lds, const c
       st.gk[b] = Elem<T>::mma(col_frag<T, NC>(q_lds, u0 + k2 * 16, b, lane), df, st.gk[b]);
     }
   }
+  reads_ahead<4 * DB, 2>();
 }
 
-// The query rows of an item, tile by tile.
+// The query rows (token, head of the group) of an item from token t0 on, tile by tile: where a tile starts.
 struct KeyWalk {
-  int G, ginv, coff, n_tok;
+  int G, ginv, coff;
   int64_t n_rows;
+  int tok0, g0;  // first token (past t0) and head
+  __device__ __forceinline__ void next(int rows_tok, int rows_g) {  // rows of a tile = rows_tok * G + rows_g
+    tok0 += rows_tok;
+    g0 += rows_g;
+    if (g0 >= G) {
+      g0 -= G;
+      ++tok0;
+    }
+  }
 };
 
 template <typename T, int DP, int RW>
@@ -129,17 +140,16 @@ struct KeyCfg {
 template <typename T, int DP, int KW, int RW>
 __device__ __forceinline__ void key_step(const char* __restrict__ cur, char* __restrict__ nxt, KeyState<T, DP>& st,
                                          const Stager<DP / 8, KW * RW, KeyCfg<T, DP, RW>::kRows>& stager, const Params& p, const KeyItem& it,
-                                         const KeyWalk& w, int hk, int t, int nt, bool wave_live, int rw, int j, int j_hi, int lane) {
+                                         const KeyWalk& w, const KeyWalk& wn, int hk, int t, int nt, bool wave_live, int rw, int j, int j_hi, int lane) {
   typedef KeyCfg<T, DP, RW> Cfg;
   const int G = w.G;
   float st_l = 0.f, st_d = 0.f;  // lse and delta of the next tile's row, on their way to LDS
   if (t + 1 < nt) {
-    const int64_t r0 = (int64_t)(t + 1) * Cfg::kRows;
-    const int tok0 = (int)(r0 / G), g0 = (int)(r0 - (int64_t)tok0 * G);
-    const int have = (int)min((int64_t)Cfg::kRows, w.n_rows - r0);
+    const int tok0 = wn.tok0, g0 = wn.g0;
+    const int have = (int)min((int64_t)Cfg::kRows, w.n_rows - (int64_t)(t + 1) * Cfg::kRows);
     const int64_t at = it.q0 + it.t0 + tok0;
     const int qts = (int)p.q_ts * 2, qhs = (int)p.q_hs * 2, ots = (int)p.do_ts * 2, ohs = (int)p.do_hs * 2;
-    const uint32_t span = (uint32_t)((g0 + have - 1) / G);  // tokens past the first
+    const uint32_t span = (uint32_t)((g0 + have - 1) * w.ginv) >> 16;  // tokens past the first
     const __amdgpu_buffer_rsrc_t qr =
         dense::tile_rsrc_u(p.q + (at * p.q_ts + (int64_t)hk * G * p.q_hs) * 2, span * qts + (G - 1) * qhs + p.dim * 2);
     const __amdgpu_buffer_rsrc_t dr =
@@ -166,9 +176,8 @@ __device__ __forceinline__ void key_step(const char* __restrict__ cur, char* __r
     }
   }
   if (t >= 0 && wave_live) {
-    const int64_t r0 = (int64_t)t * Cfg::kRows;
-    const int tok0 = (int)(r0 / G), g0 = (int)(r0 - (int64_t)tok0 * G);
-    const int have = (int)min((int64_t)Cfg::kRows, w.n_rows - r0);
+    const int tok0 = w.tok0, g0 = w.g0;
+    const int have = (int)min((int64_t)Cfg::kRows, w.n_rows - (int64_t)t * Cfg::kRows);
     const float* f = reinterpret_cast<const float*>(cur + 2 * Cfg::kTile);
 #pragma unroll
     for (int u = 0; u < Cfg::kPer; ++u) {
@@ -239,22 +248,26 @@ __global__ __launch_bounds__(KW * RW * 64, DP > 64 ? 1 : 2) void attn_dkv_kernel
   w.G = p.group;
   w.ginv = p.group_inv;
   w.coff = it.klen - it.qlen;
-  w.n_tok = it.qlen - it.t0;              // query tokens that matter
-  w.n_rows = (int64_t)w.n_tok * p.group;  // and their rows
+  w.n_rows = (int64_t)(it.qlen - it.t0) * p.group;  // rows that may read the keys
+  w.tok0 = w.g0 = 0;
   const int nt = (int)((w.n_rows + Cfg::kRows - 1) / Cfg::kRows);
   const bool wave_live = kw * 32 < it.nk;
   const int j = it.kpos + key;                             // this lane's key in its sequence
   const int j_hi = it.kpos + min(kw * 32 + 31, it.nk - 1);  // the wave's last
   if (nt > 0) {
-    key_step<T, DP, KW, RW>(smem, smem, st, stager, p, it, w, hk, -1, nt, false, rw, j, j_hi, lane);
+    KeyWalk wn = w;
+    const int rows_tok = Cfg::kRows / p.group, rows_g = Cfg::kRows - rows_tok * p.group;
+    key_step<T, DP, KW, RW>(smem, smem, st, stager, p, it, w, wn, hk, -1, nt, false, rw, j, j_hi, lane);
     for (int t = 0; t < nt; ++t) {
+      wn.next(rows_tok, rows_g);
       tile_barrier();
-      if constexpr (DP > 64) {
+      if constexpr (DP > 64) {  // the sums stay in accumulation registers (moved to others and back each tile otherwise)
 #pragma unroll
         for (int b = 0; b < DB; ++b) asm volatile("" : "+a"(st.gk[b]), "+a"(st.gv[b]));
       }
-      key_step<T, DP, KW, RW>(smem + (t & 1) * Cfg::kBuf, smem + ((t + 1) & 1) * Cfg::kBuf, st, stager, p, it, w, hk, t, nt, wave_live, rw, j,
-                              j_hi, lane);
+      key_step<T, DP, KW, RW>(smem + (t & 1) * Cfg::kBuf, smem + ((t + 1) & 1) * Cfg::kBuf, st, stager, p, it, w, wn, hk, t, nt, wave_live, rw,
+                              j, j_hi, lane);
+      w = wn;
     }
   }
   float k_out = p.scale / (st.sc == 0.f ? 1.f : st.sc);
@@ -332,6 +345,7 @@ __device__ __forceinline__ void row_tile(const char* __restrict__ cur, RowState<
     for (int ks = 0; ks < KS; ++ks) s = Elem<T>::mma(row_frag<T, NC>(cur, u * 32 + n, ks, h), st.qf[ks], s);
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) g = Elem<T>::mma(row_frag<T, NC>(cur + kTile, u * 32 + n, ks, h), st.of[ks], g);
+    reads_ahead<2 * KS, 1>();
 #pragma unroll
     for (int r = 0; r < 16; ++r) g[r] = ex2(fmaf(s[r], c, -st.lse)) * (g[r] - st.delta);
     if (cut) {
@@ -345,6 +359,7 @@ __device__ __forceinline__ void row_tile(const char* __restrict__ cur, RowState<
 #pragma unroll
       for (int b = 0; b < DB; ++b) st.acc[b] = Elem<T>::mma(col_frag<T, NC>(cur, u * 32 + k2 * 16, b, lane), df, st.acc[b]);
     }
+    reads_ahead<2 * DB, 2>();
   }
 }
 

@@ -92,6 +92,22 @@ __device__ __forceinline__ void tile_barrier() {
   asm volatile("" ::: "memory");
 }
 
+// Asks the scheduler, for N matrix products of the block before it whose operands take R LDS reads each,
+// to keep the reads kAhead products ahead (left alone it reads each fragment right before its product,
+// which then waits out the LDS latency).
+constexpr int kAhead = 4;
+template <int N, int R>
+__device__ __forceinline__ void reads_ahead() {
+  constexpr int A = N < kAhead ? N : kAhead;
+  __builtin_amdgcn_sched_group_barrier(0x100, A * R, 0);  // 0x100: LDS reads, 8: matrix products
+#pragma unroll
+  for (int i = 0; i < N - A; ++i) {
+    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+    __builtin_amdgcn_sched_group_barrier(0x100, R, 0);
+  }
+  __builtin_amdgcn_sched_group_barrier(0x008, A, 0);
+}
+
 // row of a 32x32 accumulator register r in lane half h
 __device__ __forceinline__ int acc_row(int r, int h) { return (r & 3) + 8 * (r >> 2) + 4 * h; }
 
