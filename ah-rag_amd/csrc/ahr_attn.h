@@ -10,7 +10,7 @@ namespace attn {
 
 constexpr int kKeys = 64;     // keys of one staged tile
 constexpr int kWaves = 4;     // waves of a workgroup
-constexpr int kRows = 128;    // rows of a row tile: 32 a wave
+constexpr int kRows = 128;    // rows of a row tile, keys of a key tile: 32 a wave
 constexpr int kMaxDim = 128;  // head dimensions: multiples of 8 up to this
 constexpr int kMaxGroup = 128;  // query heads that share a key head
 
@@ -26,17 +26,17 @@ struct RowItem {
   int32_t pad;
 };
 
-// One workgroup's share of dk and dv, for each key head: nk keys against all the query rows of
-// their sequence that may read them.
+// One workgroup's share of dk and dv, for each key head: nk keys against query rows of their sequence.
 struct KeyItem {
   int32_t k0, nk;      // packed keys [k0, k0 + nk)
   int32_t kpos, klen;  // position of the first within the sequence, keys of the sequence
   int32_t q0, qlen;    // the sequence's packed query tokens
-  int32_t t0;          // first query token that may read any of them
-  int32_t pad;
+  int32_t t0, t1;      // query tokens [t0, t1) of the sequence (those before read none of the keys)
+  int32_t plane, prow; // partial sums: plane and row of the first key; plane < 0: final
+  int32_t pad[2];
 };
 
-// Tokens whose np partial results (planes 0..np-1) are joined.
+// Tokens (backward: keys) whose np partial results (planes 0..np-1) are joined.
 struct JoinItem {
   int32_t q0, nq, prow, np;
 };

@@ -260,7 +260,7 @@ struct Lists {
   std::vector<RowItem> rows;
   std::vector<KeyItem> keys;
   std::vector<JoinItem> join;
-  int key_waves = 4, planes = 0, join_tokens = 0;
+  int planes = 0, join_tokens = 0;
   int64_t prows = 0;
 };
 
@@ -376,32 +376,53 @@ static void plan_rows(const std::vector<Seq>& seqs, const ahr_attn_shape& sh, in
   });
 }
 
+// Key lists: a tile takes 128 keys of a sequence. Where few tiles have very unequal numbers of query rows
+// (long causal sequences), their rows are cut into pieces whose sums are added.
 static void plan_keys(const std::vector<Seq>& seqs, const ahr_attn_shape& sh, Lists& L) {
-  auto tiles_at = [&](int keys) {
-    int64_t n = 0;
-    for (const Seq& s : seqs) n += up(s.klen, keys);
-    return n;
-  };
-  int waves = 4;
-  while (waves > 1 && tiles_at(waves * 32) * sh.kv_heads < 512) waves /= 2;
-  if (getenv("XK")) waves = atoi(getenv("XK"));  // XX
-  L.key_waves = waves;
-  const int per = waves * 32;
+  const int G = sh.heads / sh.kv_heads;
+  std::vector<KeyItem> base;
+  int64_t work = 0;
+  auto tiles_of = [&](int tokens) { return up((int64_t)tokens * G, 64); };
   for (const Seq& s : seqs)
-    for (int j = 0; j < s.klen; j += per) {
+    for (int j = 0; j < s.klen; j += kRows) {
       KeyItem k;
       memset(&k, 0, sizeof k);
       k.k0 = (int32_t)(s.k0 + j);
-      k.nk = std::min(per, s.klen - j);
+      k.nk = std::min(kRows, s.klen - j);
       k.kpos = j;
       k.klen = s.klen;
       k.q0 = (int32_t)s.q0;
-      k.qlen = s.qlen;
+      k.qlen = k.t1 = s.qlen;
       k.t0 = sh.causal ? (int32_t)std::min<int64_t>(s.qlen, std::max<int64_t>(0, (int64_t)j - (s.klen - s.qlen))) : 0;
-      L.keys.push_back(k);
+      k.plane = -1;
+      base.push_back(k);
+      work += tiles_of(k.t1 - k.t0);
     }
-  std::stable_sort(L.keys.begin(), L.keys.end(),
-                   [](const KeyItem& a, const KeyItem& b) { return a.qlen - a.t0 > b.qlen - b.t0; });
+  const int64_t slots = sh.head_dim > 64 ? 256 : 512;  // resident workgroups
+  const int64_t piece = std::max<int64_t>(16, up(work * sh.kv_heads * 2, slots * (getenv("XS") ? atoi(getenv("XS")) : 3)));
+  for (const KeyItem& k : base) {
+    const int64_t tiles = tiles_of(k.t1 - k.t0);
+    const int pieces = tiles * 4 > piece * 5 ? (int)up(tiles, piece) : 1;
+    if (pieces == 1) {
+      L.keys.push_back(k);
+      continue;
+    }
+    const int step = (int)up(k.t1 - k.t0, pieces);
+    int made = 0;
+    for (int t = k.t0; t < k.t1; t += step) {
+      KeyItem x = k;
+      x.t0 = t;
+      x.t1 = std::min(k.t1, t + step);
+      x.plane = made++;
+      x.prow = (int32_t)L.prows;
+      L.keys.push_back(x);
+    }
+    L.planes = std::max(L.planes, made);
+    L.join.push_back(JoinItem{k.k0, k.nk, (int32_t)L.prows, made});
+    L.join_tokens = std::max(L.join_tokens, k.nk);
+    L.prows += k.nk;
+  }
+  std::stable_sort(L.keys.begin(), L.keys.end(), [](const KeyItem& a, const KeyItem& b) { return a.t1 - a.t0 > b.t1 - b.t0; });
 }
 
 static int check_shape(const ahr_attn_shape& sh) {
@@ -440,11 +461,12 @@ static int build(const int32_t* q_len, const int32_t* k_len, int n, const ahr_at
   plan->n_keys = (int32_t)L.keys.size();
   plan->n_join = (int32_t)L.join.size();
   plan->join_tokens = L.join_tokens;
-  plan->key_waves = L.key_waves;
   plan->planes = L.planes;
   plan->part_rows = L.prows;
   plan->ints = (int64_t)(L.rows.size() * sizeof(RowItem) + L.keys.size() * sizeof(KeyItem) + L.join.size() * sizeof(JoinItem)) / 4;
-  plan->ws_bytes = sh.backward ? t * sh.heads * 4 : (int64_t)L.planes * L.prows * sh.heads * (sh.head_dim + 1) * 4;
+  // forward: partial rows and their lse; backward: delta, partial dk and dv
+  plan->ws_bytes = sh.backward ? up(t * sh.heads, 4) * 16 + (int64_t)L.planes * L.prows * sh.kv_heads * 2 * sh.head_dim * 4
+                               : (int64_t)L.planes * L.prows * sh.heads * (sh.head_dim + 1) * 4;
   if (!buf) return AHR_OK;
   if (cap < plan->ints) return fail(AHR_EINVAL, "buffer smaller than the plan's lists");
   char* b = reinterpret_cast<char*>(buf);
@@ -502,6 +524,7 @@ static int fill(const ahr_attn_args* a, bool backward, Params* out) {
   p.lse = a->lse;
   if (backward) {
     p.delta = (float*)a->ws;
+    p.part_o = (float*)a->ws + up(pl.tokens * sh.heads, 4) * 4;
   } else {
     p.part_o = (float*)a->ws;  // [planes][prows][heads][dim], then the lse of each
     p.part_l = (float*)a->ws + (int64_t)pl.planes * pl.part_rows * sh.heads * sh.head_dim;

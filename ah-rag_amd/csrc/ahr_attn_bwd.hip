@@ -53,6 +53,19 @@ __device__ __forceinline__ void scale_ds(f32x16& g, f32x16 (&acc)[DB], float& sc
 
 // ---- dk, dv ------------------------------------------------------------------------------------
 
+constexpr int kStageRows = 64;  // query rows of a staged tile
+
+template <int DP>
+struct KeyCfg {
+  static constexpr int kTile = kStageRows * DP * 2;
+  static constexpr int kRowVals = 2 * kTile;               // lse and delta of the rows (and two spare copies)
+  static constexpr int kBuf = kRowVals + 4 * kStageRows * 4;
+  // Three tiles: with wide heads a SIMD holds one wave, and the loads of one tile take about as long as its
+  // products, so they are issued two tiles ahead.
+  static constexpr int kBufs = 3;
+  static constexpr int kLoads = 2 * Stager<DP / 8, kWaves, kStageRows>::kPer + 1;  // of a tile, for each wave
+};
+
 // A wave's 32 keys: their rows of k and v, and the transposed sums.
 template <typename T, int DP>
 struct KeyState {
@@ -64,7 +77,7 @@ struct KeyState {
 // 32 query rows (from row u0 of the staged tiles) against the wave's keys; `cut`: only rows [from, have) of
 // the tile read this lane's key.
 template <typename T, int DP>
-__device__ __forceinline__ void key_tile(const char* __restrict__ q_lds, const char* __restrict__ o_lds, const float* __restrict__ f, int rows,
+__device__ __forceinline__ void key_tile(const char* __restrict__ q_lds, const char* __restrict__ o_lds, const float* __restrict__ f,
                                          KeyState<T, DP>& st, int u0, bool cut, int from, int have, float c, int lane) {
   typedef typename Elem<T>::v8 v8;
   constexpr int NC = DP / 8, KS = DP / 16, DB = DP / 32;
@@ -73,20 +86,19 @@ __device__ __forceinline__ void key_tile(const char* __restrict__ q_lds, const c
 #pragma unroll
   for (int r = 0; r < 16; ++r) s[r] = g[r] = 0.f;
 #pragma unroll
-  for (int ks = 0; ks < KS; ++ks) s = Elem<T>::mma(row_frag<T, NC>(q_lds, u0 + n, ks, h), st.kf[ks], s);
-#pragma unroll
-  for (int ks = 0; ks < KS; ++ks) g = Elem<T>::mma(row_frag<T, NC>(o_lds, u0 + n, ks, h), st.vf[ks], g);
+  for (int ks = 0; ks < KS; ++ks) {
+    s = Elem<T>::mma(row_frag<T, NC>(q_lds, u0 + n, ks, h), st.kf[ks], s);
+    g = Elem<T>::mma(row_frag<T, NC>(o_lds, u0 + n, ks, h), st.vf[ks], g);
+  }
   reads_ahead<2 * KS, 1>();
 #pragma unroll
   for (int r4 = 0; r4 < 4; ++r4) {
     const f32x4 ls = *reinterpret_cast<const f32x4*>(f + u0 + r4 * 8 + h * 4);
-    const f32x4 de = *reinterpret_cast<const f32x4*>(f + rows + u0 + r4 * 8 + h * 4);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int r = r4 * 4 + i;
-      s[r] = ex2(fmaf(s[r], c, -ls[i]));
-      g[r] = s[r] * (g[r] - de[i]);
-    }
+    for (int i = 0; i < 4; ++i) s[r4 * 4 + i] = ex2(fmaf(s[r4 * 4 + i], c, -ls[i]));
+    const f32x4 de = *reinterpret_cast<const f32x4*>(f + kStageRows + u0 + r4 * 8 + h * 4);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) g[r4 * 4 + i] = s[r4 * 4 + i] * (g[r4 * 4 + i] - de[i]);
   }
   if (cut) {
 #pragma unroll
@@ -129,99 +141,71 @@ struct KeyWalk {
   }
 };
 
-template <typename T, int DP, int RW>
-struct KeyCfg {
-  static constexpr int kRows = RW == 4 ? 128 : 64;      // query rows of a staged tile
-  static constexpr int kTile = kRows * DP * 2;
-  static constexpr int kBuf = 2 * kTile + 2 * kRows * 4;  // q tile, do tile, lse, delta
-  static constexpr int kPer = kRows / 32 / RW;            // 32-row parts of a tile for each wave
-};
+// Loads of the tile that starts at w, `have` rows.
+template <int DP>
+__device__ __forceinline__ void key_stage(char* __restrict__ nxt, const Stager<DP / 8, kWaves, kStageRows>& stager, const Params& p,
+                                          const KeyItem& it, const KeyWalk& w, int hk, int have) {
+  typedef KeyCfg<DP> Cfg;
+  const int G = w.G, g0 = w.g0;
+  const int64_t at = (int64_t)it.q0 + it.t0 + w.tok0;
+  const int qts = (int)p.q_ts * 2, qhs = (int)p.q_hs * 2, ots = (int)p.do_ts * 2, ohs = (int)p.do_hs * 2;
+  const uint32_t span = (uint32_t)((g0 + have - 1) * w.ginv) >> 16;  // tokens past the first
+  const __amdgpu_buffer_rsrc_t qr =
+      dense::tile_rsrc_u(p.q + (at * p.q_ts + (int64_t)hk * G * p.q_hs) * 2, span * qts + (G - 1) * qhs + p.dim * 2);
+  const __amdgpu_buffer_rsrc_t dr =
+      dense::tile_rsrc_u(p.d_o + (at * p.do_ts + (int64_t)hk * G * p.do_hs) * 2, span * ots + (G - 1) * ohs + p.dim * 2);
+  constexpr int step = Stager<DP / 8, kWaves, kStageRows>::kStep;
+  if (DP != 96 && p.dim == DP && have == kStageRows && step % G == 0) {  // whole tokens a step, so g0 = 0
+    const int tk = (stager.row0 * w.ginv) >> 16, g = stager.row0 - tk * G;
+    stager.load_full(qr, nxt, __mul24(tk, qts) + g * qhs, step / G * qts);
+    stager.load_full(dr, nxt + Cfg::kTile, __mul24(tk, ots) + g * ohs, step / G * ots);
+  } else {
+    auto off = [&](int r, int ts, int hs) {
+      const int x = g0 + min(r, have - 1);
+      const int tk = __mul24(x, w.ginv) >> 16;
+      return __mul24(tk, ts) + (x - __mul24(tk, G)) * hs;
+    };
+    stager.load(qr, nxt, p.dim, [&](int r) { return off(r, qts, qhs); });
+    stager.load(dr, nxt + Cfg::kTile, p.dim, [&](int r) { return off(r, ots, ohs); });
+  }
+  // one value a lane: lse by wave 0, delta by wave 1 (2 and 3 repeat them, so that all waves count the same loads)
+  const float* vals = (stager.wave & 1 ? p.delta : p.lse) + at * p.heads + (int64_t)hk * G;
+  const __amdgpu_buffer_rsrc_t vr = dense::tile_rsrc_u(vals, (span * p.heads + G) * 4);
+  const int x = g0 + min(stager.lane, have - 1), tk = __mul24(x, w.ginv) >> 16;
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(vr, (__attribute__((address_space(3))) void*)(nxt + Cfg::kRowVals + stager.wave * kStageRows * 4), 4,
+                                           (tk * p.heads + x - __mul24(tk, G)) * 4, 0, 0, 0);
+}
 
-template <typename T, int DP, int KW, int RW>
+template <typename T, int DP>
 __device__ __forceinline__ void key_step(const char* __restrict__ cur, char* __restrict__ nxt, KeyState<T, DP>& st,
-                                         const Stager<DP / 8, KW * RW, KeyCfg<T, DP, RW>::kRows>& stager, const Params& p, const KeyItem& it,
-                                         const KeyWalk& w, const KeyWalk& wn, int hk, int t, int nt, bool wave_live, int rw, int j, int j_hi, int lane) {
-  typedef KeyCfg<T, DP, RW> Cfg;
-  const int G = w.G;
-  float st_l = 0.f, st_d = 0.f;  // lse and delta of the next tile's row, on their way to LDS
-  if (t + 1 < nt) {
-    const int tok0 = wn.tok0, g0 = wn.g0;
-    const int have = (int)min((int64_t)Cfg::kRows, w.n_rows - (int64_t)(t + 1) * Cfg::kRows);
-    const int64_t at = it.q0 + it.t0 + tok0;
-    const int qts = (int)p.q_ts * 2, qhs = (int)p.q_hs * 2, ots = (int)p.do_ts * 2, ohs = (int)p.do_hs * 2;
-    const uint32_t span = (uint32_t)((g0 + have - 1) * w.ginv) >> 16;  // tokens past the first
-    const __amdgpu_buffer_rsrc_t qr =
-        dense::tile_rsrc_u(p.q + (at * p.q_ts + (int64_t)hk * G * p.q_hs) * 2, span * qts + (G - 1) * qhs + p.dim * 2);
-    const __amdgpu_buffer_rsrc_t dr =
-        dense::tile_rsrc_u(p.d_o + (at * p.do_ts + (int64_t)hk * G * p.do_hs) * 2, span * ots + (G - 1) * ohs + p.dim * 2);
-    constexpr int step = Stager<DP / 8, KW * RW, Cfg::kRows>::kStep;
-    if (DP != 96 && p.dim == DP && have == Cfg::kRows && step % G == 0) {  // whole tokens a step, so g0 = 0
-      const int tk = (stager.row0 * w.ginv) >> 16, g = stager.row0 - tk * G;
-      stager.load_full(qr, nxt, __mul24(tk, qts) + g * qhs, step / G * qts);
-      stager.load_full(dr, nxt + Cfg::kTile, __mul24(tk, ots) + g * ohs, step / G * ots);
-    } else {
-      auto off = [&](int r, int ts, int hs) {
-        const int x = g0 + min(r, have - 1);
-        const int tk = __mul24(x, w.ginv) >> 16;
-        return __mul24(tk, ts) + (x - __mul24(tk, G)) * hs;
-      };
-      stager.load(qr, nxt, p.dim, [&](int r) { return off(r, qts, qhs); });
-      stager.load(dr, nxt + Cfg::kTile, p.dim, [&](int r) { return off(r, ots, ohs); });
-    }
-    if (threadIdx.x < Cfg::kRows) {
-      const int r = threadIdx.x, x = g0 + min(r, have - 1), tk = (x * w.ginv) >> 16;
-      const int64_t i = (at + tk) * p.heads + hk * G + (x - tk * G);
-      st_l = p.lse[i];
-      st_d = p.delta[i];
-    }
-  }
-  if (t >= 0 && wave_live) {
-    const int tok0 = w.tok0, g0 = w.g0;
-    const int have = (int)min((int64_t)Cfg::kRows, w.n_rows - (int64_t)t * Cfg::kRows);
-    const float* f = reinterpret_cast<const float*>(cur + 2 * Cfg::kTile);
+                                         const Stager<DP / 8, kWaves, kStageRows>& stager, const Params& p, const KeyItem& it,
+                                         const KeyWalk& w, const KeyWalk& wn, int hk, int t, int nt, bool wave_live, int j, int j_hi, int lane) {
+  typedef KeyCfg<DP> Cfg;
+  constexpr int ahead = Cfg::kBufs - 1;
+  if (t + ahead < nt) key_stage<DP>(nxt, stager, p, it, wn, hk, (int)min((int64_t)kStageRows, w.n_rows - (int64_t)(t + ahead) * kStageRows));
+  if (!wave_live) return;
+  const int G = w.G, tok0 = w.tok0, g0 = w.g0;
+  const int have = (int)min((int64_t)kStageRows, w.n_rows - (int64_t)t * kStageRows);
+  const float* f = reinterpret_cast<const float*>(cur + Cfg::kRowVals);
+  // A row reads keys j <= coff + its token, which is (g0 + x) / G past tok0: row x reads key j from
+  // x = G (j - coff - t0 - tok0) - g0 on.
+  const int from = p.causal ? min(max(j - w.coff - it.t0 - tok0, -1), 1 << 20) * G - g0 : 0;
 #pragma unroll
-    for (int u = 0; u < Cfg::kPer; ++u) {
-      const int u0 = (rw * Cfg::kPer + u) * 32;
-      if (u0 >= have) break;
-      // a row reads keys j <= coff + its token; the rows' tokens rise
-      const int tok_lo = it.t0 + tok0 + (((g0 + u0) * w.ginv) >> 16);
-      const bool cut = u0 + 32 > have || (p.causal && j_hi > w.coff + tok_lo);
-      // its token is (g0 + x) / G past tok0, so row x reads key j from x = G (j - coff - t0 - tok0) - g0 on
-      const int from = p.causal ? min(max(j - w.coff - it.t0 - tok0, -1), 1 << 20) * G - g0 : 0;
-      key_tile<T, DP>(cur, cur + Cfg::kTile, f, Cfg::kRows, st, u0, cut, from, have, p.scale_log2, lane);
-    }
-  }
-  if (t + 1 < nt && threadIdx.x < Cfg::kRows) {
-    float* f = reinterpret_cast<float*>(nxt + 2 * Cfg::kTile);
-    f[threadIdx.x] = st_l;
-    f[Cfg::kRows + threadIdx.x] = st_d;
+  for (int u0 = 0; u0 < kStageRows; u0 += 32) {
+    if (u0 >= have) break;
+    const int tok_lo = it.t0 + tok0 + (((g0 + u0) * w.ginv) >> 16);
+    const bool cut = u0 + 32 > have || (p.causal && j_hi > w.coff + tok_lo);
+    key_tile<T, DP>(cur, cur + Cfg::kTile, f, st, u0, cut, from, have, p.scale_log2, lane);
   }
 }
 
-// dk, dv of KW * 32 keys of one key head. RW groups of waves take different rows of each staged tile and
-// are added through LDS at the end, in order: where there are few key tiles (or causal ones of very
-// different length) that shortens the longest workgroup without partial sums in memory.
-template <typename T, int DP, int KW, int RW>
-__global__ __launch_bounds__(KW * RW * 64, DP > 64 ? 1 : 2) void attn_dkv_kernel(Params p) {
+template <typename T, int DP>
+__device__ __forceinline__ void key_loop(const Params& p, const KeyItem& it, int hk, char* smem, int wave, int lane) {
   typedef typename Elem<T>::v8 v8;
-  typedef KeyCfg<T, DP, RW> Cfg;
-  constexpr int KS = DP / 16, DB = DP / 32, NW = KW * RW;
-  extern __shared__ __attribute__((aligned(16))) char smem[];
-  const int lane = threadIdx.x & 63, h = lane >> 5, n = lane & 31;
-  const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-  const int kw = wave % KW, rw = wave / KW;
-  const int hk = blockIdx.x % p.kv_heads;
-  const KeyItem it = p.keys[blockIdx.x / p.kv_heads];
-  const int dim = p.dim;
-
-  if (DP != dim) {
-    for (int b = 0; b < 2; ++b)
-      for (int i = threadIdx.x; i < 2 * Cfg::kTile / 16; i += NW * 64)
-        reinterpret_cast<f32x4*>(smem + b * Cfg::kBuf)[i] = f32x4{0, 0, 0, 0};
-    __syncthreads();
-  }
-
-  const int key = kw * 32 + n;
+  typedef KeyCfg<DP> Cfg;
+  constexpr int KS = DP / 16, DB = DP / 32;
+  const int h = lane >> 5, n = lane & 31, dim = p.dim;
+  const int key = wave * 32 + n;
   const bool live = key < it.nk;
   KeyState<T, DP> st;
   {
@@ -240,71 +224,64 @@ __global__ __launch_bounds__(KW * RW * 64, DP > 64 ? 1 : 2) void attn_dkv_kernel
 #pragma unroll
   for (int b = 0; b < DB; ++b)
 #pragma unroll
-    for (int r = 0; r < 16; ++r) st.gk[b][r] = st.gv[b][r] = 0.f;
+    for (int r = 0; r < 16; ++r) {
+      st.gk[b][r] = 0.f;
+      st.gv[b][r] = 0.f;
+    }
   st.sc = Elem<T>::kNarrow ? 0.f : 1.f;
 
-  const Stager<DP / 8, NW, Cfg::kRows> stager(wave, lane);
+  const Stager<DP / 8, kWaves, kStageRows> stager(wave, lane);
   KeyWalk w;
   w.G = p.group;
   w.ginv = p.group_inv;
   w.coff = it.klen - it.qlen;
-  w.n_rows = (int64_t)(it.qlen - it.t0) * p.group;  // rows that may read the keys
+  w.n_rows = (int64_t)(it.t1 - it.t0) * p.group;
   w.tok0 = w.g0 = 0;
-  const int nt = (int)((w.n_rows + Cfg::kRows - 1) / Cfg::kRows);
-  const bool wave_live = kw * 32 < it.nk;
-  const int j = it.kpos + key;                             // this lane's key in its sequence
-  const int j_hi = it.kpos + min(kw * 32 + 31, it.nk - 1);  // the wave's last
-  if (nt > 0) {
-    KeyWalk wn = w;
-    const int rows_tok = Cfg::kRows / p.group, rows_g = Cfg::kRows - rows_tok * p.group;
-    key_step<T, DP, KW, RW>(smem, smem, st, stager, p, it, w, wn, hk, -1, nt, false, rw, j, j_hi, lane);
-    for (int t = 0; t < nt; ++t) {
-      wn.next(rows_tok, rows_g);
-      tile_barrier();
-      if constexpr (DP > 64) {  // the sums stay in accumulation registers (moved to others and back each tile otherwise)
+  const int nt = (int)((w.n_rows + kStageRows - 1) / kStageRows);
+  const bool wave_live = wave * 32 < it.nk;
+  const int j = it.kpos + key;                               // this lane's key in its sequence
+  const int j_hi = it.kpos + min(wave * 32 + 31, it.nk - 1);  // the wave's last
+  const int rows_tok = kStageRows / p.group, rows_g = kStageRows - rows_tok * p.group;
+  KeyWalk wn = w;
 #pragma unroll
-        for (int b = 0; b < DB; ++b) asm volatile("" : "+a"(st.gk[b]), "+a"(st.gv[b]));
-      }
-      key_step<T, DP, KW, RW>(smem + (t & 1) * Cfg::kBuf, smem + ((t + 1) & 1) * Cfg::kBuf, st, stager, p, it, w, wn, hk, t, nt, wave_live, rw,
-                              j, j_hi, lane);
-      w = wn;
-    }
+  for (int t = 0; t < Cfg::kBufs - 1; ++t) {
+    if (t < nt) key_stage<DP>(smem + t * Cfg::kBuf, stager, p, it, wn, hk, (int)min((int64_t)kStageRows, w.n_rows - (int64_t)t * kStageRows));
+    wn.next(rows_tok, rows_g);
   }
-  float k_out = p.scale / (st.sc == 0.f ? 1.f : st.sc);
-  const float v_out = Elem<T>::kNarrow ? 0x1p-14f : 1.f;
-  if constexpr (RW > 1) {
-    float* sum = reinterpret_cast<float*>(smem);  // [kw][register][lane], one group of waves at a time
+  int cur = 0, nxt = (Cfg::kBufs - 1) * Cfg::kBuf;
+  for (int t = 0; t < nt; ++t) {
+    // the next tile's loads may stay in flight (all are waited for where lanes without a chunk may skip some)
+    if (dim == DP && t + 1 < nt) tile_barrier<Cfg::kLoads>();
+    else tile_barrier();
+    if constexpr (DP > 64) {  // the sums stay in accumulation registers (moved to others and back each tile otherwise)
+#pragma unroll
+      for (int b = 0; b < DB; ++b) asm volatile("" : "+a"(st.gk[b]), "+a"(st.gv[b]));
+    }
+    key_step<T, DP>(smem + cur, smem + nxt, st, stager, p, it, w, wn, hk, t, nt, wave_live, j, j_hi, lane);
+    w.next(rows_tok, rows_g);
+    wn.next(rows_tok, rows_g);
+    cur = cur + Cfg::kBuf == Cfg::kBufs * Cfg::kBuf ? 0 : cur + Cfg::kBuf;
+    nxt = nxt + Cfg::kBuf == Cfg::kBufs * Cfg::kBuf ? 0 : nxt + Cfg::kBuf;
+  }
+  if (!live) return;
+  const float k_out = p.scale / (st.sc == 0.f ? 1.f : st.sc), v_out = Elem<T>::kNarrow ? 0x1p-14f : 1.f;
+  if (it.plane >= 0) {  // [plane][row][key head][dk, dv][dim]
+    float* out = p.part_o + ((((int64_t)it.plane * p.prows + it.prow + key) * p.kv_heads + hk) * 2) * dim;
 #pragma unroll
     for (int b = 0; b < DB; ++b)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) st.gk[b][r] *= k_out;
-    k_out = 1.f;
-    for (int o = 1; o < RW; ++o) {
-      __syncthreads();
-      float* at = sum + kw * (2 * DB * 16 * 64) + lane;
-      if (rw == o) {
-#pragma unroll
-        for (int b = 0; b < DB; ++b)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            at[(b * 16 + r) * 64] = st.gk[b][r];
-            at[(DB * 16 + b * 16 + r) * 64] = st.gv[b][r];
-          }
+      for (int x = 0; x < 4; ++x) {
+        const int d = b * 32 + x * 8 + h * 4;
+        if (DP != dim && d >= dim) continue;
+        
+          *reinterpret_cast<f32x4*>(out + d) =
+              f32x4{st.gk[b][4 * x], st.gk[b][4 * x + 1], st.gk[b][4 * x + 2], st.gk[b][4 * x + 3]} * k_out;
+        
+          *reinterpret_cast<f32x4*>(out + dim + d) =
+              f32x4{st.gv[b][4 * x], st.gv[b][4 * x + 1], st.gv[b][4 * x + 2], st.gv[b][4 * x + 3]} * v_out;
       }
-      __syncthreads();
-      if (rw == 0) {
-#pragma unroll
-        for (int b = 0; b < DB; ++b)
-#pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            st.gk[b][r] += at[(b * 16 + r) * 64];
-            st.gv[b][r] += at[(DB * 16 + b * 16 + r) * 64];
-          }
-      }
-    }
-    if (rw != 0) return;
+    return;
   }
-  if (!live) return;
   char* kp = p.dk + ((int64_t)(it.k0 + key) * p.dk_ts + (int64_t)hk * p.dk_hs) * 2;
   char* vp = p.dv + ((int64_t)(it.k0 + key) * p.dv_ts + (int64_t)hk * p.dv_hs) * 2;
 #pragma unroll
@@ -312,12 +289,54 @@ __global__ __launch_bounds__(KW * RW * 64, DP > 64 ? 1 : 2) void attn_dkv_kernel
 #pragma unroll
     for (int x = 0; x < 4; ++x) {
       const int d = b * 32 + x * 8 + h * 4;
-      if (DP == dim || d < dim) {
-        const f32x16 &a = st.gk[b], &e = st.gv[b];
+      if (DP != dim && d >= dim) continue;
+      {
+        const f32x16& a = st.gk[b];
         store4<T>(kp + d * 2, a[4 * x] * k_out, a[4 * x + 1] * k_out, a[4 * x + 2] * k_out, a[4 * x + 3] * k_out);
+      }
+      {
+        const f32x16& e = st.gv[b];
         store4<T>(vp + d * 2, e[4 * x] * v_out, e[4 * x + 1] * v_out, e[4 * x + 2] * v_out, e[4 * x + 3] * v_out);
       }
     }
+}
+
+// dk, dv of one item for one key head
+template <typename T, int DP>
+__global__ __launch_bounds__(kWaves * 64, DP > 64 ? 1 : 2) void attn_dkv_kernel(Params p) {
+  typedef KeyCfg<DP> Cfg;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  const int hk = blockIdx.x % p.kv_heads;
+  const KeyItem it = p.keys[blockIdx.x / p.kv_heads];
+  if (DP != p.dim) {
+    for (int b = 0; b < Cfg::kBufs; ++b)
+      for (int i = threadIdx.x; i < 2 * Cfg::kTile / 16; i += kWaves * 64)
+        reinterpret_cast<f32x4*>(smem + b * Cfg::kBuf)[i] = f32x4{0, 0, 0, 0};
+    __syncthreads();
+  }
+  key_loop<T, DP>(p, it, hk, smem, wave, lane);
+}
+
+// Adds the partial sums of dk and dv, plane after plane: 4 values a thread.
+template <typename T>
+__global__ __launch_bounds__(256) void attn_sum_kernel(Params p) {
+  const JoinItem it = p.join[blockIdx.x];
+  const int per = p.kv_heads * 2 * p.dim;  // values of a key
+  const int64_t i = ((int64_t)blockIdx.y * 256 + threadIdx.x) * 4;
+  if (i >= (int64_t)it.nq * per) return;
+  const float* x = p.part_o + (int64_t)it.prow * per + i;
+  const int64_t plane = p.prows * per;
+  f32x4 s = {0, 0, 0, 0};
+#pragma unroll 4
+  for (int j = 0; j < it.np; ++j) s += *reinterpret_cast<const f32x4*>(x + j * plane);
+  const int key = (int)(i / per), rest = (int)(i - (int64_t)key * per);
+  const int hk = rest / (2 * p.dim), at = rest - hk * 2 * p.dim;
+  const bool v = at >= p.dim;
+  char* o = v ? p.dv + ((int64_t)(it.q0 + key) * p.dv_ts + (int64_t)hk * p.dv_hs + at - p.dim) * 2
+              : p.dk + ((int64_t)(it.q0 + key) * p.dk_ts + (int64_t)hk * p.dk_hs + at) * 2;
+  store4<T>(o, s[0], s[1], s[2], s[3]);
 }
 
 // ---- dq ----------------------------------------------------------------------------------------
@@ -467,15 +486,18 @@ __global__ __launch_bounds__(kWaves * 64, 2) void attn_dq_kernel(Params p) {
     }
 }
 
-template <typename T, int DP, int KW, int RW>
-static int launch_dkv(const Params& p, hipStream_t s) {
-  constexpr int tiles = 2 * KeyCfg<T, DP, RW>::kBuf, sums = RW > 1 ? KW * DP * 32 * 2 * 4 : 0;
-  constexpr int lds = tiles > sums ? tiles : sums;
-  static_assert(lds <= 160 * 1024, "LDS of one workgroup");
+template <typename T, int DP>
+static int launch_dkv(const ahr_attn_plan& pl, const Params& p, hipStream_t s) {
+  constexpr int lds = KeyCfg<DP>::kBufs * KeyCfg<DP>::kBuf;
   static std::atomic<uint64_t> done{0};
-  ensure_lds_attr(done, reinterpret_cast<const void*>(attn_dkv_kernel<T, DP, KW, RW>), lds);
-  attn_dkv_kernel<T, DP, KW, RW><<<dim3((unsigned)(p.n_keys * p.kv_heads)), KW * RW * 64, lds, s>>>(p);
+  ensure_lds_attr(done, reinterpret_cast<const void*>(attn_dkv_kernel<T, DP>), lds);
+  attn_dkv_kernel<T, DP><<<dim3((unsigned)(p.n_keys * p.kv_heads)), kWaves * 64, lds, s>>>(p);
   AHR_HIP(hipGetLastError());
+  if (p.n_join) {
+    const int64_t vals = (int64_t)pl.join_tokens * p.kv_heads * 2 * p.dim;
+    attn_sum_kernel<T><<<dim3((unsigned)p.n_join, (unsigned)((vals + 1023) / 1024)), 256, 0, s>>>(p);
+    AHR_HIP(hipGetLastError());
+  }
   return AHR_OK;
 }
 
@@ -495,10 +517,7 @@ static int launch_bwd_d(const ahr_attn_plan& pl, const Params& p, hipStream_t s)
     const int st = launch_dq<T, DP>(p, s);  // writes delta, so it comes first
     if (st != AHR_OK) return st;
   }
-  if (!p.n_keys) return AHR_OK;
-  if (pl.key_waves == 1) return launch_dkv<T, DP, 1, 4>(p, s);
-  if (pl.key_waves == 2) return launch_dkv<T, DP, 2, 2>(p, s);
-  return launch_dkv<T, DP, 4, 1>(p, s);
+  return p.n_keys ? launch_dkv<T, DP>(pl, p, s) : AHR_OK;
 }
 
 template <typename T>

@@ -85,9 +85,14 @@ __device__ __forceinline__ typename Elem<T>::v8 acc_frag(const f32x16& x, int o)
 
 // Before a tile that LDS-DMA fills is read: this wave's loads have landed, then every wave's (the
 // compiler's own barrier does not wait for LDS-DMA). All waves of the workgroup pass here once per tile,
-// whether or not they have work in it.
+// whether or not they have work in it. The wait is the builtin, which the compiler counts: after one in
+// inline asm it waits again, at the first use of registers loaded before the loop, for whatever the tile
+// has in flight by then.
+// N: loads of this wave that may still be in flight (of tiles further ahead).
+template <int N = 0>
 __device__ __forceinline__ void tile_barrier() {
-  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt((N & 15) | 0x0070 | (N >> 4) << 14);  // vmcnt(N) lgkmcnt(0)
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
 }
@@ -130,7 +135,8 @@ __device__ __forceinline__ void store4(char* p, float a, float b, float c, float
 // its lanes keep one row and chunk, and the step goes into the scalar offset.
 template <int NC, int NW, int ROWS>
 struct Stager {
-  static constexpr int kPer = NC * ROWS / 64 / NW;
+  static constexpr int kLoads = NC * ROWS / 64, kPer = (kLoads + NW - 1) / NW;
+  static_assert(NC == 12 || kLoads % NW == 0, "every wave has the same loads");
   static constexpr int kStep = NC == 12 ? 0 : NW * 64 / NC;
   int wave, lane, row0, c0;
   __device__ __forceinline__ Stager(int w, int l) : wave(w), lane(l) {
@@ -149,6 +155,7 @@ struct Stager {
   __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t r, char* tile, int dim, F off) const {
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
+      if (kLoads % NW != 0 && i * NW + wave >= kLoads) break;
       const int ci = (i * NW + wave) * 64 + lane, row = ci / NC, c = (ci % NC) ^ swz<NC>(row);
       if (c * 8 < dim) dense::blds16(r, (uint32_t)(off(row) + c * 16), tile + (i * NW + wave) * 1024);
     }

@@ -6,7 +6,7 @@ import numpy as np
 import pytest
 
 ROW = ("q0", "nq", "k0", "klen", "koff", "kb", "ke", "pb", "pe", "plane", "prow", "pad")
-KEY = ("k0", "nk", "kpos", "klen", "q0", "qlen", "t0", "pad")
+KEY = ("k0", "nk", "kpos", "klen", "q0", "qlen", "t0", "t1", "plane", "prow", "pad", "pad2")
 
 
 def _plan(q_lens, k_lens=None, heads=12, kv_heads=12, dim=64, causal=0, backward=0, prefix=0, dtype=2):
@@ -45,6 +45,8 @@ CASES = [
     dict(q_lens=[700] * 20, prefix=1, heads=32, kv_heads=8, causal=1),
     dict(q_lens=[3, 0], k_lens=[0, 0], prefix=65),
     dict(q_lens=[]),
+    dict(q_lens=[4000, 300], heads=16, kv_heads=4, dim=128, causal=1),
+    dict(q_lens=[3000], k_lens=[700], heads=6, kv_heads=2),
 ]
 
 
@@ -106,20 +108,30 @@ def test_key_lists_cover_every_pair_once(case):
     causal = case.get("causal", 0)
     kstarts = np.concatenate(([0], np.cumsum(kl))).astype(int)
     starts = np.concatenate(([0], np.cumsum(ql))).astype(int)
-    seen = np.zeros(sum(kl), int)
+    seen, final = [np.zeros(ql[s], int) for s in np.repeat(np.arange(len(kl)), kl)], np.zeros(sum(kl), int)
+    planes = [set() for _ in range(sum(kl))]
     for k in keys:
         s = int(np.searchsorted(kstarts, k["k0"], side="right") - 1)
         assert k["klen"] == kl[s] and k["qlen"] == ql[s] and k["q0"] == starts[s] and k["kpos"] == k["k0"] - kstarts[s]
-        assert 0 < k["nk"] <= plan.key_waves * 32 and k["kpos"] + k["nk"] <= kl[s]
-        seen[k["k0"]:k["k0"] + k["nk"]] += 1
-        # tokens before t0 read none of the keys
-        assert 0 <= k["t0"] <= ql[s]
-        if causal and k["t0"] > 0:
-            assert k["t0"] - 1 + kl[s] - ql[s] < k["kpos"]
-        if not causal:
-            assert k["t0"] == 0
-    assert (seen == 1).all()
-    assert not join and all(r["plane"] < 0 and r["kb"] == 0 and r["pe"] == 0 for r in rows)
+        assert 0 < k["nk"] <= 128 and k["kpos"] + k["nk"] <= kl[s] and 0 <= k["t0"] <= k["t1"] <= ql[s]
+        for i in range(k["k0"], k["k0"] + k["nk"]):
+            seen[i][k["t0"]:k["t1"]] += 1
+            if k["plane"] < 0:
+                final[i] += 1
+            else:
+                assert k["plane"] < plan.planes and k["prow"] + k["nk"] <= plan.part_rows
+                planes[i].add((k["plane"], k["prow"] + i - k["k0"]))
+    for s in range(len(kl)):
+        for j in range(kl[s]):
+            got = seen[kstarts[s] + j]
+            first = max(0, j - (kl[s] - ql[s])) if causal else 0  # the first token that reads key j
+            assert (got[first:] == 1).all() and (got <= 1).all()
+    joined = {k0 + i: {(j, prow + i) for j in range(n)} for k0, nk, prow, n in join for i in range(nk)}
+    for i in range(sum(kl)):
+        assert (final[i] == 1 and not planes[i] and i not in joined) or (final[i] == 0 and planes[i] == joined[i])
+    flat = [x for p in planes for x in p]
+    assert len(flat) == len(set(flat))
+    assert all(r["plane"] < 0 and r["kb"] == 0 and r["pe"] == 0 for r in rows)
     assert sum(r["nq"] for r in rows) == sum(ql)
 
 
