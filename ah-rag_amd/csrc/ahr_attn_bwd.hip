@@ -199,6 +199,16 @@ __device__ __forceinline__ void key_step(const char* __restrict__ cur, char* __r
   }
 }
 
+// Wide heads: the sums stay in accumulation registers, at both ends of the loop (held in others there, all
+// 128 are moved over and back each tile).
+template <int DP>
+__device__ __forceinline__ void pin(f32x16 (&a)[DP / 32], f32x16 (&b)[DP / 32]) {
+  if constexpr (DP > 64) {
+#pragma unroll
+    for (int i = 0; i < DP / 32; ++i) asm volatile("" : "+a"(a[i]), "+a"(b[i]));
+  }
+}
+
 template <typename T, int DP>
 __device__ __forceinline__ void key_loop(const Params& p, const KeyItem& it, int hk, char* smem, int wave, int lane) {
   typedef typename Elem<T>::v8 v8;
@@ -249,19 +259,18 @@ __device__ __forceinline__ void key_loop(const Params& p, const KeyItem& it, int
     wn.next(rows_tok, rows_g);
   }
   int cur = 0, nxt = (Cfg::kBufs - 1) * Cfg::kBuf;
+  pin<DP>(st.gk, st.gv);
   for (int t = 0; t < nt; ++t) {
     // the next tile's loads may stay in flight (all are waited for where lanes without a chunk may skip some)
     if (dim == DP && t + 1 < nt) tile_barrier<Cfg::kLoads>();
     else tile_barrier();
-    if constexpr (DP > 64) {  // the sums stay in accumulation registers (moved to others and back each tile otherwise)
-#pragma unroll
-      for (int b = 0; b < DB; ++b) asm volatile("" : "+a"(st.gk[b]), "+a"(st.gv[b]));
-    }
+    pin<DP>(st.gk, st.gv);
     key_step<T, DP>(smem + cur, smem + nxt, st, stager, p, it, w, wn, hk, t, nt, wave_live, j, j_hi, lane);
     w.next(rows_tok, rows_g);
     wn.next(rows_tok, rows_g);
     cur = cur + Cfg::kBuf == Cfg::kBufs * Cfg::kBuf ? 0 : cur + Cfg::kBuf;
     nxt = nxt + Cfg::kBuf == Cfg::kBufs * Cfg::kBuf ? 0 : nxt + Cfg::kBuf;
+    pin<DP>(st.gk, st.gv);
   }
   if (!live) return;
   const float k_out = p.scale / (st.sc == 0.f ? 1.f : st.sc), v_out = Elem<T>::kNarrow ? 0x1p-14f : 1.f;
