@@ -322,8 +322,9 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, layout: 
 
     Differentiable in q, k and v (no atomics: repeated runs give the same bits). `out`, where no gradient
     is wanted: written in place of a new tensor; it must not overlap the inputs. `stream`: runs there,
-    after the current stream's work; the caller orders what follows. A value that is not finite stays
-    within its own sequence."""
+    after the current stream's work; the caller orders what follows. A key or value that a row's mask
+    hides never reaches that row's output, whatever it holds; in the gradients a value that is not finite may
+    reach any row of its own sequence, and none of another."""
     scale = _check_attention(q, k, v, layout, scale)
     _check_out(out, q)
     grad = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)

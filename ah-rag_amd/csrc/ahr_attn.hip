@@ -96,6 +96,53 @@ __device__ __forceinline__ void fwd_tile(const char* __restrict__ cur, FwdState<
   reads_ahead<4 * DB, 2>();
 }
 
+// The row of this lane again, in plain steps: where a product of zero weights with a value that is not finite
+// reached an accumulator (a tile's matrix product multiplies every row's weight, also the zero of a key that
+// the row does not read, with every value), or where inputs that the row does read are not finite.
+template <typename T, int DP>
+__device__ __forceinline__ void strict_row(FwdState<T, DP>& st, const Params& p, const RowItem& it, int hk, int head, int tok, int lim, int h) {
+  typedef typename Elem<T>::v8 v8;
+  typedef typename Elem<T>::v4 v4;
+  const char* qp = p.q + ((int64_t)(it.q0 + tok) * p.q_ts + (int64_t)head * p.q_hs) * 2;
+  auto score = [&](const char* k) {
+    float x = 0.f;
+    for (int d = 0; d < p.dim; d += 8) {
+      const v8 a = *reinterpret_cast<const v8*>(qp + d * 2), b = *reinterpret_cast<const v8*>(k + d * 2);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x = fmaf((float)a[i], (float)b[i], x);
+    }
+    return x;
+  };
+  auto each = [&](auto f) {
+    for (int j = it.pb; j < it.pe; ++j) f(p.pk + ((int64_t)j * p.pk_ts + hk * p.pk_hs) * 2, p.pv + ((int64_t)j * p.pv_ts + hk * p.pv_hs) * 2);
+    for (int j = it.kb; j < min(it.ke, lim); ++j)
+      f(p.k + ((int64_t)(it.k0 + j) * p.k_ts + hk * p.k_hs) * 2, p.v + ((int64_t)(it.k0 + j) * p.v_ts + hk * p.v_hs) * 2);
+  };
+  float m = -INFINITY;
+  each([&](const char* k, const char*) { m = fmaxf(m, score(k) * p.scale_log2); });
+  const float ref = m == -INFINITY ? 0.f : m;
+  st.m = m;
+  st.l = 0.f;
+#pragma unroll
+  for (int b = 0; b < DP / 32; ++b)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) st.acc[b][r] = 0.f;
+  each([&](const char* k, const char* v) {
+    const float w = ex2(fmaf(score(k), p.scale_log2, -ref));
+    if (h == 0) st.l += w;
+#pragma unroll
+    for (int b = 0; b < DP / 32; ++b)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const int d = b * 32 + g * 8 + h * 4;
+        if (DP != p.dim && d >= p.dim) continue;
+        const v4 x = *reinterpret_cast<const v4*>(v + d * 2);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) st.acc[b][4 * g + i] = fmaf(w, (float)x[i], st.acc[b][4 * g + i]);
+      }
+  });
+}
+
 template <typename T, int DP>
 __device__ __forceinline__ void fwd_step(const char* __restrict__ cur, char* __restrict__ nxt, FwdState<T, DP>& st,
                                          const Stager<DP / 8, kWaves, kKeys>& stager, const Params& p, const RowItem& it, int hk, int t, int np,
@@ -118,10 +165,11 @@ __device__ __forceinline__ void fwd_step(const char* __restrict__ cur, char* __r
   fwd_tile<T, DP>(cur, st, kt + kKeys > stop || (!pre && kt + kKeys > lim_lo), (pre ? stop : min(lim, stop)) - kt, p.scale_log2, lane);
 }
 
+// (Up to 64 wide: 128 registers, four waves a SIMD. 256 texts of up to 384 tokens, 12 heads of 64: 73 us, 79
+// with the 162 registers that the compiler takes when left alone.)
 template <typename T, int DP>
-__global__ __launch_bounds__(kWaves * 64, 2) void attn_fwd_kernel(Params p) {
-  typedef typename Elem<T>::v8 v8;
-  constexpr int KS = DP / 16, DB = DP / 32;
+__global__ __launch_bounds__(kWaves * 64, DP <= 64 ? 4 : 2) void attn_fwd_kernel(Params p) {
+  constexpr int DB = DP / 32;
   constexpr int kTile = kKeys * DP * 2;
   extern __shared__ __attribute__((aligned(16))) char smem[];  // [2][K tile, V tile]
   const int lane = threadIdx.x & 63, h = lane >> 5, n = lane & 31;
@@ -149,15 +197,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void attn_fwd_kernel(Params p) {
   const int lim_hi = p.causal ? min(it.klen, it.koff + last + 1) : it.klen;
 
   FwdState<T, DP> st;
-  {
-    const char* qp = p.q + ((int64_t)(it.q0 + tok) * p.q_ts + (int64_t)head * p.q_hs) * 2;
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks) {
-      const int d = (2 * ks + h) * 8;
-      const v8 z = {};
-      st.qf[ks] = (live && (DP == dim || d < dim)) ? *reinterpret_cast<const v8*>(qp + d * 2) : z;
-    }
-  }
+  load_row<T, DP>(st.qf, p.q + ((int64_t)(it.q0 + tok) * p.q_ts + (int64_t)head * p.q_hs) * 2, dim, h);
 #pragma unroll
   for (int b = 0; b < DB; ++b)
 #pragma unroll
@@ -177,6 +217,16 @@ __global__ __launch_bounds__(kWaves * 64, 2) void attn_fwd_kernel(Params p) {
     }
   }
 
+  {
+    float x = st.l;
+#pragma unroll
+    for (int b = 0; b < DB; ++b)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) x = fmaf(st.acc[b][r], 0.f, x);
+    // (both half-lanes of a row have to agree)
+    const bool odd = live && !(fabsf(x) < INFINITY);
+    if (odd || __shfl_xor((int)odd, 32, 64)) strict_row<T, DP>(st, p, it, hk, head, tok, lim, h);
+  }
   if (!live) return;
   const float l = st.l + other_half(st.l);
   const float inv = l == 0.f ? 0.f : 1.f / l;
@@ -399,7 +449,9 @@ static void plan_keys(const std::vector<Seq>& seqs, const ahr_attn_shape& sh, Li
       work += tiles_of(k.t1 - k.t0);
     }
   const int64_t slots = sh.head_dim > 64 ? 256 : 512;  // resident workgroups
-  const int64_t piece = std::max<int64_t>(16, up(work * sh.kv_heads * 2, slots * (getenv("XS") ? atoi(getenv("XS")) : 3)));
+  // (5.8k causal tokens in 3 sequences, 16/4 heads of 128: two thirds of a slot's share 438 us for the whole
+  // step, a whole share 474, half 470, two shares 605)
+  const int64_t piece = std::max<int64_t>(16, up(work * sh.kv_heads * 2, slots * 3));
   for (const KeyItem& k : base) {
     const int64_t tiles = tiles_of(k.t1 - k.t0);
     const int pieces = tiles * 4 > piece * 5 ? (int)up(tiles, piece) : 1;

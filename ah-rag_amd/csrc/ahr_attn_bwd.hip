@@ -211,7 +211,6 @@ __device__ __forceinline__ void pin(f32x16 (&a)[DP / 32], f32x16 (&b)[DP / 32]) 
 
 template <typename T, int DP>
 __device__ __forceinline__ void key_loop(const Params& p, const KeyItem& it, int hk, char* smem, int wave, int lane) {
-  typedef typename Elem<T>::v8 v8;
   typedef KeyCfg<DP> Cfg;
   constexpr int KS = DP / 16, DB = DP / 32;
   const int h = lane >> 5, n = lane & 31, dim = p.dim;
@@ -220,16 +219,8 @@ __device__ __forceinline__ void key_loop(const Params& p, const KeyItem& it, int
   KeyState<T, DP> st;
   {
     const int64_t at = it.k0 + (live ? key : 0);
-    const char* kp = p.k + (at * p.k_ts + (int64_t)hk * p.k_hs) * 2;
-    const char* vp = p.v + (at * p.v_ts + (int64_t)hk * p.v_hs) * 2;
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks) {
-      const int d = (2 * ks + h) * 8;
-      const v8 z = {};
-      const bool in = live && (DP == dim || d < dim);
-      st.kf[ks] = in ? *reinterpret_cast<const v8*>(kp + d * 2) : z;
-      st.vf[ks] = in ? *reinterpret_cast<const v8*>(vp + d * 2) : z;
-    }
+    load_row<T, DP>(st.kf, p.k + (at * p.k_ts + (int64_t)hk * p.k_hs) * 2, dim, h);
+    load_row<T, DP>(st.vf, p.v + (at * p.v_ts + (int64_t)hk * p.v_hs) * 2, dim, h);
   }
 #pragma unroll
   for (int b = 0; b < DB; ++b)
@@ -370,9 +361,10 @@ __device__ __forceinline__ void row_tile(const char* __restrict__ cur, RowState<
 #pragma unroll
     for (int r = 0; r < 16; ++r) s[r] = g[r] = 0.f;
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks) s = Elem<T>::mma(row_frag<T, NC>(cur, u * 32 + n, ks, h), st.qf[ks], s);
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks) g = Elem<T>::mma(row_frag<T, NC>(cur + kTile, u * 32 + n, ks, h), st.of[ks], g);
+    for (int ks = 0; ks < KS; ++ks) {
+      s = Elem<T>::mma(row_frag<T, NC>(cur, u * 32 + n, ks, h), st.qf[ks], s);
+      g = Elem<T>::mma(row_frag<T, NC>(cur + kTile, u * 32 + n, ks, h), st.of[ks], g);
+    }
     reads_ahead<2 * KS, 1>();
 #pragma unroll
     for (int r = 0; r < 16; ++r) g[r] = ex2(fmaf(s[r], c, -st.lse)) * (g[r] - st.delta);
@@ -410,7 +402,6 @@ __device__ __forceinline__ void row_step(const char* __restrict__ cur, char* __r
 // dq of the rows of one item, 32 a wave
 template <typename T, int DP>
 __global__ __launch_bounds__(kWaves * 64, 2) void attn_dq_kernel(Params p) {
-  typedef typename Elem<T>::v8 v8;
   constexpr int KS = DP / 16, DB = DP / 32;
   constexpr int kTile = kKeys * DP * 2;
   extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -434,36 +425,13 @@ __global__ __launch_bounds__(kWaves * 64, 2) void attn_dq_kernel(Params p) {
   const int lim_lo = p.causal ? min(it.klen, it.koff + first + 1) : it.klen;
   const int lim_hi = p.causal ? min(it.klen, it.koff + last + 1) : it.klen;
   RowState<T, DP> st;
-  {
-    const char* qp = p.q + ((int64_t)(it.q0 + tok) * p.q_ts + (int64_t)head * p.q_hs) * 2;
-    const char* op = p.d_o + ((int64_t)(it.q0 + tok) * p.do_ts + (int64_t)head * p.do_hs) * 2;
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks) {
-      const int d = (2 * ks + h) * 8;
-      const v8 z = {};
-      const bool in = live && (DP == dim || d < dim);
-      st.qf[ks] = in ? *reinterpret_cast<const v8*>(qp + d * 2) : z;
-      st.of[ks] = in ? *reinterpret_cast<const v8*>(op + d * 2) : z;
-    }
-  }
-  const int64_t li = (int64_t)(it.q0 + tok) * p.heads + head;
+  const int64_t qt = it.q0 + tok;
+  typename Elem<T>::v8 ov[KS];
+  load_row<T, DP>(st.qf, p.q + (qt * p.q_ts + (int64_t)head * p.q_hs) * 2, dim, h);
+  load_row<T, DP>(st.of, p.d_o + (qt * p.do_ts + (int64_t)head * p.do_hs) * 2, dim, h);
+  load_row<T, DP>(ov, p.o + (qt * p.o_ts + (int64_t)head * p.o_hs) * 2, dim, h);
+  const int64_t li = qt * p.heads + head;
   st.lse = live ? p.lse[li] : 0.f;
-  // delta = sum_d do o of this lane's row, written for the dk/dv kernel that follows
-  {
-    const char* op = p.o + ((int64_t)(it.q0 + tok) * p.o_ts + (int64_t)head * p.o_hs) * 2;
-    float x = 0.f;
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks) {
-      const int d = (2 * ks + h) * 8;
-      if (live && (DP == dim || d < dim)) {
-        const v8 o = *reinterpret_cast<const v8*>(op + d * 2);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x = fmaf((float)o[i], (float)st.of[ks][i], x);
-      }
-    }
-    st.delta = x + other_half(x);
-    if (live && h == 0) p.delta[li] = st.delta;
-  }
   st.sc = Elem<T>::kNarrow ? 0.f : 1.f;
 #pragma unroll
   for (int b = 0; b < DB; ++b)
@@ -472,8 +440,17 @@ __global__ __launch_bounds__(kWaves * 64, 2) void attn_dq_kernel(Params p) {
 
   const Stager<DP / 8, kWaves, kKeys> stager(wave, lane);
   const int nt = (it.ke + kKeys - 1) / kKeys;
+  if (nt > 0) row_step<T, DP>(smem, smem, st, stager, p, it, hk, -1, nt, false, 0, 0, 0, lane);
+  {  // delta = sum_d do o of this lane's row, written for the dk/dv kernel that follows
+    float x = 0.f;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x = fmaf((float)ov[ks][i], (float)st.of[ks][i], x);
+    st.delta = x + other_half(x);
+    if (live && h == 0) p.delta[li] = st.delta;
+  }
   if (nt > 0) {
-    row_step<T, DP>(smem, smem, st, stager, p, it, hk, -1, nt, false, 0, 0, 0, lane);
     for (int t = 0; t < nt; ++t) {
       tile_barrier();
       row_step<T, DP>(smem + (t & 1) * 2 * kTile, smem + ((t + 1) & 1) * 2 * kTile, st, stager, p, it, hk, t, nt, wave_live, lim, lim_lo,

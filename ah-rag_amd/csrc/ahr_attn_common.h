@@ -98,12 +98,11 @@ __device__ __forceinline__ void tile_barrier() {
 }
 
 // Asks the scheduler, for N matrix products of the block before it whose operands take R LDS reads each,
-// to keep the reads kAhead products ahead (left alone it reads each fragment right before its product,
+// to keep the reads AHEAD products ahead (left alone it reads each fragment right before its product,
 // which then waits out the LDS latency).
-constexpr int kAhead = 4;
-template <int N, int R>
+template <int N, int R, int AHEAD = 4>
 __device__ __forceinline__ void reads_ahead() {
-  constexpr int A = N < kAhead ? N : kAhead;
+  constexpr int A = N < AHEAD ? N : AHEAD;
   __builtin_amdgcn_sched_group_barrier(0x100, A * R, 0);  // 0x100: LDS reads, 8: matrix products
 #pragma unroll
   for (int i = 0; i < N - A; ++i) {
@@ -111,6 +110,23 @@ __device__ __forceinline__ void reads_ahead() {
     __builtin_amdgcn_sched_group_barrier(0x100, R, 0);
   }
   __builtin_amdgcn_sched_group_barrier(0x008, A, 0);
+}
+
+// A row's fragments from memory (lane half h: elements 16 ks + 8 h ..), zeros past dim. The loads are
+// unconditional, so that all are in flight together and nothing waits for them before the first tile's
+// loads are issued: lanes without a row of their own read a valid one (their results go nowhere), chunks
+// past dim the last.
+template <typename T, int DP>
+__device__ __forceinline__ void load_row(typename Elem<T>::v8 (&f)[DP / 16], const char* row, int dim, int h) {
+#pragma unroll
+  for (int ks = 0; ks < DP / 16; ++ks) f[ks] = *reinterpret_cast<const typename Elem<T>::v8*>(row + min((2 * ks + h) * 8, dim - 8) * 2);
+  if (dim != DP) {
+#pragma unroll
+    for (int ks = 0; ks < DP / 16; ++ks) {
+      const typename Elem<T>::v8 z = {};
+      if ((2 * ks + h) * 8 >= dim) f[ks] = z;
+    }
+  }
 }
 
 // row of a 32x32 accumulator register r in lane half h

@@ -259,6 +259,38 @@ def test_other_sequences_never_leak(cuda):
                 assert torch.equal(a[s], b[s])
 
 
+@pytest.mark.parametrize("dim,dt", [(64, BF), (40, HF), (128, BF)])
+@pytest.mark.parametrize("val", [math.nan, math.inf, -math.inf])
+def test_hidden_values_never_reach_a_row(cuda, dim, dt, val):
+    """A causal sequence whose token 37 holds such keys and values: the rows before it keep their bits, the rows
+    that read it have what the definition gives."""
+    from ah_rag.packed import PackedLayout, packed_attention, prefix_attention
+    lens = [100]
+    q, k, v, _ = _make((lens, None, 4, 2, dim, True, dt), 37, cuda)
+    lay = PackedLayout(lens, device=cuda)
+    want, tol = ref.attention(q, k, v, lens, lens, True, dim ** -0.5)
+    pk = k[:70].clone()
+    k2, v2 = k.clone(), v.clone()
+    k2[37] = val
+    v2[37] = val
+    o = packed_attention(q, k2, v, lay, causal=True)
+    _within(o[:37], want[:37], tol[:37], "behind a hidden key")
+    o = packed_attention(q, k, v2, lay, causal=True)
+    _within(o[:37], want[:37], tol[:37], "behind a hidden value")
+    assert (o[37:].isnan().all() if math.isnan(val) else (o[37:] == val).all())
+    w2, t2 = ref.attention(q, k, v, lens, lens, True, dim ** -0.5, pk, pk)
+    o = prefix_attention(q, k, v2, pk, pk, lay)
+    _within(o[:37], w2[:37], t2[:37], "behind a hidden value, with a prefix")
+    # the last key of a tile that is not full
+    v3 = v.clone()
+    v3[99] = val
+    o = packed_attention(q, k, v3, lay, causal=True)
+    _within(o[:99], want[:99], tol[:99], "before the last key")
+    single = PackedLayout([1], [100], cuda)
+    o = packed_attention(q[:1], k, v3, single, causal=True)
+    assert (o.isnan().all() if math.isnan(val) else (o == val).all())
+
+
 def test_rows_outside_are_left_alone(cuda):
     """out is a slice of a larger buffer: nothing around it is written."""
     from ah_rag.packed import PackedLayout, packed_attention
