@@ -218,14 +218,14 @@ __global__ __launch_bounds__(kWaves * 64, DP <= 64 ? 4 : 2) void attn_fwd_kernel
   }
 
   {
-    float x = st.l;
+    float x[4] = {st.l, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int b = 0; b < DB; ++b)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) x = fmaf(st.acc[b][r], 0.f, x);
+      for (int r = 0; r < 16; ++r) x[r & 3] = fmaf(st.acc[b][r], 0.f, x[r & 3]);
+    const bool odd = live && !(fabsf((x[0] + x[1]) + (x[2] + x[3])) < INFINITY);
     // (both half-lanes of a row have to agree)
-    const bool odd = live && !(fabsf(x) < INFINITY);
-    if (odd || __shfl_xor((int)odd, 32, 64)) strict_row<T, DP>(st, p, it, hk, head, tok, lim, h);
+    if (__any(odd) && (odd || __shfl_xor((int)odd, 32, 64))) strict_row<T, DP>(st, p, it, hk, head, tok, lim, h);
   }
   if (!live) return;
   const float l = st.l + other_half(st.l);
