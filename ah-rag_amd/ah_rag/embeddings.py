@@ -71,7 +71,7 @@ class EncoderUnavailableError(RuntimeError):
     """The requested sentence encoder cannot be loaded (and no stand-in was asked for)."""
 
 
-ENCODER_MODES = ("", "sentence-transformers", "hash", "torch")
+ENCODER_MODES = ("", "sentence-transformers", "hash", "torch", "packed")
 
 
 def load_encoder(model_name: str = DEFAULT_MODEL, dim: Optional[int] = None):
@@ -85,14 +85,16 @@ def load_encoder(model_name: str = DEFAULT_MODEL, dim: Optional[int] = None):
       "hash": HashEncoder, the deterministic stand-in (tests and synthetic benchmarks);
       "torch": the model's architecture as a batched bf16 PyTorch forward on the GPU
           (ah_rag.encoder.TorchEncoder: a local checkpoint directory if `model_name` is one, else
-          seeded random weights for a known architecture).
+          seeded random weights for a known architecture);
+      "packed": the same weights without padding, on this library's attention and pooling kernels
+          (ah_rag.packed_encoder); a model whose layers it does not know raises.
     """
     mode = os.environ.get("AHR_ENCODER", "").lower()
     if mode not in ENCODER_MODES:
         raise ValueError(f"AHR_ENCODER={mode!r}: expected one of {', '.join(repr(m) for m in ENCODER_MODES)}")
-    if mode == "torch":
+    if mode in ("torch", "packed"):
         from .encoder import torch_encoder
-        return torch_encoder(model_name)
+        return torch_encoder(model_name, packed=mode == "packed")
     if mode == "hash":
         return HashEncoder(model_name, dim)
     try:

@@ -89,7 +89,9 @@ class TorchEncoder:
     on_device = True  # search_batch asks for the device tensor
 
     def __init__(self, model_name: str = "all-MiniLM-L6-v2", device: Optional[Union[str, torch.device]] = None,
-                 dtype: torch.dtype = torch.bfloat16, seed: int = 20251003) -> None:
+                 dtype: torch.dtype = torch.bfloat16, seed: int = 20251003, packed: bool = False) -> None:
+        """packed: run batches without padding (ah_rag.packed_encoder: this library's attention and pooling
+        kernels); a model whose layers it does not know raises UnsupportedLayoutError."""
         from transformers import AutoConfig, AutoModel, BertConfig, BertModel
         if not torch.cuda.is_available():
             raise RuntimeError("TorchEncoder runs the encoder forward on a ROCm GPU")
@@ -127,6 +129,10 @@ class TorchEncoder:
         # <s> token every sequence starts with); BERT and the seeded stand-in pad with 0
         pad = getattr(self.model.config, "pad_token_id", None)
         self.pad_id = int(pad) if pad is not None else PAD_ID
+        self.packed = None
+        if packed:
+            from .packed_encoder import PackedTransformer
+            self.packed = PackedTransformer(self.model, self.device)
 
     def get_sentence_embedding_dimension(self) -> int:
         return self.dim
@@ -134,9 +140,13 @@ class TorchEncoder:
     @torch.inference_mode()
     def encode(self, texts: Union[str, Sequence[str]], normalize_embeddings: bool = False,
                show_progress_bar: bool = False, batch_size: int = 256, convert_to_tensor: bool = False,
-               convert_to_numpy: bool = True, **_: object):
+               convert_to_numpy: bool = True, prompt: Optional[str] = None, **_: object):
+        """prompt (packed encoders; ignored by the padded forward): text put in front of every text. A causal model
+        runs the tokens that all texts of a batch share once."""
         single = isinstance(texts, str)
         items = [texts] if single else list(texts)
+        if self.packed is not None and prompt:
+            items = [prompt + t for t in items]
         out = torch.empty((len(items), self.dim), dtype=torch.float32, device=self.device)
         if items:
             ids = self.tokenizer(items)
@@ -144,6 +154,10 @@ class TorchEncoder:
             order = sorted(range(len(ids)), key=lambda i: -len(ids[i]))
             for s in range(0, len(order), batch_size):
                 sel = order[s:s + batch_size]
+                if self.packed is not None:
+                    with torch.cuda.device(self.device):
+                        out[torch.as_tensor(sel, device=self.device)] = self.packed.pooled([ids[i] for i in sel], normalize_embeddings)
+                    continue
                 L = max(len(ids[i]) for i in sel)
                 tok = np.full((len(sel), L), self.pad_id, np.int64)
                 for j, i in enumerate(sel):
@@ -165,17 +179,27 @@ class TorchEncoder:
         return arr[0] if single else arr
 
 
+    def embed(self, texts: Sequence[str], normalize_embeddings: bool = False) -> torch.Tensor:
+        """Device float32 [n, d] of one packed batch with gradients to the model's parameters: the forward of a
+        fine-tuning step (packed encoders). The caller enables the parameters' gradients, takes the loss
+        and the optimizer's step, and calls packed.refresh() before encoding with the new weights."""
+        if self.packed is None:
+            raise ValueError("embed() needs a packed encoder: TorchEncoder(..., packed=True)")
+        with torch.cuda.device(self.device):
+            return self.packed.pooled(self.tokenizer(list(texts)), normalize_embeddings)
+
+
 _CACHE: Dict[tuple, TorchEncoder] = {}
 _LOCK = threading.Lock()
 
 
-def torch_encoder(model_name: str, device: Optional[Union[str, torch.device]] = None) -> TorchEncoder:
-    """One TorchEncoder per (model, device) per process (the reference caches its query encoder
+def torch_encoder(model_name: str, device: Optional[Union[str, torch.device]] = None, packed: bool = False) -> TorchEncoder:
+    """One TorchEncoder per (model, device, packed) per process (the reference caches its query encoder
     per graph, hierarchical_graph.py:709-711; corpus builds re-load it, here they reuse it)."""
     dev = torch.device(device) if device is not None else torch.device("cuda", torch.cuda.current_device())
-    key = (model_name, str(dev))
+    key = (model_name, str(dev), packed)
     with _LOCK:
         enc = _CACHE.get(key)
         if enc is None:
-            enc = _CACHE[key] = TorchEncoder(model_name, dev)
+            enc = _CACHE[key] = TorchEncoder(model_name, dev, packed=packed)
     return enc

@@ -89,8 +89,10 @@ class PackedLayout:
             if torch.cuda.is_current_stream_capturing():
                 raise RuntimeError("a layout's first call for a shape copies its work lists to the device: make it "
                                    "before the capture")
-            # a blocking copy: the lists are complete for every stream
-            t = torch.from_numpy(host).to(self.device)
+            # a blocking copy: the lists are complete for every stream (and no inference tensor, whatever mode the
+            # first call runs in: later ones may save it for their backward pass)
+            with torch.inference_mode(False):
+                t = torch.from_numpy(host).to(self.device)
             t.ahr_stream = nat.stream_ptr(device_index=self._index)
             return t
 
@@ -371,9 +373,10 @@ def rotary_table(n_positions: int, dim: int, base: float = 10000.0,
     angles are computed in 64 bits (in 32 a far position's angle is off by position * 2^-24)."""
     if n_positions < 0 or dim < 2 or dim % 2:
         raise ValueError("n_positions must be >= 0 and dim even")
-    i = torch.arange(0, dim, 2, dtype=torch.float64)
-    angle = torch.arange(n_positions, dtype=torch.float64)[:, None] * float(base) ** (-i / dim)
-    return angle.cos().float().to(device), angle.sin().float().to(device)
+    with torch.inference_mode(False):
+        i = torch.arange(0, dim, 2, dtype=torch.float64)
+        angle = torch.arange(n_positions, dtype=torch.float64)[:, None] * float(base) ** (-i / dim)
+        return angle.cos().float().to(device), angle.sin().float().to(device)
 
 
 def _launch_rope(call, name, q, k, cos, sin, positions, eps, interleaved, wq, wk, yq, yk, dq=None, dk=None, dw=None, ws=None) -> None:

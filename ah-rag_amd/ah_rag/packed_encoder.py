@@ -1,0 +1,206 @@
+"""ah_rag.packed_encoder — a transformer's forward over packed sequences (no padding), on ah_rag.packed.
+
+PackedTransformer takes the weights of a loaded model (any module with the state dict and config of one of
+two layer layouts) and runs them over the tokens of a batch lying behind each other:
+
+  "post":   absolute positions, bidirectional attention with as many key heads as query heads, layer norm
+            after each residual (the architectures of ah_rag.encoder.ARCHS);
+  "causal": rotary positions, causal attention with grouped heads and a norm of each query and key head,
+            RMS norm before each block, gated feed-forward (decoder-style embedding checkpoints).
+
+Projections, norms of whole rows and activations are torch / hipBLASLt calls; attention, the heads' norm
+with the rotation, and pooling are this library's kernels. Other layouts are refused when the object is
+made, never approximated.
+
+In a causal model the hidden states of a prefix do not depend on what follows, so tokens that all texts of
+a batch begin with (an instruction in front of every query) are run once, and the rest of each text reads
+their keys through prefix_attention.
+
+Reference seam: SentenceTransformer.encode, src/ah_rag/graph/hierarchical_graph.py:655-656, :709-712.
+"""
+from __future__ import annotations
+
+from typing import Dict, List, Optional, Sequence, Tuple
+
+import numpy as np
+import torch
+import torch.nn.functional as F
+
+from .packed import PackedLayout, packed_attention, packed_mean_pool, prefix_attention, qk_norm_rope, rotary_table
+
+SHARE_FROM = 16  # a common prefix of at least this many tokens is run once (a causal model, two texts or more)
+
+
+class UnsupportedLayoutError(ValueError):
+    """The model's layers are neither of the two layouts that the packed forward runs."""
+
+
+def _get(cfg, *names, default=None):
+    for n in names:
+        v = getattr(cfg, n, None)
+        if v is not None:
+            return v
+    return default
+
+
+class PackedTransformer:
+    """Weights are the model's own tensors (parameters receive gradients); `model` stays referenced."""
+
+    def __init__(self, model, device: torch.device) -> None:
+        self.model, self.device = model, device
+        cfg = model.config
+        w: Dict[str, torch.Tensor] = dict(model.named_parameters())
+        self.w = w
+        self.heads = int(cfg.num_attention_heads)
+        self.layers = int(cfg.num_hidden_layers)
+        self.hidden = int(cfg.hidden_size)
+        if "encoder.layer.0.attention.self.query.weight" in w and "embeddings.position_embeddings.weight" in w:
+            self.kind = "post"
+            self.kv_heads, self.head_dim = self.heads, self.hidden // self.heads
+            self.eps = float(cfg.layer_norm_eps)
+            if _get(cfg, "position_embedding_type", default="absolute") != "absolute":
+                raise UnsupportedLayoutError("packed forward: positions other than absolute ones")
+            if "encoder.relative_attention_bias.weight" in w or _get(cfg, "model_type") in ("roberta", "xlm-roberta", "mpnet"):
+                raise UnsupportedLayoutError("packed forward: this model's positions are not those of its tokens")
+            self.act = self._activation(cfg.hidden_act)
+            self.fused = [("encoder.layer.%d.attention.self." % i, ("query", "key", "value")) for i in range(self.layers)]
+        elif "layers.0.self_attn.q_norm.weight" in w and "layers.0.mlp.gate_proj.weight" in w:
+            self.kind = "causal"
+            self.kv_heads = int(_get(cfg, "num_key_value_heads", default=self.heads))
+            self.head_dim = int(_get(cfg, "head_dim", default=self.hidden // self.heads))
+            self.eps = float(cfg.rms_norm_eps)
+            if w["layers.0.self_attn.q_norm.weight"].shape != (self.head_dim,):
+                raise UnsupportedLayoutError("packed forward: the query norm is not one of single heads")
+            if _get(cfg, "use_sliding_window", default=False) and _get(cfg, "sliding_window") is not None:
+                raise UnsupportedLayoutError("packed forward: sliding windows")
+            rope = dict(_get(cfg, "rope_parameters", "rope_scaling", default={}) or {})
+            if rope.get("rope_type", rope.get("type", "default")) != "default" or float(rope.get("partial_rotary_factor", 1.0)) != 1.0:
+                raise UnsupportedLayoutError("packed forward: scaled or partial rotary positions")
+            self.theta = float(rope.get("rope_theta", _get(cfg, "rope_theta", default=10000.0)))
+            self.act = self._activation(cfg.hidden_act)
+            self.fused = [("layers.%d.self_attn." % i, ("q_proj", "k_proj", "v_proj")) for i in range(self.layers)]
+            self._table: Optional[Tuple[torch.Tensor, torch.Tensor]] = None
+        else:
+            raise UnsupportedLayoutError("packed forward: unknown layer layout")
+        p = next(iter(w.values()))
+        if p.dtype not in (torch.float16, torch.bfloat16):
+            raise UnsupportedLayoutError(f"packed forward: weights in float16 or bfloat16, got {p.dtype}")
+        if self.head_dim % 8 or self.head_dim > 128 or self.heads % self.kv_heads:
+            raise UnsupportedLayoutError(f"packed forward: {self.heads}/{self.kv_heads} heads of {self.head_dim}")
+        self._joint: Dict[int, Tuple[torch.Tensor, Optional[torch.Tensor]]] = {}
+
+    @staticmethod
+    def _activation(name: str):
+        acts = {"gelu": F.gelu, "silu": F.silu, "swish": F.silu, "relu": F.relu,
+                "gelu_new": lambda x: F.gelu(x, approximate="tanh"), "gelu_pytorch_tanh": lambda x: F.gelu(x, approximate="tanh")}
+        if name not in acts:
+            raise UnsupportedLayoutError(f"packed forward: activation {name!r}")
+        return acts[name]
+
+    # ---- layers --------------------------------------------------------------------------------
+
+    def _qkv(self, i: int, x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+        """Queries, keys and values [tokens, heads, head_dim]: views of one projection's output, or three products
+        where the weights' gradients are wanted."""
+        prefix, names = self.fused[i]
+        ws = [self.w[prefix + n + ".weight"] for n in names]
+        bs = [self.w.get(prefix + n + ".bias") for n in names]
+        d = self.head_dim
+        if torch.is_grad_enabled() and any(t.requires_grad for t in ws):
+            return tuple(F.linear(x, a, b).view(x.shape[0], -1, d) for a, b in zip(ws, bs))
+        joint = self._joint.get(i)
+        if joint is None:
+            with torch.inference_mode(False):
+                joint = self._joint[i] = (torch.cat([a.detach() for a in ws]), None if bs[0] is None else torch.cat([b.detach() for b in bs]))
+        y = F.linear(x, *joint).view(x.shape[0], -1, d)
+        return y[:, :self.heads], y[:, self.heads:self.heads + self.kv_heads], y[:, self.heads + self.kv_heads:]
+
+    def refresh(self) -> None:
+        """After the model's weights have changed: drops the joint projections made from them."""
+        self._joint.clear()
+
+    def _lin(self, name: str, x: torch.Tensor) -> torch.Tensor:
+        return F.linear(x, self.w[name + ".weight"], self.w.get(name + ".bias"))
+
+    def _ln(self, name: str, x: torch.Tensor) -> torch.Tensor:
+        return F.layer_norm(x, (self.hidden,), self.w[name + ".weight"], self.w[name + ".bias"], self.eps)
+
+    def _rms(self, name: str, x: torch.Tensor) -> torch.Tensor:
+        return F.rms_norm(x, (self.hidden,), self.w[name + ".weight"], self.eps)
+
+    def _post(self, ids: torch.Tensor, layout: PackedLayout) -> torch.Tensor:
+        e = "embeddings."
+        x = F.embedding(ids, self.w[e + "word_embeddings.weight"]) + F.embedding(layout.positions(), self.w[e + "position_embeddings.weight"])
+        if e + "token_type_embeddings.weight" in self.w:
+            x = x + self.w[e + "token_type_embeddings.weight"][0]
+        x = self._ln(e + "LayerNorm", x)
+        for i in range(self.layers):
+            b = "encoder.layer.%d." % i
+            q, k, v = self._qkv(i, x)
+            o = packed_attention(q, k, v, layout).flatten(1)
+            x = self._ln(b + "attention.output.LayerNorm", x + self._lin(b + "attention.output.dense", o))
+            y = self._lin(b + "output.dense", self.act(self._lin(b + "intermediate.dense", x)))
+            x = self._ln(b + "output.LayerNorm", x + y)
+        return x
+
+    def _rotary(self, n: int) -> Tuple[torch.Tensor, torch.Tensor]:
+        if self._table is None or self._table[0].shape[0] < n:
+            self._table = rotary_table(max(512, n), self.head_dim, self.theta, self.device)
+        return self._table
+
+    def _causal(self, ids: torch.Tensor, layout: PackedLayout, first: int = 0, shared: Optional[List[tuple]] = None,
+                keep: Optional[List[tuple]] = None) -> torch.Tensor:
+        """shared: (keys, values) of a common prefix of `first` tokens, one pair a layer; keep: appended to, for such."""
+        cos, sin = self._rotary(first + (int(layout.lengths.max()) if len(layout) else 0))
+        pos = layout.positions() + first if first else layout.positions()
+        x = F.embedding(ids, self.w["embed_tokens.weight"])
+        for i in range(self.layers):
+            b = "layers.%d." % i
+            q, k, v = self._qkv(i, self._rms(b + "input_layernorm", x))
+            q, k = qk_norm_rope(q, k, self.w[b + "self_attn.q_norm.weight"], self.w[b + "self_attn.k_norm.weight"], cos, sin, pos, eps=self.eps)
+            if keep is not None:
+                keep.append((k, v))
+            o = packed_attention(q, k, v, layout, causal=True) if shared is None else prefix_attention(q, k, v, *shared[i], layout)
+            x = x + self._lin(b + "self_attn.o_proj", o.flatten(1))
+            y = self._rms(b + "post_attention_layernorm", x)
+            x = x + self._lin(b + "mlp.down_proj", self.act(self._lin(b + "mlp.gate_proj", y)) * self._lin(b + "mlp.up_proj", y))
+        return self._rms("norm", x)
+
+    # ---- batches -------------------------------------------------------------------------------
+
+    def _tokens(self, ids: Sequence[Sequence[int]]) -> Tuple[torch.Tensor, PackedLayout]:
+        flat = np.fromiter((t for s in ids for t in s), np.int64, sum(len(s) for s in ids))
+        return torch.from_numpy(flat).to(self.device), PackedLayout([len(s) for s in ids], device=self.device)
+
+    def hidden_states(self, ids: Sequence[Sequence[int]]) -> Tuple[torch.Tensor, PackedLayout]:
+        """Last hidden states [tokens, hidden] of token id sequences, and their layout."""
+        tok, layout = self._tokens(ids)
+        return (self._post if self.kind == "post" else self._causal)(tok, layout), layout
+
+    def pooled(self, ids: Sequence[Sequence[int]], normalize: bool) -> torch.Tensor:
+        """float32 [n, hidden]: the mean of each sequence's last hidden states."""
+        share = 0 if self.kind == "post" or torch.is_grad_enabled() else common_prefix(ids)
+        if share < SHARE_FROM:
+            h, layout = self.hidden_states(ids)
+            return packed_mean_pool(h, layout, normalize=normalize)
+        kept: List[tuple] = []
+        tok, layout = self._tokens([ids[0][:share]])
+        head = self._causal(tok, layout, keep=kept).float().sum(0)
+        tok, layout = self._tokens([s[share:] for s in ids])
+        mean = packed_mean_pool(self._causal(tok, layout, share, kept), layout)
+        n = torch.tensor([len(s) for s in ids], dtype=torch.float32, device=self.device)[:, None]
+        y = (mean * (n - share) + head) / n
+        return F.normalize(y, dim=1) if normalize else y
+
+
+def common_prefix(ids: Sequence[Sequence[int]]) -> int:
+    """Tokens that all sequences begin with; each keeps one of its own. 0 for fewer than two sequences."""
+    if len(ids) < 2:
+        return 0
+    a, b = min(ids), max(ids)  # in order, what the first and the last share, all share
+    n = 0
+    for x, y in zip(a, b):
+        if x != y:
+            break
+        n += 1
+    return max(0, min(n, min(len(s) for s in ids) - 1))

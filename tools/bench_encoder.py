@@ -60,12 +60,13 @@ def main():
     ap.add_argument("--corpus", type=int, default=20000)
     ap.add_argument("--batch", type=int, default=1024)
     ap.add_argument("--reps", type=int, default=3)
+    ap.add_argument("--packed", action="store_true", help="batches without padding (ah_rag.packed_encoder)")
     a = ap.parse_args()
     dev = torch.device("cuda", 0)
     out = {"weights": "seeded random (no checkpoint offline); forward, shapes and sequence lengths are the real ones"}
     corpus_texts = texts(a.corpus, 1)
     for model in ("all-MiniLM-L6-v2", "all-mpnet-base-v2"):
-        enc = TorchEncoder(model, dev)
+        enc = TorchEncoder(model, dev, packed=a.packed)
         ntok = sum(len(t) for t in enc.tokenizer(corpus_texts))
         seq = ntok / len(corpus_texts)
         dt = timed(lambda: enc.encode(corpus_texts, normalize_embeddings=True, convert_to_tensor=True), a.reps)
