@@ -227,6 +227,13 @@ def _keep(lists: Optional[torch.Tensor], stream: int, device: torch.device) -> N
 # ---- attention -------------------------------------------------------------------------------
 
 
+def _once() -> None:
+    """The gradients are not differentiable again. (torch's once_differentiable says the same at the cost of a
+    small kernel.)"""
+    if torch.is_grad_enabled():
+        raise RuntimeError("the packed operators have no second derivative (backward with create_graph=True)")
+
+
 def _workspace(plan: nat.AttnPlan, device: torch.device) -> Optional[torch.Tensor]:
     return torch.empty(plan.ws_bytes, dtype=torch.uint8, device=device) if plan.ws_bytes else None
 
@@ -260,20 +267,21 @@ class _PackedAttention(torch.autograd.Function):
         lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device)
         o = _attention(q, k, v, layout, causal, scale, lse)
         # the backward pass's lists too: its first call may be inside a capture
-        layout._plan(_CODES[q.dtype], q.shape[1], k.shape[1], q.shape[2], causal, True, 0)
+        ctx.plan = layout._plan(_CODES[q.dtype], q.shape[1], k.shape[1], q.shape[2], causal, True, 0)
         ctx.save_for_backward(q, k, v, o, lse)
-        ctx.layout, ctx.causal, ctx.scale = layout, causal, scale
+        ctx.scale = scale
         return o
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, d_o):
+    def backward(ctx, d_o):  # (on the device and stream of the forward call)
+        _once()
         q, k, v, o, lse = ctx.saved_tensors
-        with torch.cuda.device(q.device):
-            plan, lists = ctx.layout._plan(_CODES[q.dtype], q.shape[1], k.shape[1], q.shape[2], ctx.causal, True, 0)
-            dq, dk, dv = (torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in (q, k, v))
-            _launch_attention(_calls().attn_backward, "ahr_attn_backward", plan, lists, ctx.scale, q, k, v, None, None, _aligned(o), lse,
-                              _aligned(d_o), dq, dk, dv)
+        plan, lists = ctx.plan
+        shape, kshape, dtype, device = q.shape, k.shape, q.dtype, q.device
+        dq = torch.empty(shape, dtype=dtype, device=device)
+        dk, dv = torch.empty((2, *kshape), dtype=dtype, device=device).unbind(0)
+        _launch_attention(_calls().attn_backward, "ahr_attn_backward", plan, lists, ctx.scale, q, k, v, None, None, _aligned(o), lse,
+                          _aligned(d_o), dq, dk, dv)
         return dq, dk, dv, None, None, None
 
 
@@ -417,21 +425,23 @@ class _QkNormRope(torch.autograd.Function):
         return _rope_forward(q, k, wq, wk, cos, sin, positions, eps, interleaved)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dyq, dyk):
+        _once()
         q, k, wq, wk, cos, sin, positions = ctx.saved_tensors
-        with torch.cuda.device(q.device):
-            dim = q.shape[2]
-            dq, dk = torch.empty(q.shape, dtype=q.dtype, device=q.device), torch.empty(k.shape, dtype=k.dtype, device=k.device)
-            dw = ws = None
-            if wq is not None:
-                n = ctypes.c_int64()
-                nat.check(nat.lib().ahr_rope_ws_bytes(q.shape[0], dim, ctypes.byref(n)), "ahr_rope_ws_bytes")
-                ws = torch.empty(n.value, dtype=torch.uint8, device=q.device)
-                dw = torch.empty((2, dim), dtype=torch.float32, device=q.device)
-            _launch_rope(_calls().rope_backward, "ahr_qk_norm_rope_backward", q, k, cos, sin, positions, ctx.eps, ctx.interleaved, wq, wk,
-                         _unit(dyq), _unit(dyk), dq, dk, dw, ws)
-        gq, gk = (None, None) if dw is None else (dw[0].to(ctx.w_dtype[0]), dw[1].to(ctx.w_dtype[1]))
+        dim, device = q.shape[2], q.device
+        dq, dk = torch.empty(q.shape, dtype=q.dtype, device=device), torch.empty(k.shape, dtype=k.dtype, device=device)
+        dw = ws = gq = gk = None
+        if wq is not None:
+            n = ctypes.c_int64()
+            nat.check(nat.lib().ahr_rope_ws_bytes(q.shape[0], dim, ctypes.byref(n)), "ahr_rope_ws_bytes")
+            ws = torch.empty(n.value, dtype=torch.uint8, device=device)
+            dw = torch.empty((2, dim), dtype=torch.float32, device=device)
+        _launch_rope(_calls().rope_backward, "ahr_qk_norm_rope_backward", q, k, cos, sin, positions, ctx.eps, ctx.interleaved, wq, wk,
+                     _unit(dyq), _unit(dyk), dq, dk, dw, ws)
+        if dw is not None:
+            gq, gk = dw.unbind(0)
+            if ctx.w_dtype != (torch.float32, torch.float32):
+                gq, gk = gq.to(ctx.w_dtype[0]), gk.to(ctx.w_dtype[1])
         return dq, dk, gq, gk, None, None, None, None, None
 
 
@@ -513,18 +523,18 @@ class _PackedMeanPool(torch.autograd.Function):
         return out
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, d_out):
+        _once()
         out, norm = ctx.saved_tensors
-        with torch.cuda.device(out.device):
-            n_chunks, lists = ctx.layout._pool_lists()
-            d_out = d_out.contiguous()
-            d_rows = torch.empty(ctx.shape, dtype=ctx.dtype, device=out.device)
-            stream = nat.stream_ptr(device_index=out.device.index)
-            nat.check(nat.lib().ahr_pool_mean_backward(_CODES[ctx.dtype], d_rows.data_ptr(), ctx.shape[1], lists.data_ptr(),
-                                                       n_chunks, len(ctx.layout), int(ctx.normalize), d_out.data_ptr(),
-                                                       out.data_ptr(), norm.data_ptr(), stream), "ahr_pool_mean_backward")
-            _keep(lists, stream, out.device)
+        layout = ctx.layout
+        n_chunks, lists = layout._pool_lists()
+        d_out = d_out.contiguous()
+        d_rows = torch.empty(ctx.shape, dtype=ctx.dtype, device=out.device)
+        stream = nat.stream_ptr(device_index=out.device.index)
+        nat.check(nat.lib().ahr_pool_mean_backward(_CODES[ctx.dtype], d_rows.data_ptr(), ctx.shape[1], lists.data_ptr(), n_chunks,
+                                                   len(layout), ctx.normalize, d_out.data_ptr(), out.data_ptr(), norm.data_ptr(), stream),
+                  "ahr_pool_mean_backward")
+        _keep(lists, stream, out.device)
         return d_rows, None, None
 
 

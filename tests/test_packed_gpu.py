@@ -423,6 +423,16 @@ def test_empty_batches(cuda):
         assert not torch.autograd.grad((a, b), w, (a.detach(), b.detach()))[0].any()
 
 
+def test_second_derivatives_are_refused(cuda):
+    from ah_rag.packed import PackedLayout, packed_attention, packed_mean_pool, qk_norm_rope, rotary_table
+    lay = PackedLayout([4], device=cuda)
+    x = torch.randn(4, 2, 64, dtype=BF, device=cuda, requires_grad=True)
+    cos, sin = rotary_table(4, 64, device=cuda)
+    for y in (packed_attention(x, x, x, lay), packed_mean_pool(x.flatten(1), lay), qk_norm_rope(x, x, None, None, cos, sin, lay.positions())[0]):
+        with pytest.raises(RuntimeError, match="second derivative"):
+            torch.autograd.grad(y.sum(), x, create_graph=True)
+
+
 def test_gpu_refusals(cuda):
     from ah_rag.packed import PackedLayout, packed_attention, prefix_attention
     lay = PackedLayout([4], device=cuda)
