@@ -53,7 +53,7 @@ def _host_lengths(x: Lengths, what: str) -> np.ndarray:
         raise ValueError(f"{what} must be a list of whole numbers")
     if a.size and (a.min() < 0 or int(a.sum(dtype=np.int64)) > 1 << 30):
         raise ValueError(f"{what} must be >= 0 and sum to at most 2**30")
-    return np.ascontiguousarray(a, dtype=np.int32)
+    return np.array(a, dtype=np.int32)  # (a copy: the layout's own)
 
 
 class PackedLayout:
@@ -219,9 +219,17 @@ def _on(stream: Optional[torch.cuda.Stream], device: torch.device, *tensors: Opt
 
 
 def _keep(lists: Optional[torch.Tensor], stream: int, device: torch.device) -> None:
-    """The layout may be dropped while another stream than the one that made its lists still reads them."""
-    if lists is not None and lists.ahr_stream != stream and not torch.cuda.is_current_stream_capturing():
+    """The layout may be dropped while another stream than the one that made its lists still reads them, or
+    while a graph that captured the call can still be replayed (such lists, a few KB, are never freed)."""
+    if lists is None:
+        return
+    if torch.cuda.is_current_stream_capturing():
+        _CAPTURED[id(lists)] = lists
+    elif lists.ahr_stream != stream:
         lists.record_stream(torch.cuda.current_stream(device))
+
+
+_CAPTURED: Dict[int, torch.Tensor] = {}
 
 
 # ---- attention -------------------------------------------------------------------------------

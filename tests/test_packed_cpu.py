@@ -223,6 +223,10 @@ def test_layout_refusals():
     lay = PackedLayout(torch.tensor([2, 0, 3]), [4, 1, 3], device="cuda:0")
     assert (len(lay), lay.tokens, lay.key_tokens) == (3, 5, 8)
     assert PackedLayout([], device="cuda:0").tokens == 0
+    mine = np.array([4, 5], np.int32)
+    lay = PackedLayout(mine, device="cuda:0")
+    mine[:] = 9
+    assert lay.lengths.tolist() == [4, 5]
 
 
 def test_call_refusals():

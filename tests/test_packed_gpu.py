@@ -109,6 +109,36 @@ def test_prefix_attention(cuda, shape, prefix):
     _within(o, w, t, "o")
 
 
+@pytest.mark.parametrize("dim,heads,kv_heads,causal", [(64, 12, 12, False), (32, 12, 12, True), (128, 8, 2, True)])
+def test_a_batch_of_many_texts(cuda, dim, heads, kv_heads, causal):
+    """64 texts of 1 to 384 tokens, as an encoder's batch: tiles of every fill, workgroups at different tiles at once.
+    The reference padded, in 64 bits on the GPU; the bound that of the small cases for values of size one."""
+    from ah_rag.packed import PackedLayout, packed_attention
+    rng = torch.Generator().manual_seed(8)
+    lens = torch.randint(1, 385, (64,), generator=rng).tolist()
+    q, k, v, d_o = _make((lens, None, heads, kv_heads, dim, causal, BF), 9, cuda)
+    leaves = [x.detach().requires_grad_() for x in (q, k, v)]
+    o = packed_attention(*leaves, PackedLayout(lens, device=cuda), causal=causal)
+    grads = torch.autograd.grad(o, leaves, d_o)
+    n = torch.tensor(lens, device=cuda)
+    at = torch.arange(384, device=cuda)
+    real = at < n[:, None]
+    idx = torch.where(real, (torch.cumsum(n, 0) - n)[:, None] + at, 0)
+    L = [x.detach().double().requires_grad_() for x in (q, k, v)]
+    Q, K, V = (x[idx].transpose(1, 2) for x in L)
+    K, V = (x.repeat_interleave(heads // kv_heads, 1) for x in (K, V))
+    see = real[:, None, None, :] & (~torch.ones(384, 384, dtype=torch.bool, device=cuda).triu(1) | (not causal))
+    p = torch.softmax((Q @ K.transpose(2, 3) * dim ** -0.5).masked_fill(~see, -math.inf), -1)
+    w = (p @ V).transpose(1, 2)[real]
+    wg = torch.autograd.grad(w, L, d_o.double())
+    u = ref.half_step(BF)
+    # o: the weights' rounding (u of sum p |v|, here at most u max |v|) and its own; gradients: twice as many roundings of
+    # terms that are sums over up to 384 rows of such size
+    assert ((o - w).abs() <= u * (w.abs() + 6.0)).all()
+    for a, b in zip(grads, wg):
+        assert float((a - b).norm() / b.norm()) < 4 * u
+
+
 def test_one_long_sequence(cuda):
     """Many tiles, a length that ends inside one; the reference by blocks in 64 bits."""
     from ah_rag.packed import PackedLayout, packed_attention
@@ -384,6 +414,36 @@ def test_captured_step_replays(cuda):
         torch.cuda.synchronize()
         for a, b in zip(outs, want):
             assert torch.equal(a, b)
+
+
+def test_graph_outlives_its_layout(cuda):
+    """Nothing but the graph holds the work lists when it is replayed."""
+    import gc
+    from ah_rag.packed import PackedLayout, packed_attention, packed_mean_pool
+    shape = ([50, 3, 80], None, 4, 2, 64, True, BF)
+    q, k, v, d_o = _make(shape, 43, cuda)
+    leaves = [x.detach().requires_grad_() for x in (q, k, v)]
+
+    def step(lay):
+        o = packed_attention(*leaves, lay, causal=True)
+        return [o.detach(), packed_mean_pool(o.detach().flatten(1), lay), *torch.autograd.grad(o, leaves, d_o)]
+
+    lay = PackedLayout(shape[0], device=cuda)
+    want = step(lay)
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        outs = step(lay)
+    del lay
+    gc.collect()
+    junk = [torch.full((1 << n,), -1, dtype=torch.int32, device=cuda) for n in range(4, 16) for _ in range(8)]
+    for _ in range(3):
+        for o in outs:
+            o.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(outs, want))
+    assert len(junk) == 96
 
 
 def test_layout_during_capture_is_refused(cuda):
