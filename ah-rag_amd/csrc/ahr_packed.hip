@@ -45,40 +45,55 @@ struct Rope {
   int64_t q_ts, q_hs, k_ts, k_hs, yq_ts, yq_hs, yk_ts, yk_hs, oq_ts, oq_hs, ok_ts, ok_hs;
   const float *wq, *wk, *cos, *sin;
   const int32_t* pos;
-  float* part;  // backward: [blocks][2][dim]
+  float* part;  // backward: [part_q + part_k][dim], the weights' gradients of q's and k's workgroups
   int64_t tokens, n_pos;
   int heads, kv_heads, dim, rot;
+  int q_blocks;  // vector form: workgroups (x) of q, the others take k
   float eps;
 };
 
 // Vector form (rot == head_dim, a multiple of 16, aligned rows). LPR lanes share a head's row; a lane
 // owns 8 pairs of the rotation: elements a = e0 .. e0+7 and b = e0 + dim/2 .. (interleaved: 16
-// consecutive elements, pair i = (2i, 2i+1)), so the rotation needs no exchange between lanes. A wave
-// takes one token at a time and keeps the lane's cos and sin for all its heads. BWD: dx and the
-// weights' gradients; each lane adds its part of dw over its tokens in registers, the workgroup joins
-// them into one partial row.
+// consecutive elements, pair i = (2i, 2i+1)), so the rotation needs no exchange between lanes. A
+// workgroup takes q or k, so that a lane keeps one side's weights (and one side's part of their
+// gradients: both sides' took 138 registers, three waves a SIMD, and a select for each use; 170 us
+// backward where this takes 150); a wave takes one token at a time and keeps the lane's cos and sin
+// for all its heads. BWD: dx and the weights' gradients; each lane adds its part of dw over its
+// tokens in registers, the workgroup joins them into one partial row.
+// Bound by memory: 22.8k tokens of 32 + 8 heads of 128 in bf16 take 95 us forward (467 MB, 4.9 TB/s,
+// which is what a copy reaches) and 150 us backward (700 MB, 4.7 TB/s).
 template <typename T, int DIM, bool IL, bool BWD>
-__global__ __launch_bounds__(256) void rope_vec_kernel(Rope p) {
+__global__ __launch_bounds__(256, 4) void rope_vec_kernel(Rope p) {
   constexpr int LPR = DIM / 16;          // lanes of a row
-  constexpr int RPW = 64 / LPR;          // rows of a wave (lanes past RPW * LPR idle)
+  constexpr int RPW = 64 / LPR;          // rows of a wave
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int sub = lane / LPR, li = lane % LPR;
-  const bool on = sub < RPW;
   const int e0 = IL ? li * 16 : li * 8;
-  const bool normed = p.wq != nullptr;
-  float w[2][16], dw[2][16];
+  const bool normed = p.wq != nullptr, is_k = (int)blockIdx.x >= p.q_blocks;
+  const int heads = is_k ? p.kv_heads : p.heads;
+  const int block = is_k ? blockIdx.x - p.q_blocks : blockIdx.x, blocks = is_k ? gridDim.x - p.q_blocks : p.q_blocks;
+  const T* xs = (const T*)(is_k ? p.k : p.q);
+  const T* ys = (const T*)(is_k ? p.yk : p.yq);
+  T* os = (T*)(is_k ? p.ok : p.oq);
+  const int64_t x_ts = is_k ? p.k_ts : p.q_ts, x_hs = is_k ? p.k_hs : p.q_hs, y_ts = is_k ? p.yk_ts : p.yq_ts, y_hs = is_k ? p.yk_hs : p.yq_hs,
+                o_ts = is_k ? p.ok_ts : p.oq_ts, o_hs = is_k ? p.ok_hs : p.oq_hs;
+  float w[16], dw[16];
 #pragma unroll
-  for (int s = 0; s < 2; ++s)
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const int e = IL ? e0 + i : (i < 8 ? e0 + i : DIM / 2 + e0 + i - 8);
-      w[s][i] = normed ? (s ? p.wk : p.wq)[e] : 1.f;
-      dw[s][i] = 0.f;
+  for (int i = 0; i < 16; ++i) {
+    const int e = IL ? e0 + i : (i < 8 ? e0 + i : DIM / 2 + e0 + i - 8);
+    w[i] = normed ? (is_k ? p.wk : p.wq)[e] : 1.f;
+    dw[i] = 0.f;
+  }
+  auto load = [&](float* to, const T* row) {
+    if (IL) {
+      load_f32<T, 16>(to, row + e0);
+    } else {
+      load_f32<T, 8>(to, row + e0);
+      load_f32<T, 8>(to + 8, row + DIM / 2 + e0);
     }
-  const int all = p.heads + p.kv_heads;
+  };
   // heads of a token are dealt to gridDim.y slices
-  const int first = blockIdx.y * RPW, step = gridDim.y * RPW;
-  for (int64_t t = (int64_t)blockIdx.x * 4 + wave; t < p.tokens; t += (int64_t)gridDim.x * 4) {
+  for (int64_t t = (int64_t)block * 4 + wave; t < p.tokens; t += (int64_t)blocks * 4) {
     const int64_t at = p.pos[t];
     const bool known = at >= 0 && at < p.n_pos;
     float c[8], s[8];
@@ -91,29 +106,13 @@ __global__ __launch_bounds__(256) void rope_vec_kernel(Rope p) {
         for (int i = 0; i < 8; ++i) c[i] = s[i] = NAN;
       }
     }
-    for (int h0 = first; h0 < all; h0 += step) {
+    for (int h0 = blockIdx.y * RPW; h0 < heads; h0 += gridDim.y * RPW) {
       const int hd = h0 + sub;
-      const bool have = on && hd < all;
-      const bool is_k = hd >= p.heads;
-      const int hh = is_k ? hd - p.heads : hd;
+      const bool have = hd < heads;
       float x[16], y[16];
       if (have) {
-        const T* xp = (const T*)(is_k ? p.k : p.q) + (is_k ? t * p.k_ts + hh * p.k_hs : t * p.q_ts + hh * p.q_hs);
-        if (IL) {
-          load_f32<T, 16>(x, xp + e0);
-        } else {
-          load_f32<T, 8>(x, xp + e0);
-          load_f32<T, 8>(x + 8, xp + DIM / 2 + e0);
-        }
-        if (BWD) {
-          const T* yp = (const T*)(is_k ? p.yk : p.yq) + (is_k ? t * p.yk_ts + hh * p.yk_hs : t * p.yq_ts + hh * p.yq_hs);
-          if (IL) {
-            load_f32<T, 16>(y, yp + e0);
-          } else {
-            load_f32<T, 8>(y, yp + e0);
-            load_f32<T, 8>(y + 8, yp + DIM / 2 + e0);
-          }
-        }
+        load(x, xs + t * x_ts + hd * x_hs);
+        if (BWD) load(y, ys + t * y_ts + hd * y_hs);
       } else {
 #pragma unroll
         for (int i = 0; i < 16; ++i) x[i] = y[i] = 0.f;
@@ -128,13 +127,12 @@ __global__ __launch_bounds__(256) void rope_vec_kernel(Rope p) {
           if (m < LPR) sum += __shfl_xor(sum, m, 64);
         r = 1.f / sqrtf(sum * (1.f / DIM) + p.eps);
       }
-      const int sl = is_k ? 1 : 0;
       float o[16];
       if (!BWD) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           const int a = IL ? 2 * i : i, b = IL ? 2 * i + 1 : i + 8;
-          const float na = x[a] * r * (sl ? w[1][a] : w[0][a]), nb = x[b] * r * (sl ? w[1][b] : w[0][b]);
+          const float na = x[a] * r * w[a], nb = x[b] * r * w[b];
           o[a] = na * c[i] - nb * s[i];
           o[b] = nb * c[i] + na * s[i];
         }
@@ -145,16 +143,13 @@ __global__ __launch_bounds__(256) void rope_vec_kernel(Rope p) {
         for (int i = 0; i < 8; ++i) {
           const int a = IL ? 2 * i : i, b = IL ? 2 * i + 1 : i + 8;
           float da = y[a] * c[i] + y[b] * s[i], db = y[b] * c[i] - y[a] * s[i];
-          const float ua = da * x[a] * r, ub = db * x[b] * r;
           // (idle rows hold zeros; an unknown position's NaN belongs to rows that exist)
           if (have) {
-            dw[0][a] += sl ? 0.f : ua;
-            dw[0][b] += sl ? 0.f : ub;
-            dw[1][a] += sl ? ua : 0.f;
-            dw[1][b] += sl ? ub : 0.f;
+            dw[a] = fmaf(da, x[a] * r, dw[a]);
+            dw[b] = fmaf(db, x[b] * r, dw[b]);
           }
-          da *= sl ? w[1][a] : w[0][a];
-          db *= sl ? w[1][b] : w[0][b];
+          da *= w[a];
+          db *= w[b];
           dot = fmaf(da, x[a], fmaf(db, x[b], dot));
           o[a] = da;
           o[b] = db;
@@ -169,7 +164,7 @@ __global__ __launch_bounds__(256) void rope_vec_kernel(Rope p) {
         }
       }
       if (have) {
-        T* op = (T*)(is_k ? p.ok : p.oq) + (is_k ? t * p.ok_ts + hh * p.ok_hs : t * p.oq_ts + hh * p.oq_hs);
+        T* op = os + t * o_ts + hd * o_hs;
         if (IL) {
           store_f32<T, 16>(op + e0, o);
         } else {
@@ -181,22 +176,16 @@ __global__ __launch_bounds__(256) void rope_vec_kernel(Rope p) {
   }
   if (BWD && normed) {
     // the rows of a wave, then the four waves, in a fixed order
-    __shared__ float acc[4][RPW][2][DIM];
-    if (on) {
+    __shared__ float acc[4][RPW][DIM];
 #pragma unroll
-      for (int s = 0; s < 2; ++s)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int e = IL ? e0 + i : (i < 8 ? e0 + i : DIM / 2 + e0 + i - 8);
-          acc[wave][sub][s][e] = dw[s][i];
-        }
-    }
+    for (int i = 0; i < 16; ++i) acc[wave][sub][IL ? e0 + i : (i < 8 ? e0 + i : DIM / 2 + e0 + i - 8)] = dw[i];
     __syncthreads();
-    for (int i = threadIdx.x; i < 2 * DIM; i += 256) {
+    for (int e = threadIdx.x; e < DIM; e += 256) {
       float sum = 0.f;
       for (int a = 0; a < 4; ++a)
-        for (int b = 0; b < RPW; ++b) sum += acc[a][b][i / DIM][i % DIM];
-      p.part[((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * 2 * DIM + i] = sum;
+        for (int b = 0; b < RPW; ++b) sum += acc[a][b][e];
+      const int row = (is_k ? p.q_blocks * gridDim.y : 0) + blockIdx.y * blocks + block;
+      p.part[(int64_t)row * DIM + e] = sum;
     }
   }
 }
@@ -278,25 +267,32 @@ __global__ __launch_bounds__(256) void rope_any_kernel(Rope p, int il) {
     __syncthreads();
     for (int i = threadIdx.x; i < 2 * p.dim; i += 256) {
       const int s = i / p.dim, e = i % p.dim;
-      p.part[(int64_t)blockIdx.x * 2 * p.dim + i] = acc[0][s][e] + acc[1][s][e] + acc[2][s][e] + acc[3][s][e];
+      p.part[((int64_t)s * gridDim.x + blockIdx.x) * p.dim + e] = acc[0][s][e] + acc[1][s][e] + acc[2][s][e] + acc[3][s][e];
     }
   }
 }
 
-// dw = the sum of the workgroups' partial rows: a workgroup per 16 columns, 16 threads a column
-__global__ __launch_bounds__(256) void rope_dw_kernel(const float* part, int blocks, int dim, float* dwq, float* dwk) {
-  __shared__ float acc[16][17];
-  const int col = blockIdx.x * 16 + (threadIdx.x & 15), y = threadIdx.x >> 4;
+// dw = the sum of the workgroups' partial rows: a workgroup per 16 columns, 64 threads a column, so that few
+// loads of a thread follow each other (1024 rows of 128, 16 threads a column: 17 us, 64: 6)
+__global__ __launch_bounds__(1024) void rope_dw_kernel(const float* part, int part_q, int part_k, int dim, float* dwq, float* dwk) {
+  __shared__ float acc[16][16];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int col = blockIdx.x * 16 + (lane & 15);
+  const bool is_k = col >= dim;
+  const int rows = col < 2 * dim ? (is_k ? part_k : part_q) : 0;
+  const float* from = part + (is_k ? (int64_t)part_q * dim + col - dim : col);
   float s = 0.f;
-  if (col < 2 * dim)
 #pragma unroll 8
-    for (int b = y; b < blocks; b += 16) s += part[(int64_t)b * 2 * dim + col];
-  acc[y][threadIdx.x & 15] = s;
+  for (int b = threadIdx.x >> 4; b < rows; b += 64) s += from[(int64_t)b * dim];
+  s += __shfl_xor(s, 16, 64);
+  s += __shfl_xor(s, 32, 64);
+  if (lane < 16) acc[wave][lane] = s;
   __syncthreads();
-  if (y == 0 && col < 2 * dim) {
+  if (threadIdx.x < 16 && col < 2 * dim) {
     float t = 0.f;
-    for (int i = 0; i < 16; ++i) t += acc[i][threadIdx.x & 15];
-    (col < dim ? dwq : dwk)[col % dim] = t;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) t += acc[i][threadIdx.x];
+    (is_k ? dwk : dwq)[is_k ? col - dim : col] = t;
   }
 }
 
@@ -328,7 +324,7 @@ static int rope_check(const ahr_rope_args* a, bool bwd) {
 }
 
 template <typename T, bool BWD>
-static int rope_launch(const ahr_rope_args* a, const Rope& p, hipStream_t s) {
+static int rope_launch(const ahr_rope_args* a, Rope p, hipStream_t s) {
   const ahr_tensor3* t[6] = {&a->q, &a->yq, &a->dq, &a->k, &a->yk, &a->dk};
   const int al = 16 / (int)sizeof(T);
   bool vec = a->rot == a->head_dim;
@@ -338,32 +334,38 @@ static int rope_launch(const ahr_rope_args* a, const Rope& p, hipStream_t s) {
   }
   vec = vec && reinterpret_cast<uintptr_t>(p.cos) % 16 == 0 && reinterpret_cast<uintptr_t>(p.sin) % 16 == 0;
   const int all = a->heads + a->kv_heads;
-  int blocks = 0;
+  int part_q = 0, part_k = 0;
   const int il = a->interleaved;
 #define AHR_ROPE(D)                                                                                     \
   {                                                                                                     \
-    const int rpw = 64 / (D / 16), rounds = (all + rpw - 1) / rpw;                                      \
+    const int rpw = 64 / (D / 16), rounds = (std::max(a->heads, a->kv_heads) + rpw - 1) / rpw;          \
     const int64_t want = (a->tokens + 3) / 4;                                                           \
     /* few tokens: a token's heads are spread over more waves, for latency */                           \
     int gy = 1;                                                                                         \
     while (gy < rounds && want * gy < 512) gy *= 2;                                                     \
-    const int gx = (int)std::min<int64_t>(want, BWD ? kRopeBlocks / gy : 65536);                        \
-    blocks = gx * gy;                                                                                   \
-    if (il) rope_vec_kernel<T, D, true, BWD><<<dim3(gx, gy), 256, 0, s>>>(p);                           \
-    else rope_vec_kernel<T, D, false, BWD><<<dim3(gx, gy), 256, 0, s>>>(p);                             \
+    /* backward: one round of resident workgroups, dealt to q and k as the heads are */                 \
+    const int most = BWD ? kRopeBlocks / gy : 65536;                                                    \
+    const int k_most = BWD ? std::max(1, (int)((int64_t)most * a->kv_heads / all)) : most;              \
+    const int bq = a->heads ? (int)std::min<int64_t>(want, BWD ? std::max(1, most - k_most) : most) : 0; \
+    const int bk = a->kv_heads ? (int)std::min<int64_t>(want, k_most) : 0;                              \
+    p.q_blocks = bq;                                                                                    \
+    part_q = bq * gy, part_k = bk * gy;                                                                 \
+    if (il) rope_vec_kernel<T, D, true, BWD><<<dim3(bq + bk, gy), 256, 0, s>>>(p);                      \
+    else rope_vec_kernel<T, D, false, BWD><<<dim3(bq + bk, gy), 256, 0, s>>>(p);                        \
   }
   if (vec && a->head_dim == 32) AHR_ROPE(32)
   else if (vec && a->head_dim == 64) AHR_ROPE(64)
   else if (vec && a->head_dim == 128) AHR_ROPE(128)
   else if (vec && a->head_dim == 256) AHR_ROPE(256)
   else {
-    blocks = (int)std::min<int64_t>((a->tokens * all + 3) / 4, BWD ? kRopeBlocks : 65536);
+    const int blocks = (int)std::min<int64_t>((a->tokens * all + 3) / 4, BWD ? kRopeBlocks : 65536);
+    part_q = part_k = blocks;
     rope_any_kernel<T, BWD><<<dim3(blocks), 256, 0, s>>>(p, il);
   }
 #undef AHR_ROPE
   AHR_HIP(hipGetLastError());
   if (BWD && a->wq) {
-    rope_dw_kernel<<<dim3((2 * a->head_dim + 15) / 16), 256, 0, s>>>(p.part, blocks, a->head_dim, a->dwq, a->dwk);
+    rope_dw_kernel<<<dim3((2 * a->head_dim + 15) / 16), 1024, 0, s>>>(p.part, part_q, part_k, a->head_dim, a->dwq, a->dwk);
     AHR_HIP(hipGetLastError());
   }
   return AHR_OK;
@@ -390,7 +392,7 @@ static int rope(const ahr_rope_args* a, void* stream) {
   p.eps = a->eps;
   if (a->tokens == 0) {
     if (BWD && a->wq) {  // no rows: zero weight gradients
-      rope_dw_kernel<<<dim3((2 * a->head_dim + 15) / 16), 256, 0, s>>>(p.part, 0, a->head_dim, a->dwq, a->dwk);
+      rope_dw_kernel<<<dim3((2 * a->head_dim + 15) / 16), 1024, 0, s>>>(p.part, 0, 0, a->head_dim, a->dwq, a->dwk);
       AHR_HIP(hipGetLastError());
     }
     return AHR_OK;
