@@ -1,6 +1,6 @@
 // Attention over packed sequences, backward (include/ahr.h ahr_attn_backward).
 //
-// With p = 2^(c s - lse), delta = sum_d do o and ds = p (do . v - delta):
+// With p = 2^(c s - lse), delta = sum_d do o (= sum_j p (do . v)) and ds = p (do . v - delta):
 //   dv_j = sum_i p_ij do_i,   dk_j = scale sum_i ds_ij q_i,   dq_i = scale sum_j ds_ij k_j.
 // Two kernels recompute p, one for each direction of the sum: dk and dv stay in the registers of the
 // wave that owns 32 keys while the query rows of every head of the group pass through LDS; dq stays
@@ -383,6 +383,31 @@ __device__ __forceinline__ void row_tile(const char* __restrict__ cur, RowState<
   }
 }
 
+// delta = sum_j p_j (do . v_j) of this lane's row, whose keys all lie in one staged tile. Equal to sum_d do o but
+// for o's rounding to 16 bits, which with few keys is as large as that of ds (in units of dq, bf16, against
+// 0.0024 with an exact delta: 0.0030 for 4 keys a row, 0.0025 for 16, 0.0024 from 64 on, where it no longer counts).
+template <typename T, int DP>
+__device__ __forceinline__ float row_delta(const char* __restrict__ cur, const RowState<T, DP>& st, int mine, float c, int lane) {
+  constexpr int NC = DP / 8, KS = DP / 16;
+  constexpr int kTile = kKeys * DP * 2;
+  const int h = lane >> 5, n = lane & 31;
+  float sum = 0.f;
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    f32x16 s, g;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s[r] = g[r] = 0.f;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      s = Elem<T>::mma(row_frag<T, NC>(cur, u * 32 + n, ks, h), st.qf[ks], s);
+      g = Elem<T>::mma(row_frag<T, NC>(cur + kTile, u * 32 + n, ks, h), st.of[ks], g);
+    }
+#pragma unroll
+    for (int r = 0; r < 16; ++r) sum += u * 32 + acc_row(r, h) < mine ? ex2(fmaf(s[r], c, -st.lse)) * g[r] : 0.f;
+  }
+  return sum + other_half(sum);
+}
+
 template <typename T, int DP>
 __device__ __forceinline__ void row_step(const char* __restrict__ cur, char* __restrict__ nxt, RowState<T, DP>& st,
                                          const Stager<DP / 8, kWaves, kKeys>& stager, const Params& p, const RowItem& it, int hk, int t, int nt,
@@ -441,13 +466,17 @@ __global__ __launch_bounds__(kWaves * 64, 2) void attn_dq_kernel(Params p) {
   const Stager<DP / 8, kWaves, kKeys> stager(wave, lane);
   const int nt = (it.ke + kKeys - 1) / kKeys;
   if (nt > 0) row_step<T, DP>(smem, smem, st, stager, p, it, hk, -1, nt, false, 0, 0, 0, lane);
-  {  // delta = sum_d do o of this lane's row, written for the dk/dv kernel that follows
+  {  // delta of this lane's row, written for the dk/dv kernel that follows
     float x = 0.f;
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
       for (int i = 0; i < 8; ++i) x = fmaf((float)ov[ks][i], (float)st.of[ks][i], x);
     st.delta = x + other_half(x);
+    if (nt == 1) {
+      tile_barrier();
+      if (wave_live) st.delta = row_delta<T, DP>(smem, st, min(lim, it.ke), p.scale_log2, lane);
+    }
     if (live && h == 0) p.delta[li] = st.delta;
   }
   if (nt > 0) {

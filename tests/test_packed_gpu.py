@@ -251,6 +251,37 @@ def test_scales_and_large_scores(cuda, scale):
         _within(a, w, t, name)
 
 
+@pytest.mark.parametrize("dt", [BF, HF])
+@pytest.mark.parametrize("lens,causal", [([1, 2, 3, 8, 64, 33], False), ([1, 5, 40, 2], True)])
+def test_few_keys_keep_the_small_gradients(cuda, lens, causal, dt):
+    """Where one key takes nearly all the weight, ds = p (dp - delta) is far smaller than delta, and a delta from the
+    rounded output would drown it. The kernel's is exact to 32 bits where a row's keys lie in one tile: with u half a
+    step of the type, p off by 2^-17 (the roundings of c s and of the stored logarithm, each below 2^7, 2^-17 in
+    exp2's argument, times ln 2), ds_j is off by u |ds_j| + 2^-16 p_j (|dp_j| + sum_i p_i |dp_i|), and dq by the sum of
+    these times |k_j| and its own rounding. (f16 holds ds times a power of two, so it has no smallest value here.)"""
+    from ah_rag.packed import PackedLayout, packed_attention
+    hq, hk, d = 4, 2, 64
+    q, k, v, do = _make((lens, None, hq, hk, d, causal, dt), 5, cuda)
+    q, k, v = (x.detach().clone().requires_grad_() for x in (q, k, v))
+    packed_attention(q, k, v, PackedLayout(lens, device=cuda), scale=1.0, causal=causal).backward(do)
+    u = torch.finfo(dt).eps / 2
+    q64, k64, v64, do64 = (x.detach().cpu().double() for x in (q, k, v, do))
+    k64, v64 = (x.repeat_interleave(hq // hk, 1) for x in (k64, v64))
+    at = 0
+    for n in lens:
+        Q, K, V, D = (x[at:at + n].transpose(0, 1) for x in (q64, k64, v64, do64))
+        s = Q @ K.transpose(1, 2)
+        assert float(s.abs().max()) * 1.4427 < 128
+        if causal:
+            s = s.masked_fill(torch.ones(n, n, dtype=torch.bool).triu(1), -math.inf)
+        p, dp = torch.softmax(s, 2), D @ V.transpose(1, 2)
+        ds = p * (dp - (p * dp).sum(2, keepdim=True))
+        off = u * ds.abs() + 2.0 ** -16 * p * (dp.abs() + (p * dp.abs()).sum(2, keepdim=True))
+        want = (ds @ K).transpose(0, 1)
+        _within(q.grad[at:at + n], want, (off @ K.abs()).transpose(0, 1) * 1.01 + u * want.abs() + 1e-7, "dq of %d tokens" % n)
+        at += n
+
+
 @pytest.mark.parametrize("size", [2.0 ** -12, 2.0 ** 9])
 def test_small_and_large_f16_gradients(cuda, size):
     """f16 holds neither ds of a long row with small gradients nor that of large ones by itself."""
