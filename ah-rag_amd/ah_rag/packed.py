@@ -17,7 +17,8 @@ longest costs both the padded tokens' projections and the square of the padded l
 Everything runs in libahr_hip.so (include/ahr.h); there is no CPU fallback. Calls are enqueued on the
 current stream of the tensors' device (or `stream`), synchronise nothing and may be captured into a
 hipGraph once a layout has served a call of the same shape (its work lists are copied to the device
-then). Tensors that the kernels cannot read in place (rows that do not start at multiples of 16
+then; a captured backward pass also needs leaves without a living graph from outside the capture, whose
+gradients torch accumulates on the stream of that graph). Tensors that the kernels cannot read in place (rows that do not start at multiples of 16
 bytes, a strided last dimension) are copied first.
 
 Replaces, behind the reference's SentenceTransformer.encode seam
@@ -53,7 +54,9 @@ def _host_lengths(x: Lengths, what: str) -> np.ndarray:
         raise ValueError(f"{what} must be a list of whole numbers")
     if a.size and (a.min() < 0 or int(a.sum(dtype=np.int64)) > 1 << 30):
         raise ValueError(f"{what} must be >= 0 and sum to at most 2**30")
-    return np.array(a, dtype=np.int32)  # (a copy: the layout's own)
+    own = np.array(a, dtype=np.int32)  # (a copy, and read-only: the work lists are made from it once)
+    own.setflags(write=False)
+    return own
 
 
 class PackedLayout:
@@ -322,6 +325,8 @@ def _check_out(out: Optional[torch.Tensor], q: torch.Tensor) -> None:
         return
     if out.shape != q.shape or out.dtype != q.dtype or out.device != q.device:
         raise ValueError("out must have q's shape, dtype and device")
+    if any(n > 1 and st == 0 for n, st in zip(out.shape, out.stride())):
+        raise ValueError("out must not be expanded")
     if _aligned(out) is not out:
         raise ValueError("out's rows must be contiguous and start at multiples of 16 bytes")
 
@@ -490,6 +495,8 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: Optional[torch.Tens
         raise ValueError("positions must be int32 or int64 [tokens]")
     if not 0 <= eps < 3e38:
         raise ValueError("eps must be finite and not negative")
+    if torch.is_grad_enabled() and (cos.requires_grad or sin.requires_grad):
+        raise ValueError("the table has no gradient")
     device = q.device
     if device.type != "cuda":
         raise nat.NativeLibraryError("qk_norm_rope needs tensors on a ROCm GPU")

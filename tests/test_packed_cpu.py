@@ -257,6 +257,16 @@ def test_call_refusals():
         rotary_table(3, 7)
 
 
+def test_a_table_that_wants_a_gradient_is_refused():
+    import torch
+    from ah_rag.packed import qk_norm_rope
+    x, pos = torch.zeros(3, 2, 8), torch.zeros(3, dtype=torch.int32)
+    cos, sin = torch.ones(4, 4), torch.zeros(4, 4)
+    for pair in ((cos.clone().requires_grad_(), sin), (cos, sin.clone().requires_grad_())):
+        with pytest.raises(ValueError, match="no gradient"):
+            qk_norm_rope(x, x, None, None, *pair, pos)
+
+
 def test_rotary_table_is_exact_far_out():
     import math
     from ah_rag.packed import rotary_table

@@ -537,6 +537,10 @@ def test_gpu_refusals(cuda):
         packed_attention(x, x, x, lay, out=torch.empty_like(x).half())
     with pytest.raises(ValueError, match="out's rows"):
         packed_attention(x, x, x, lay, out=torch.empty(4, 2, 65, dtype=BF, device=cuda)[..., 1:])
+    with pytest.raises(ValueError, match="expanded"):
+        packed_attention(x, x, x, lay, out=torch.empty(1, 2, 64, dtype=BF, device=cuda).expand(4, 2, 64))
+    with pytest.raises(ValueError, match="read-only"):
+        lay.lengths[0] = 3
     for s in (0.0, -1.0, math.inf, math.nan):
         with pytest.raises(ValueError, match="scale"):
             packed_attention(x, x, x, lay, scale=s)
