@@ -181,8 +181,8 @@ class TorchEncoder:
 
     def embed(self, texts: Sequence[str], normalize_embeddings: bool = False) -> torch.Tensor:
         """Device float32 [n, d] of one packed batch with gradients to the model's parameters: the forward of a
-        fine-tuning step (packed encoders). The caller enables the parameters' gradients, takes the loss
-        and the optimizer's step, and calls packed.refresh() before encoding with the new weights."""
+        fine-tuning step (packed encoders). The caller enables the parameters' gradients and takes the loss
+        and the optimizer's step."""
         if self.packed is None:
             raise ValueError("embed() needs a packed encoder: TorchEncoder(..., packed=True)")
         with torch.cuda.device(self.device):

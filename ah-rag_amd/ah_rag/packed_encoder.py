@@ -43,6 +43,12 @@ def _get(cfg, *names, default=None):
     return default
 
 
+_POST = ("attention.self.query", "attention.self.key", "attention.self.value", "attention.output.dense", "attention.output.LayerNorm",
+         "intermediate.dense", "output.dense", "output.LayerNorm")
+_CAUSAL = ("self_attn.q_proj", "self_attn.k_proj", "self_attn.v_proj", "self_attn.o_proj", "mlp.gate_proj", "mlp.up_proj", "mlp.down_proj")
+_CAUSAL_NORMS = ("self_attn.q_norm", "self_attn.k_norm", "input_layernorm", "post_attention_layernorm")
+
+
 class PackedTransformer:
     """Weights are the model's own tensors (parameters receive gradients); `model` stays referenced."""
 
@@ -58,6 +64,12 @@ class PackedTransformer:
             self.kind = "post"
             self.kv_heads, self.head_dim = self.heads, self.hidden // self.heads
             self.eps = float(cfg.layer_norm_eps)
+            known = ["embeddings.%s_embeddings.weight" % n for n in ("word", "position", "token_type")]
+            known += ["embeddings.LayerNorm.weight", "embeddings.LayerNorm.bias"]
+            known += ["encoder.layer.%d.%s.%s" % (i, n, t) for i in range(self.layers) for n in _POST for t in ("weight", "bias")]
+            self._names(known, optional=("embeddings.token_type_embeddings.weight",), unused="pooler.")
+            if _get(cfg, "is_decoder", default=False):
+                raise UnsupportedLayoutError("packed forward: a decoder's masks")
             if _get(cfg, "position_embedding_type", default="absolute") != "absolute":
                 raise UnsupportedLayoutError("packed forward: positions other than absolute ones")
             if "encoder.relative_attention_bias.weight" in w or _get(cfg, "model_type") in ("roberta", "xlm-roberta", "mpnet"):
@@ -69,6 +81,17 @@ class PackedTransformer:
             self.kv_heads = int(_get(cfg, "num_key_value_heads", default=self.heads))
             self.head_dim = int(_get(cfg, "head_dim", default=self.hidden // self.heads))
             self.eps = float(cfg.rms_norm_eps)
+            known = ["embed_tokens.weight", "norm.weight"]
+            known += ["layers.%d.%s.weight" % (i, n) for i in range(self.layers) for n in _CAUSAL + _CAUSAL_NORMS]
+            biases = ["layers.%d.%s.bias" % (i, n) for i in range(self.layers) for n in _CAUSAL]
+            self._names(known + biases, optional=biases)
+            # (settings that change the forward without a parameter of their own)
+            if any(_get(cfg, n, default=1.0) != 1.0 for n in ("embedding_multiplier", "residual_multiplier", "attention_multiplier")):
+                raise UnsupportedLayoutError("packed forward: scaled embeddings, residuals or scores")
+            if (_get(cfg, "attn_logit_softcapping") is not None or _get(cfg, "is_causal", default=True) is False
+                    or _get(cfg, "use_bidirectional_attention", default=False)
+                    or any(t != "full_attention" for t in _get(cfg, "layer_types", default=()))):
+                raise UnsupportedLayoutError("packed forward: attention other than causal softmax over all earlier tokens")
             if w["layers.0.self_attn.q_norm.weight"].shape != (self.head_dim,):
                 raise UnsupportedLayoutError("packed forward: the query norm is not one of single heads")
             if _get(cfg, "use_sliding_window", default=False) and _get(cfg, "sliding_window") is not None:
@@ -87,7 +110,14 @@ class PackedTransformer:
             raise UnsupportedLayoutError(f"packed forward: weights in float16 or bfloat16, got {p.dtype}")
         if self.head_dim % 8 or self.head_dim > 128 or self.heads % self.kv_heads:
             raise UnsupportedLayoutError(f"packed forward: {self.heads}/{self.kv_heads} heads of {self.head_dim}")
-        self._joint: Dict[int, Tuple[torch.Tensor, Optional[torch.Tensor]]] = {}
+        self._joint: Dict[int, Tuple[tuple, torch.Tensor, Optional[torch.Tensor]]] = {}
+
+    def _names(self, known: Sequence[str], optional: Sequence[str] = (), unused: Optional[str] = None) -> None:
+        """Every parameter of the model takes part in the forward here, and none is missing."""
+        more = sorted(n for n in self.w if n not in set(known) and not (unused and n.startswith(unused)))
+        less = sorted(set(known) - set(optional) - set(self.w))
+        if more or less:
+            raise UnsupportedLayoutError(f"packed forward: {'unknown' if more else 'no'} parameter {(more or less)[0]!r}")
 
     @staticmethod
     def _activation(name: str):
@@ -108,15 +138,19 @@ class PackedTransformer:
         d = self.head_dim
         if torch.is_grad_enabled() and any(t.requires_grad for t in ws):
             return tuple(F.linear(x, a, b).view(x.shape[0], -1, d) for a, b in zip(ws, bs))
+        if len({b is None for b in bs}) != 1:
+            bs = [torch.zeros_like(a[:, 0]) if b is None else b for a, b in zip(ws, bs)]
+        state = tuple(0 if t.is_inference() else t._version for t in (*ws, *bs) if t is not None)  # (counts writes to a tensor)
         joint = self._joint.get(i)
-        if joint is None:
+        if joint is None or joint[0] != state:
             with torch.inference_mode(False):
-                joint = self._joint[i] = (torch.cat([a.detach() for a in ws]), None if bs[0] is None else torch.cat([b.detach() for b in bs]))
-        y = F.linear(x, *joint).view(x.shape[0], -1, d)
+                joint = self._joint[i] = (state, torch.cat([a.detach() for a in ws]), None if bs[0] is None else torch.cat([b.detach() for b in bs]))
+        y = F.linear(x, joint[1], joint[2]).view(x.shape[0], -1, d)
         return y[:, :self.heads], y[:, self.heads:self.heads + self.kv_heads], y[:, self.heads + self.kv_heads:]
 
     def refresh(self) -> None:
-        """After the model's weights have changed: drops the joint projections made from them."""
+        """Drops the joint projections made from the model's weights. Writes to a weight are noticed without it; writes
+        through `.data` are not."""
         self._joint.clear()
 
     def _lin(self, name: str, x: torch.Tensor) -> torch.Tensor:
@@ -168,13 +202,26 @@ class PackedTransformer:
 
     # ---- batches -------------------------------------------------------------------------------
 
-    def _tokens(self, ids: Sequence[Sequence[int]]) -> Tuple[torch.Tensor, PackedLayout]:
-        flat = np.fromiter((t for s in ids for t in s), np.int64, sum(len(s) for s in ids))
-        return torch.from_numpy(flat).to(self.device), PackedLayout([len(s) for s in ids], device=self.device)
+    def _flat(self, ids: Sequence[Sequence[int]]) -> Tuple[np.ndarray, np.ndarray]:
+        """Token ids behind each other, and the lengths; indexes past a table, which on the device would be a fault, are
+        refused here."""
+        lens = np.fromiter((len(s) for s in ids), np.int64, len(ids))
+        flat = np.fromiter((t for s in ids for t in s), np.int64, int(lens.sum()))
+        table = self.w["embeddings.word_embeddings.weight" if self.kind == "post" else "embed_tokens.weight"]
+        if flat.size and (flat.min() < 0 or flat.max() >= table.shape[0]):
+            raise ValueError(f"token ids must lie in [0, {table.shape[0]})")
+        if self.kind == "post" and lens.size:
+            most = self.w["embeddings.position_embeddings.weight"].shape[0]
+            if lens.max() > most:
+                raise ValueError(f"a sequence is longer than the model's {most} positions")
+        return flat, lens
+
+    def _tokens(self, flat: np.ndarray, lens: np.ndarray) -> Tuple[torch.Tensor, PackedLayout]:
+        return torch.from_numpy(flat).to(self.device), PackedLayout(lens, device=self.device)
 
     def hidden_states(self, ids: Sequence[Sequence[int]]) -> Tuple[torch.Tensor, PackedLayout]:
         """Last hidden states [tokens, hidden] of token id sequences, and their layout."""
-        tok, layout = self._tokens(ids)
+        tok, layout = self._tokens(*self._flat(ids))
         return (self._post if self.kind == "post" else self._causal)(tok, layout), layout
 
     def pooled(self, ids: Sequence[Sequence[int]], normalize: bool) -> torch.Tensor:
@@ -183,10 +230,11 @@ class PackedTransformer:
         if share < SHARE_FROM:
             h, layout = self.hidden_states(ids)
             return packed_mean_pool(h, layout, normalize=normalize)
+        first, rest = self._flat([ids[0][:share]]), self._flat([s[share:] for s in ids])
         kept: List[tuple] = []
-        tok, layout = self._tokens([ids[0][:share]])
+        tok, layout = self._tokens(*first)
         head = self._causal(tok, layout, keep=kept).float().sum(0)
-        tok, layout = self._tokens([s[share:] for s in ids])
+        tok, layout = self._tokens(*rest)
         mean = packed_mean_pool(self._causal(tok, layout, share, kept), layout)
         n = torch.tensor([len(s) for s in ids], dtype=torch.float32, device=self.device)[:, None]
         y = (mean * (n - share) + head) / n

@@ -112,6 +112,51 @@ def test_unknown_layouts_are_refused():
             PackedTransformer(m, dev)
 
 
+def post(hidden=64, heads=2, layers=2, vocab=50, positions=20, dtype=torch.bfloat16, more=(), **cfg):
+    """Parameters of the bidirectional layout; `more`: further ones, name -> shape."""
+    names = ("attention.self.query", "attention.self.key", "attention.self.value", "attention.output.dense", "attention.output.LayerNorm",
+             "intermediate.dense", "output.dense", "output.LayerNorm")
+    s = {"embeddings.word_embeddings.weight": (vocab, hidden), "embeddings.position_embeddings.weight": (positions, hidden),
+         "embeddings.LayerNorm.weight": (hidden,), "embeddings.LayerNorm.bias": (hidden,)}
+    for i in range(layers):
+        for n in names:
+            shape = (hidden,) if "Norm" in n else (hidden, hidden)
+            s.update({f"encoder.layer.{i}.{n}.weight": shape, f"encoder.layer.{i}.{n}.bias": (hidden,)})
+    s.update(more)
+    return Weights(dict(num_attention_heads=heads, num_hidden_layers=layers, hidden_size=hidden, layer_norm_eps=1e-12, hidden_act="gelu", **cfg),
+                   s, 4, dtype)
+
+
+def test_parameters_and_settings_that_the_forward_does_not_have_are_refused():
+    from ah_rag.packed_encoder import PackedTransformer, UnsupportedLayoutError
+    dev = torch.device("cuda", 0)
+    PackedTransformer(post(), dev)
+    PackedTransformer(post(more={"pooler.dense.weight": (64, 64), "embeddings.token_type_embeddings.weight": (2, 64)}), dev)
+    PackedTransformer(causal(layer_types=["full_attention"] * 2, residual_multiplier=1.0), dev)
+    bad = [post(more={"embeddings_project.weight": (64, 64)}), post(more={"encoder.layer.0.crossattention.self.query.weight": (64, 64)}),
+           post(layers=1, more={"encoder.layer.1.output.dense.weight": (64, 64)}), post(is_decoder=True), post(position_embedding_type="relative_key"),
+           causal(layer_types=["full_attention", "sliding_attention"]), causal(residual_multiplier=0.2), causal(attn_logit_softcapping=30.0),
+           causal(is_causal=False), causal(use_bidirectional_attention=True)]
+    m = causal()
+    m.layers._modules["1"].register_parameter("layer_scale", torch.nn.Parameter(torch.ones(3, dtype=torch.bfloat16)))
+    bad.append(m)
+    m = causal()
+    del m.layers._modules["1"]._modules["input_layernorm"]
+    bad.append(m)
+    for m in bad:
+        with pytest.raises(UnsupportedLayoutError):
+            PackedTransformer(m, dev)
+
+
+def test_ids_and_lengths_past_the_tables_are_refused():
+    from ah_rag.packed_encoder import PackedTransformer
+    dev = torch.device("cuda", 0)
+    for m, ids in ((causal(), [[3, 500]]), (causal(), [[3], [-1, 2]]), (post(), [[50]]), (post(), [[1] * 21, [2]]),
+                   (causal(), [[7] * 30 + [1], [7] * 30 + [900]])):
+        with torch.inference_mode(), pytest.raises(ValueError, match="must lie|longer"):
+            PackedTransformer(m, dev).pooled(ids, False)
+
+
 # ---- on the GPU --------------------------------------------------------------------------------
 
 
@@ -208,6 +253,29 @@ def test_gradients_of_a_training_step(cuda):
     with torch.inference_mode():
         after = t.pooled(ids, False)
     assert _off(after, causal64(m, ids, w64)) < 16 * ref.half_step(torch.bfloat16) and not torch.equal(after, before)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("make", [causal, post])
+def test_written_weights_are_noticed(cuda, make):
+    """The joint projections follow writes to the weights: an optimizer's, and a loaded state dict."""
+    from ah_rag.packed_encoder import PackedTransformer
+    m = make().to(cuda)
+    t = PackedTransformer(m, cuda)
+    ids = _ids([7, 12, 1], vocab=50)
+    old = {n: p.detach().clone() for n, p in m.named_parameters()}
+    with torch.inference_mode():
+        before = t.pooled(ids, False)
+    opt = torch.optim.SGD(m.parameters(), lr=0.5)
+    t.pooled(ids, True).square().sum(0)[:8].sum().backward()
+    opt.step()
+    with torch.inference_mode():
+        after = t.pooled(ids, False)
+        t.refresh()
+        assert torch.equal(after, t.pooled(ids, False)) and not torch.equal(after, before)
+    m.load_state_dict(old)
+    with torch.inference_mode():
+        assert torch.equal(t.pooled(ids, False), before)
 
 
 @pytest.mark.gpu
