@@ -9,8 +9,8 @@ Reference seams this module replaces (Yaron9/AH-RAG):
 The encoder stays a thin PyTorch call (north star: "not re-implemented"). sentence-transformers
 is the default, as in the reference; this image has neither the package nor weights, so a run
 here must choose another encoder explicitly (AHR_ENCODER=hash: deterministic, L2-normalised
-stand-in vectors; AHR_ENCODER=torch: the model's architecture on the GPU). Nothing falls back
-silently.
+stand-in vectors; AHR_ENCODER=torch: the model's architecture on the GPU; AHR_ENCODER=packed: the same without
+padding, on this library's attention and pooling kernels). Nothing falls back silently.
 
 DenseIndex is the device half: fp32 vectors go in, the index keeps them row-major in HBM as
 bf16 / f16 / f32 and answers batched top-k queries through libahr_hip.so. Nothing here falls

@@ -12,6 +12,16 @@
 // stay within the lane and its other half, and S^T's registers are, converted to 16 bits, exactly the
 // second operand of O^T = V^T P^T when V^T is read with its keys in accumulator order (col_frag). Keys
 // and values go through LDS by DMA, double buffered, one barrier per 64 keys.
+//
+// What bounds it. Many rows: the matrix units, whose products and the exponentials between them overlap only
+// across the two waves of a SIMD (4 causal sequences of 1.5k-8.2k tokens, 32/8 heads of 128, bf16: 1.06-1.12
+// ms, 1.0 PFLOP/s where a library product of 8192^3 reaches 1.18). Single tokens: memory (24 over 1k-33k keys
+// each, 8 key heads of 128, f16: 240 us and 7 for the join, 5.4 TB/s). Short texts lie between (256 of up to
+// 384 tokens, 12 heads of 64: 73 us, 3.3 TB/s). Few workgroups (64 queries of 4-40 tokens behind a prefix of
+// 900, 16/8 heads of 64: 27 us) wait out each tile's chain of barrier, products, exponentials, products. Three
+// tile buffers instead of two (1.45 ms for the long sequences, 27 us for the prefix), two waves that share a
+// tile's keys where an item has few rows (26 us, but 2 % more for the long ones) and an order of the
+// workgroups that spreads key heads over the XCDs (1.16 ms, 28 us) were measured and not kept.
 #include "ahr_attn_common.h"
 
 #include <algorithm>
