@@ -170,6 +170,11 @@ def _aligned(t: torch.Tensor) -> torch.Tensor:
     return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
+def _new(t: torch.Tensor) -> torch.Tensor:
+    """An uninitialised contiguous tensor of t's kind (half the host time of torch.empty with its arguments)."""
+    return torch.empty_like(t, memory_format=torch.contiguous_format)
+
+
 def _rows(t: Optional[torch.Tensor]) -> Tuple[int, int, int]:
     """A struct ahr_tensor3: address and strides of tokens and heads (of an axis of one element arbitrary)."""
     if t is None:
@@ -266,7 +271,7 @@ def _attention(q, k, v, layout, causal, scale, lse, prefix_k=None, prefix_v=None
     if prefix_k is not None:
         prefix_k, prefix_v = _aligned(prefix_k), _aligned(prefix_v)
     plan, lists = layout._plan(_CODES[q.dtype], shape[1], k.shape[1], shape[2], causal, False, 0 if prefix_k is None else prefix_k.shape[0])
-    o = torch.empty(shape, dtype=q.dtype, device=q.device) if out is None else out
+    o = _new(q) if out is None else out
     _launch_attention(_calls().attn_forward, "ahr_attn_forward", plan, lists, scale, q, k, v, prefix_k, prefix_v, o, lse, None, None, None, None)
     return o
 
@@ -275,7 +280,7 @@ class _PackedAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, layout, causal, scale):
         q, k, v = _aligned(q), _aligned(k), _aligned(v)
-        lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device)
+        lse = q.new_empty(q.shape[:2], dtype=torch.float32)
         o = _attention(q, k, v, layout, causal, scale, lse)
         # the backward pass's lists too: its first call may be inside a capture
         ctx.plan = layout._plan(_CODES[q.dtype], q.shape[1], k.shape[1], q.shape[2], causal, True, 0)
@@ -288,9 +293,7 @@ class _PackedAttention(torch.autograd.Function):
         _once()
         q, k, v, o, lse = ctx.saved_tensors
         plan, lists = ctx.plan
-        shape, kshape, dtype, device = q.shape, k.shape, q.dtype, q.device
-        dq = torch.empty(shape, dtype=dtype, device=device)
-        dk, dv = torch.empty((2, *kshape), dtype=dtype, device=device).unbind(0)
+        dq, dk, dv = _new(q), _new(k), _new(k)
         _launch_attention(_calls().attn_backward, "ahr_attn_backward", plan, lists, ctx.scale, q, k, v, None, None, _aligned(o), lse,
                           _aligned(d_o), dq, dk, dv)
         return dq, dk, dv, None, None, None
@@ -413,7 +416,7 @@ def _launch_rope(call, name, q, k, cos, sin, positions, eps, interleaved, wq, wk
 
 
 def _rope_forward(q, k, wq, wk, cos, sin, positions, eps, interleaved):
-    yq, yk = torch.empty(q.shape, dtype=q.dtype, device=q.device), torch.empty(k.shape, dtype=k.dtype, device=k.device)
+    yq, yk = _new(q), _new(k)
     _launch_rope(_calls().rope, "ahr_qk_norm_rope", q, k, cos, sin, positions, eps, interleaved, wq, wk, yq, yk)
     return yq, yk
 
@@ -442,7 +445,7 @@ class _QkNormRope(torch.autograd.Function):
         _once()
         q, k, wq, wk, cos, sin, positions = ctx.saved_tensors
         dim, device = q.shape[2], q.device
-        dq, dk = torch.empty(q.shape, dtype=q.dtype, device=device), torch.empty(k.shape, dtype=k.dtype, device=device)
+        dq, dk = _new(q), _new(k)
         dw = ws = gq = gk = None
         if wq is not None:
             n = ctypes.c_int64()
@@ -519,8 +522,8 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: Optional[torch.Tens
 def _pool_forward(rows, layout, normalize, norm):
     n_chunks, lists = layout._pool_lists()
     n, width = len(layout), rows.shape[1]
-    out = torch.empty((n, width), dtype=torch.float32, device=rows.device)
-    ws = torch.empty(max(1, n_chunks * ((width + 3) // 4 * 4)), dtype=torch.float32, device=rows.device)
+    out = rows.new_empty((n, width), dtype=torch.float32)
+    ws = rows.new_empty(max(1, n_chunks * ((width + 3) // 4 * 4)), dtype=torch.float32)
     stream = nat.stream_ptr(device_index=rows.device.index)
     nat.check(nat.lib().ahr_pool_mean(_CODES[rows.dtype], rows.data_ptr(), rows.stride(0), width, lists.data_ptr(), n_chunks, n,
                                       int(normalize), out.data_ptr(), nat.ptr(norm), ws.data_ptr(), ws.numel() * 4, stream), "ahr_pool_mean")
@@ -531,7 +534,7 @@ def _pool_forward(rows, layout, normalize, norm):
 class _PackedMeanPool(torch.autograd.Function):
     @staticmethod
     def forward(ctx, rows, layout, normalize):
-        norm = torch.empty(len(layout), dtype=torch.float32, device=rows.device)
+        norm = rows.new_empty(len(layout), dtype=torch.float32)
         out = _pool_forward(rows, layout, normalize, norm)
         ctx.save_for_backward(out, norm)
         ctx.layout, ctx.normalize, ctx.shape, ctx.dtype = layout, normalize, rows.shape, rows.dtype
@@ -544,7 +547,7 @@ class _PackedMeanPool(torch.autograd.Function):
         layout = ctx.layout
         n_chunks, lists = layout._pool_lists()
         d_out = d_out.contiguous()
-        d_rows = torch.empty(ctx.shape, dtype=ctx.dtype, device=out.device)
+        d_rows = out.new_empty(ctx.shape, dtype=ctx.dtype)
         stream = nat.stream_ptr(device_index=out.device.index)
         nat.check(nat.lib().ahr_pool_mean_backward(_CODES[ctx.dtype], d_rows.data_ptr(), ctx.shape[1], lists.data_ptr(), n_chunks,
                                                    len(layout), ctx.normalize, d_out.data_ptr(), out.data_ptr(), norm.data_ptr(), stream),
