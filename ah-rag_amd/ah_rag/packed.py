@@ -250,12 +250,8 @@ def _once() -> None:
         raise RuntimeError("the packed operators have no second derivative (backward with create_graph=True)")
 
 
-def _workspace(plan: nat.AttnPlan, device: torch.device) -> Optional[torch.Tensor]:
-    return torch.empty(plan.ws_bytes, dtype=torch.uint8, device=device) if plan.ws_bytes else None
-
-
 def _launch_attention(call, name, plan, lists, scale, q, k, v, pk, pv, o, lse, d_o, dq, dk, dv) -> None:
-    ws = _workspace(plan, q.device)
+    ws = q.new_empty(plan.ws_bytes, dtype=torch.uint8) if plan.ws_bytes else None
     stream = nat.stream_ptr(device_index=q.device.index)
     args = _ATTN_ARGS.pack(ctypes.addressof(plan), 0 if lists is None else lists.data_ptr(), scale, 0, *_rows(q), *_rows(k), *_rows(v),
                            *_rows(pk), *_rows(pv), *_rows(o), 0 if lse is None else lse.data_ptr(), *_rows(d_o), *_rows(dq), *_rows(dk),
@@ -294,7 +290,7 @@ class _PackedAttention(torch.autograd.Function):
         q, k, v, o, lse = ctx.saved_tensors
         plan, lists = ctx.plan
         dq, dk, dv = _new(q), _new(k), _new(k)
-        _launch_attention(_calls().attn_backward, "ahr_attn_backward", plan, lists, ctx.scale, q, k, v, None, None, _aligned(o), lse,
+        _launch_attention(_calls().attn_backward, "ahr_attn_backward", plan, lists, ctx.scale, q, k, v, None, None, o, lse,
                           _aligned(d_o), dq, dk, dv)
         return dq, dk, dv, None, None, None
 
