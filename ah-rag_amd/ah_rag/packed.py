@@ -29,6 +29,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
+import functools
 import struct
 from types import SimpleNamespace
 from typing import Dict, Optional, Sequence, Tuple, Union
@@ -399,16 +400,23 @@ def rotary_table(n_positions: int, dim: int, base: float = 10000.0,
         return angle.cos().float().to(device), angle.sin().float().to(device)
 
 
-def _launch_rope(call, name, q, k, cos, sin, positions, eps, interleaved, wq, wk, yq, yk, dq=None, dk=None, dw=None, ws=None) -> None:
+def _launch_rope(call, name, q, k, cos, sin, positions, eps, interleaved, wq, wk, yq, yk, dq=None, dk=None, dwq=None, dwk=None, ws=None) -> None:
     tokens, heads, dim = q.shape
     n_pos, half = cos.shape
-    dwq, dwk = (0, 0) if dw is None else (dw.data_ptr(), dw.data_ptr() + 4 * dim)
     args = _ROPE_ARGS.pack(_CODES[q.dtype], heads, k.shape[1], dim, 2 * half, interleaved, tokens, n_pos, eps, 0, *_rows(q), *_rows(k),
                            *_rows(yq), *_rows(yk), *_rows(dq), *_rows(dk), 0 if wq is None else wq.data_ptr(),
-                           0 if wk is None else wk.data_ptr(), cos.data_ptr(), sin.data_ptr(), positions.data_ptr(), dwq, dwk,
+                           0 if wk is None else wk.data_ptr(), cos.data_ptr(), sin.data_ptr(), positions.data_ptr(),
+                           0 if dwq is None else dwq.data_ptr(), 0 if dwk is None else dwk.data_ptr(),
                            0 if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel())
     if call(args, nat.stream_ptr(device_index=q.device.index)):
         nat.check(-1, name)
+
+
+@functools.lru_cache(maxsize=64)
+def _rope_ws(tokens: int, dim: int) -> int:
+    n = ctypes.c_int64()
+    nat.check(nat.lib().ahr_rope_ws_bytes(tokens, dim, ctypes.byref(n)), "ahr_rope_ws_bytes")
+    return n.value
 
 
 def _rope_forward(q, k, wq, wk, cos, sin, positions, eps, interleaved):
@@ -440,18 +448,14 @@ class _QkNormRope(torch.autograd.Function):
     def backward(ctx, dyq, dyk):
         _once()
         q, k, wq, wk, cos, sin, positions = ctx.saved_tensors
-        dim, device = q.shape[2], q.device
         dq, dk = _new(q), _new(k)
-        dw = ws = gq = gk = None
+        ws = gq = gk = None
         if wq is not None:
-            n = ctypes.c_int64()
-            nat.check(nat.lib().ahr_rope_ws_bytes(q.shape[0], dim, ctypes.byref(n)), "ahr_rope_ws_bytes")
-            ws = torch.empty(n.value, dtype=torch.uint8, device=device)
-            dw = torch.empty((2, dim), dtype=torch.float32, device=device)
+            ws = q.new_empty(_rope_ws(q.shape[0], q.shape[2]), dtype=torch.uint8)
+            gq, gk = _new(wq), _new(wk)
         _launch_rope(_calls().rope_backward, "ahr_qk_norm_rope_backward", q, k, cos, sin, positions, ctx.eps, ctx.interleaved, wq, wk,
-                     _unit(dyq), _unit(dyk), dq, dk, dw, ws)
-        if dw is not None:
-            gq, gk = dw.unbind(0)
+                     _unit(dyq), _unit(dyk), dq, dk, gq, gk, ws)
+        if gq is not None:
             if ctx.w_dtype != (torch.float32, torch.float32):
                 gq, gk = gq.to(ctx.w_dtype[0]), gk.to(ctx.w_dtype[1])
         return dq, dk, gq, gk, None, None, None, None, None
