@@ -52,9 +52,10 @@ struct Rope {
   float eps;
 };
 
-// Vector form (rot == head_dim, a multiple of 16, aligned rows). LPR lanes share a head's row; a lane
-// owns 8 pairs of the rotation: elements a = e0 .. e0+7 and b = e0 + dim/2 .. (interleaved: 16
-// consecutive elements, pair i = (2i, 2i+1)), so the rotation needs no exchange between lanes. A
+// Vector form (rot == head_dim, a multiple of 8, aligned rows). LPR lanes share a head's row; a lane
+// owns P pairs of the rotation (8; 4 where head_dim is no multiple of 16): elements a = e0 .. e0+P-1 and
+// b = e0 + dim/2 .. (interleaved: 2 P consecutive elements, pair i = (2i, 2i+1)), so the rotation needs
+// no exchange between lanes. D is head_dim, or 0: read at run time, with LPR of any size. A
 // workgroup takes q or k, so that a lane keeps one side's weights (and one side's part of their
 // gradients: both sides' took 138 registers, three waves a SIMD, and a select for each use; 170 us
 // backward where this takes 150); a wave takes one token at a time and keeps the lane's cos and sin
@@ -62,13 +63,14 @@ struct Rope {
 // tokens in registers, the workgroup joins them into one partial row.
 // Bound by memory: 22.8k tokens of 32 + 8 heads of 128 in bf16 take 95 us forward (467 MB, 4.9 TB/s,
 // which is what a copy reaches) and 150 us backward (700 MB, 4.7 TB/s).
-template <typename T, int DIM, bool IL, bool BWD>
+template <typename T, int D, int P, bool IL, bool BWD>
 __global__ __launch_bounds__(256, 4) void rope_vec_kernel(Rope p) {
-  constexpr int LPR = DIM / 16;          // lanes of a row
-  constexpr int RPW = 64 / LPR;          // rows of a wave
+  const int dim = D ? D : p.dim;
+  const int LPR = dim / (2 * P), RPW = 64 / LPR;  // lanes of a row, rows of a wave (lanes past them idle)
+  const float mean = 1.f / dim;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int sub = lane / LPR, li = lane % LPR;
-  const int e0 = IL ? li * 16 : li * 8;
+  const int e0 = IL ? li * 2 * P : li * P;
   const bool normed = p.wq != nullptr, is_k = (int)blockIdx.x >= p.q_blocks;
   const int heads = is_k ? p.kv_heads : p.heads;
   const int block = is_k ? blockIdx.x - p.q_blocks : blockIdx.x, blocks = is_k ? gridDim.x - p.q_blocks : p.q_blocks;
@@ -77,61 +79,73 @@ __global__ __launch_bounds__(256, 4) void rope_vec_kernel(Rope p) {
   T* os = (T*)(is_k ? p.ok : p.oq);
   const int64_t x_ts = is_k ? p.k_ts : p.q_ts, x_hs = is_k ? p.k_hs : p.q_hs, y_ts = is_k ? p.yk_ts : p.yq_ts, y_hs = is_k ? p.yk_hs : p.yq_hs,
                 o_ts = is_k ? p.ok_ts : p.oq_ts, o_hs = is_k ? p.ok_hs : p.oq_hs;
-  float w[16], dw[16];
+  float w[2 * P], dw[2 * P];
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const int e = IL ? e0 + i : (i < 8 ? e0 + i : DIM / 2 + e0 + i - 8);
+  for (int i = 0; i < 2 * P; ++i) {
+    const int e = IL || i < P ? e0 + i : dim / 2 + e0 + i - P;
     w[i] = normed ? (is_k ? p.wk : p.wq)[e] : 1.f;
     dw[i] = 0.f;
   }
   auto load = [&](float* to, const T* row) {
     if (IL) {
-      load_f32<T, 16>(to, row + e0);
+      load_f32<T, 2 * P>(to, row + e0);
     } else {
-      load_f32<T, 8>(to, row + e0);
-      load_f32<T, 8>(to + 8, row + DIM / 2 + e0);
+      load_f32<T, P>(to, row + e0);
+      load_f32<T, P>(to + P, row + dim / 2 + e0);
     }
   };
-  // heads of a token are dealt to gridDim.y slices
-  for (int64_t t = (int64_t)block * 4 + wave; t < p.tokens; t += (int64_t)blocks * 4) {
-    const int64_t at = p.pos[t];
+  auto row_sum = [&](float x) {  // over the row's lanes, the same in all of them
+    if (D) {
+#pragma unroll
+      for (int m = 1; m < 64; m *= 2)
+        if (m < LPR) x += __shfl_xor(x, m, 64);
+      return x;
+    }
+    float all = 0.f;
+    for (int j = 0; j < LPR; ++j) all += __shfl(x, sub * LPR + j, 64);
+    return all;
+  };
+  // Heads of a token are dealt to gridDim.y slices; with fewer heads than rows a wave takes several tokens.
+  const int per = heads < RPW ? RPW / heads : 1;
+  const int token = per > 1 ? sub / heads : 0, head = sub - token * heads;
+  const bool on = sub < (per > 1 ? per * heads : RPW);
+  for (int64_t t0 = ((int64_t)block * 4 + wave) * per; t0 < p.tokens; t0 += (int64_t)blocks * 4 * per) {
+    const int64_t t = t0 + token;
+    const int64_t at = p.pos[t < p.tokens ? t : t0];
     const bool known = at >= 0 && at < p.n_pos;
-    float c[8], s[8];
+    float c[P], s[P];
     {
-      const int64_t o = (known ? at : 0) * (DIM / 2) + li * 8;
-      load_f32<float, 8>(c, p.cos + o);
-      load_f32<float, 8>(s, p.sin + o);
+      const int64_t o = (known ? at : 0) * (dim / 2) + li * P;
+      load_f32<float, P>(c, p.cos + o);
+      load_f32<float, P>(s, p.sin + o);
       if (!known) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) c[i] = s[i] = NAN;
+        for (int i = 0; i < P; ++i) c[i] = s[i] = NAN;
       }
     }
     for (int h0 = blockIdx.y * RPW; h0 < heads; h0 += gridDim.y * RPW) {
-      const int hd = h0 + sub;
-      const bool have = hd < heads;
-      float x[16], y[16];
+      const int hd = h0 + head;
+      const bool have = on && t < p.tokens && hd < heads;
+      float x[2 * P], y[2 * P];
       if (have) {
         load(x, xs + t * x_ts + hd * x_hs);
         if (BWD) load(y, ys + t * y_ts + hd * y_hs);
       } else {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) x[i] = y[i] = 0.f;
+        for (int i = 0; i < 2 * P; ++i) x[i] = y[i] = 0.f;
       }
       float r = 1.f;
       if (normed) {
         float sum = 0.f;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) sum = fmaf(x[i], x[i], sum);
-#pragma unroll
-        for (int m = 1; m < 64; m *= 2)
-          if (m < LPR) sum += __shfl_xor(sum, m, 64);
-        r = 1.f / sqrtf(sum * (1.f / DIM) + p.eps);
+        for (int i = 0; i < 2 * P; ++i) sum = fmaf(x[i], x[i], sum);
+        r = 1.f / sqrtf(row_sum(sum) * mean + p.eps);
       }
-      float o[16];
+      float o[2 * P];
       if (!BWD) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int a = IL ? 2 * i : i, b = IL ? 2 * i + 1 : i + 8;
+        for (int i = 0; i < P; ++i) {
+          const int a = IL ? 2 * i : i, b = IL ? 2 * i + 1 : i + P;
           const float na = x[a] * r * w[a], nb = x[b] * r * w[b];
           o[a] = na * c[i] - nb * s[i];
           o[b] = nb * c[i] + na * s[i];
@@ -140,8 +154,8 @@ __global__ __launch_bounds__(256, 4) void rope_vec_kernel(Rope p) {
         // dn = R^T dy; dw += dn x r; dx = r (dn w - x r^2 mean(dn w x))
         float dot = 0.f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const int a = IL ? 2 * i : i, b = IL ? 2 * i + 1 : i + 8;
+        for (int i = 0; i < P; ++i) {
+          const int a = IL ? 2 * i : i, b = IL ? 2 * i + 1 : i + P;
           float da = y[a] * c[i] + y[b] * s[i], db = y[b] * c[i] - y[a] * s[i];
           // (idle rows hold zeros; an unknown position's NaN belongs to rows that exist)
           if (have) {
@@ -155,42 +169,42 @@ __global__ __launch_bounds__(256, 4) void rope_vec_kernel(Rope p) {
           o[b] = db;
         }
         if (normed) {
+          const float f = row_sum(dot) * mean * r * r;
 #pragma unroll
-          for (int m = 1; m < 64; m *= 2)
-            if (m < LPR) dot += __shfl_xor(dot, m, 64);
-          const float f = dot * (1.f / DIM) * r * r;
-#pragma unroll
-          for (int i = 0; i < 16; ++i) o[i] = r * (o[i] - x[i] * f);
+          for (int i = 0; i < 2 * P; ++i) o[i] = r * (o[i] - x[i] * f);
         }
       }
       if (have) {
         T* op = os + t * o_ts + hd * o_hs;
         if (IL) {
-          store_f32<T, 16>(op + e0, o);
+          store_f32<T, 2 * P>(op + e0, o);
         } else {
-          store_f32<T, 8>(op + e0, o);
-          store_f32<T, 8>(op + DIM / 2 + e0, o + 8);
+          store_f32<T, P>(op + e0, o);
+          store_f32<T, P>(op + dim / 2 + e0, o + P);
         }
       }
     }
   }
   if (BWD && normed) {
     // the rows of a wave, then the four waves, in a fixed order
-    __shared__ float acc[4][RPW][DIM];
+    __shared__ float acc[4][64 * 2 * P];
+    if (sub < RPW) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) acc[wave][sub][IL ? e0 + i : (i < 8 ? e0 + i : DIM / 2 + e0 + i - 8)] = dw[i];
+      for (int i = 0; i < 2 * P; ++i) acc[wave][sub * dim + (IL || i < P ? e0 + i : dim / 2 + e0 + i - P)] = dw[i];
+    }
     __syncthreads();
-    for (int e = threadIdx.x; e < DIM; e += 256) {
+    for (int e = threadIdx.x; e < dim; e += 256) {
       float sum = 0.f;
       for (int a = 0; a < 4; ++a)
-        for (int b = 0; b < RPW; ++b) sum += acc[a][b][e];
+        for (int b = 0; b < RPW; ++b) sum += acc[a][b * dim + e];
       const int row = (is_k ? p.q_blocks * gridDim.y : 0) + blockIdx.y * blocks + block;
-      p.part[(int64_t)row * DIM + e] = sum;
+      p.part[(int64_t)row * dim + e] = sum;
     }
   }
 }
 
-// General form: any even head_dim up to 512, any even rot <= head_dim, any alignment; one wave per
+// General form: any even head_dim up to 512, any even rot <= head_dim, any alignment (925 us where the vector form
+// takes VECUS: 20 + 4 heads of 80, NTOK tokens in bf16, both passes); one wave per
 // head row at a time, element e of a row in lane e % 64. Rotation partners are read from memory again.
 template <typename T, bool BWD>
 __global__ __launch_bounds__(256) void rope_any_kernel(Rope p, int il) {
@@ -327,7 +341,7 @@ template <typename T, bool BWD>
 static int rope_launch(const ahr_rope_args* a, Rope p, hipStream_t s) {
   const ahr_tensor3* t[6] = {&a->q, &a->yq, &a->dq, &a->k, &a->yk, &a->dk};
   const int al = 16 / (int)sizeof(T);
-  bool vec = a->rot == a->head_dim;
+  bool vec = a->rot == a->head_dim && a->head_dim % 8 == 0;
   for (int i = 0; i < 6; ++i) {
     if ((i < 3 ? a->heads : a->kv_heads) == 0 || (i % 3 == 2 && !BWD)) continue;
     vec = vec && reinterpret_cast<uintptr_t>(t[i]->p) % 16 == 0 && t[i]->ts % al == 0 && t[i]->hs % al == 0;
@@ -336,27 +350,32 @@ static int rope_launch(const ahr_rope_args* a, Rope p, hipStream_t s) {
   const int all = a->heads + a->kv_heads;
   int part_q = 0, part_k = 0;
   const int il = a->interleaved;
-#define AHR_ROPE(D)                                                                                     \
+#define AHR_ROPE(D, P)                                                                                  \
   {                                                                                                     \
-    const int rpw = 64 / (D / 16), rounds = (std::max(a->heads, a->kv_heads) + rpw - 1) / rpw;          \
-    const int64_t want = (a->tokens + 3) / 4;                                                           \
+    const int rpw = 64 / (a->head_dim / (2 * P)), rounds = (std::max(a->heads, a->kv_heads) + rpw - 1) / rpw; \
+    auto want = [&](int heads) {                                                                        \
+      const int64_t per = 4 * (heads > 0 && heads < rpw ? rpw / heads : 1);                             \
+      return (a->tokens + per - 1) / per;                                                               \
+    };                                                                                                  \
     /* few tokens: a token's heads are spread over more waves, for latency */                           \
     int gy = 1;                                                                                         \
-    while (gy < rounds && want * gy < 512) gy *= 2;                                                     \
+    while (gy < rounds && (a->tokens + 3) / 4 * gy < 512) gy *= 2;                                                   \
     /* backward: one round of resident workgroups, dealt to q and k as the heads are */                 \
     const int most = BWD ? kRopeBlocks / gy : 65536;                                                    \
     const int k_most = BWD ? std::max(1, (int)((int64_t)most * a->kv_heads / all)) : most;              \
-    const int bq = a->heads ? (int)std::min<int64_t>(want, BWD ? std::max(1, most - k_most) : most) : 0; \
-    const int bk = a->kv_heads ? (int)std::min<int64_t>(want, k_most) : 0;                              \
+    const int bq = a->heads ? (int)std::min<int64_t>(want(a->heads), BWD ? std::max(1, most - k_most) : most) : 0; \
+    const int bk = a->kv_heads ? (int)std::min<int64_t>(want(a->kv_heads), k_most) : 0;                 \
     p.q_blocks = bq;                                                                                    \
     part_q = bq * gy, part_k = bk * gy;                                                                 \
-    if (il) rope_vec_kernel<T, D, true, BWD><<<dim3(bq + bk, gy), 256, 0, s>>>(p);                      \
-    else rope_vec_kernel<T, D, false, BWD><<<dim3(bq + bk, gy), 256, 0, s>>>(p);                        \
+    if (il) rope_vec_kernel<T, D, P, true, BWD><<<dim3(bq + bk, gy), 256, 0, s>>>(p);                      \
+    else rope_vec_kernel<T, D, P, false, BWD><<<dim3(bq + bk, gy), 256, 0, s>>>(p);                        \
   }
-  if (vec && a->head_dim == 32) AHR_ROPE(32)
-  else if (vec && a->head_dim == 64) AHR_ROPE(64)
-  else if (vec && a->head_dim == 128) AHR_ROPE(128)
-  else if (vec && a->head_dim == 256) AHR_ROPE(256)
+  if (vec && a->head_dim == 32) AHR_ROPE(32, 8)
+  else if (vec && a->head_dim == 64) AHR_ROPE(64, 8)
+  else if (vec && a->head_dim == 128) AHR_ROPE(128, 8)
+  else if (vec && a->head_dim == 256) AHR_ROPE(256, 8)
+  else if (vec && a->head_dim % 16 == 0) AHR_ROPE(0, 8)
+  else if (vec) AHR_ROPE(0, 4)
   else {
     const int blocks = (int)std::min<int64_t>((a->tokens * all + 3) / 4, BWD ? kRopeBlocks : 65536);
     part_q = part_k = blocks;

@@ -557,6 +557,10 @@ ROPE = [
     (33, 4, 2, 64, 64, True, HF), (40, 5, 3, 256, 256, False, HF), (600, 2, 1, 128, 128, True, torch.float32),
     (19, 6, 2, 96, 96, False, BF), (19, 2, 2, 80, 40, False, HF), (19, 2, 1, 80, 40, True, BF), (9, 3, 2, 6, 4, True, torch.float32),
     (5, 2, 1, 512, 512, False, BF), (2100, 3, 1, 64, 64, False, BF),
+    # rows that do not divide a wave, and heads whose halves are no multiples of 8
+    (50, 8, 1, 48, 48, False, HF), (33, 13, 5, 80, 80, True, BF), (700, 20, 4, 80, 80, False, BF), (21, 11, 10, 112, 112, False, torch.float32),
+    (9, 7, 7, 160, 160, True, HF), (40, 5, 3, 40, 40, False, BF), (40, 23, 2, 24, 24, True, HF), (65, 70, 9, 8, 8, False, BF),
+    (17, 3, 3, 104, 104, False, torch.float32), (3, 2, 1, 504, 504, True, BF), (5, 3, 2, 480, 480, False, HF),
 ]
 
 
