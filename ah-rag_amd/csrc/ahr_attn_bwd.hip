@@ -163,10 +163,12 @@ __device__ __forceinline__ void key_stage(char* __restrict__ nxt, const Stager<D
   const __amdgpu_buffer_rsrc_t dr =
       dense::tile_rsrc_u(p.d_o + (at * p.do_ts + (int64_t)hk * G * p.do_hs) * 2, span * ots + (G - 1) * ohs + p.dim * 2);
   constexpr int step = Stager<DP / 8, kWaves, kStageRows>::kStep;
-  if (DP != 96 && p.dim == DP && have == kStageRows && step % G == 0) {  // whole tokens a step, so g0 = 0
+  if (DP != 96 && have == kStageRows && step % G == 0) {  // whole tokens a step, so g0 = 0
     const int tk = (stager.row0 * w.ginv) >> 16, g = stager.row0 - tk * G;
-    stager.load_full(qr, nxt, __mul24(tk, qts) + g * qhs, step / G * qts);
-    stager.load_full(dr, nxt + Cfg::kTile, __mul24(tk, ots) + g * ohs, step / G * ots);
+    if (p.dim == DP || stager.c0 * 8 < p.dim) {
+      stager.load_full(qr, nxt, __mul24(tk, qts) + g * qhs, step / G * qts);
+      stager.load_full(dr, nxt + Cfg::kTile, __mul24(tk, ots) + g * ohs, step / G * ots);
+    }
   } else {
     auto off = [&](int r, int ts, int hs) {
       const int x = g0 + min(r, have - 1);

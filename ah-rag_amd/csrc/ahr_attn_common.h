@@ -159,7 +159,7 @@ struct Stager {
     row0 = (w * 64 + l) / NC;
     c0 = ((w * 64 + l) % NC) ^ swz<NC>(row0);
   }
-  // a whole tile of NC * 8 = dim elements: row r lies at row_off (of row0) + (r - row0) / kStep * step
+  // a whole tile of rows (of lanes whose chunk lies within dim): row r lies at row_off (of row0) + (r - row0) / kStep * step
   __device__ __forceinline__ void load_full(__amdgpu_buffer_rsrc_t r, char* tile, int row_off, int step) const {
     const uint32_t v = (uint32_t)(row_off + c0 * 16);
 #pragma unroll
@@ -185,10 +185,12 @@ __device__ __forceinline__ void stage_kv(char* __restrict__ nxt, const Stager<DP
   const int kst = (int)kts * 2, vst = (int)vts * 2;
   const __amdgpu_buffer_rsrc_t kr = dense::tile_rsrc_u(k, (uint32_t)((have - 1) * kst + dim * 2));
   const __amdgpu_buffer_rsrc_t vr = dense::tile_rsrc_u(v, (uint32_t)((have - 1) * vst + dim * 2));
-  if (DP != 96 && dim == DP && have == kKeys) {
+  if (DP != 96 && have == kKeys) {
     constexpr int step = Stager<DP / 8, kWaves, kKeys>::kStep;
-    stager.load_full(kr, nxt, __mul24(stager.row0, kst), step * kst);
-    stager.load_full(vr, nxt + kKeys * DP * 2, __mul24(stager.row0, vst), step * vst);
+    if (dim == DP || stager.c0 * 8 < dim) {  // (chunks past dim: left alone)
+      stager.load_full(kr, nxt, __mul24(stager.row0, kst), step * kst);
+      stager.load_full(vr, nxt + kKeys * DP * 2, __mul24(stager.row0, vst), step * vst);
+    }
   } else {
     stager.load(kr, nxt, dim, [&](int r) { return __mul24(min(r, have - 1), kst); });
     stager.load(vr, nxt + kKeys * DP * 2, dim, [&](int r) { return __mul24(min(r, have - 1), vst); });

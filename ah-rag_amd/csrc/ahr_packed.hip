@@ -58,8 +58,9 @@ struct Rope {
 // no exchange between lanes. D is head_dim, or 0: read at run time, with LPR of any size. A
 // workgroup takes q or k, so that a lane keeps one side's weights (and one side's part of their
 // gradients: both sides' took 138 registers, three waves a SIMD, and a select for each use; 170 us
-// backward where this takes 150); a wave keeps the lane's cos and sin for all heads of its token. BWD: dx and the weights' gradients; each lane adds its part of dw over its
-// tokens in registers, the workgroup joins them into one partial row.
+// backward where this takes 150); a wave keeps the lane's cos and sin for all heads of its token. BWD:
+// dx and the weights' gradients; each lane adds its part of dw over its tokens in registers, the
+// workgroup joins them into one partial row.
 // Bound by memory: 22.8k tokens of 32 + 8 heads of 128 in bf16 take 95 us forward (467 MB, 4.9 TB/s,
 // which is what a copy reaches) and 150 us backward (700 MB, 4.7 TB/s).
 template <typename T, int D, int P, bool IL, bool BWD>
