@@ -18,10 +18,10 @@
 // ms, 1.0 PFLOP/s where a library product of 8192^3 reaches 1.18). Single tokens: memory (24 over 1k-33k keys
 // each, 8 key heads of 128, f16: 240 us and 7 for the join, 5.4 TB/s). Short texts lie between (256 of up to
 // 384 tokens, 12 heads of 64: 73 us, 3.3 TB/s). Few workgroups (64 queries of 4-40 tokens behind a prefix of
-// 900, 16/8 heads of 64: 27 us) wait out each tile's chain of barrier, products, exponentials, products. Three
-// tile buffers instead of two (1.45 ms for the long sequences, 27 us for the prefix), two waves that share a
-// tile's keys where an item has few rows (26 us, but 2 % more for the long ones) and an order of the
-// workgroups that spreads key heads over the XCDs (1.16 ms, 28 us) were measured and not kept.
+// 700, 16/8 heads of 64: 23 us) wait out each tile's chain of barrier, products, exponentials, products. Three
+// tile buffers instead of two (1.45 ms for the long sequences, no change for the prefix), two waves that share a
+// tile's keys where an item has few rows (6 % less for the prefix, but 2 % more for the long ones) and an order of the
+// workgroups that spreads key heads over the XCDs (1.16 ms) were measured and not kept.
 #include "ahr_attn_common.h"
 
 #include <algorithm>
@@ -348,9 +348,15 @@ static void plan_rows(const std::vector<Seq>& seqs, const ahr_attn_shape& sh, in
     waves += up((int64_t)s.qlen * G, 32);
   }
   const int64_t ptiles = up(prefix, kKeys), across = up(total, per);
-  // (prefix 4000, 64 sequences of 10 tokens, 32/8 heads of 64: within 94 us, apart 49; 64 of 57 tokens,
-  // 16/8 heads, prefix 900: within 33, apart 42; equal where the waves of the former hold 1.5 times the rows)
-  const bool apart = prefix > 0 && may_split && 2 * waves > 3 * up(total * G, 32);
+  // Apart takes fewer tiles, each a little dearer for its fuller waves, and a join: its launch, a start of each
+  // tile's own keys (both in units of a key tile, 2.6 ns of the whole card; less where workgroups are few and join
+  // anyway) and the partial rows through memory. 64 sequences, 16/8 heads of 64: 22 tokens, prefix 900 / 2000 / 6000:
+  // within 29 / 53 / 136 us, apart 30 / 39 / 75; 14 tokens: 25 / 45 / 114 and 24 / 30 / 52; 32/8 heads of 128,
+  // 22 tokens: 39 / 70 / 182 and 56 / 80 / 177; 40 sequences of 20 tokens, 12 heads of 64, prefix 300 / 900: 13 / 27
+  // and 16 / 22; 30 of 8 tokens, 4/1 heads of 128, prefix 2000 / 8000: 15 / 30 and 17 / 23.
+  const double saved = ((double)tiles - 1.25 * across) * ptiles * sh.kv_heads;
+  const double join = 1000 + 2600 * std::min(1.0, (double)tiles * sh.kv_heads / 512) + (double)total * sh.heads * sh.head_dim / 1300;
+  const bool apart = prefix > 0 && may_split && saved > join;
   std::vector<RowItem> base;
   std::vector<int> load;
   for (const Seq& s : seqs)

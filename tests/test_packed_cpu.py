@@ -47,6 +47,8 @@ CASES = [
     dict(q_lens=[]),
     dict(q_lens=[4000, 300], heads=16, kv_heads=4, dim=128, causal=1),
     dict(q_lens=[3000], k_lens=[700], heads=6, kv_heads=2),
+    dict(q_lens=[2, 0, 5, 1] * 20, prefix=700, causal=1),
+    dict(q_lens=[4] * 30, k_lens=[2] * 30, prefix=2000, heads=4, kv_heads=2),
 ]
 
 
@@ -98,6 +100,18 @@ def test_row_lists_cover_every_pair_once(case):
     flat = [x for p in planes for x in p]
     assert len(flat) == len(set(flat))
     assert plan.ws_bytes == plan.planes * plan.part_rows * case.get("heads", 12) * (case.get("dim", 64) + 1) * 4
+
+
+@pytest.mark.parametrize("case,apart", [
+    (dict(q_lens=[2, 0, 5, 1] * 20, prefix=700, causal=1), True), (dict(q_lens=[4] * 30, k_lens=[2] * 30, prefix=2000, heads=4, kv_heads=2), True),
+    (dict(q_lens=[1] * 60, k_lens=[3] * 59 + [0], prefix=5000, heads=16, kv_heads=4, causal=1), True),
+    (dict(q_lens=[2, 0, 5, 1] * 20, prefix=60, causal=1), False), (dict(q_lens=[128] * 30, prefix=5000), False),
+    (dict(q_lens=[5], prefix=100000), False)])
+def test_a_prefix_is_read_apart_where_that_saves_tiles(case, apart):
+    _, rows, _, _ = _plan(**case)
+    seq_of = np.repeat(np.arange(len(case["q_lens"])), case["q_lens"])
+    across = [r for r in rows if seq_of[r["q0"]] != seq_of[r["q0"] + r["nq"] - 1]]
+    assert bool(across) == apart and all(r["ke"] == r["kb"] and r["pe"] > r["pb"] for r in across)
 
 
 @pytest.mark.parametrize("case", [c for c in CASES if "prefix" not in c])

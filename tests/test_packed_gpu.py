@@ -96,6 +96,10 @@ def test_attention_and_gradients(cuda, shape):
     (([40, 3], [20, 0], 2, 1, 40, True, BF), 100),
     (([40, 3], [20, 0], 2, 1, 64, False, BF), 0),
     (([2, 2], None, 3, 1, 80, False, HF), 4000),
+    (([3] * 40, None, 8, 4, 64, True, BF), 1300),
+    (([2, 0, 5, 1] * 20, None, 12, 12, 40, True, HF), 700),
+    (([4] * 30, [2] * 30, 4, 2, 64, False, BF), 2000),   # rows that read the prefix alone, and keys short of the queries
+    (([4] * 30, [2] * 30, 4, 2, 64, True, BF), 2000),
 ], ids=lambda x: _ids(x) if isinstance(x, tuple) else "prefix%d" % x)
 def test_prefix_attention(cuda, shape, prefix):
     from ah_rag.packed import PackedLayout, prefix_attention
