@@ -13,8 +13,6 @@ A packed batch holds the tokens of all its sequences behind each other, with no 
 `own` False: elementary torch operations in 32 bits on padded batches. `own` True: the framework's calls.
 """
 import math
-import os
-import sys
 
 import torch
 
@@ -194,17 +192,9 @@ def prepare(case, seed):
     return s
 
 
-def _package():
-    """The package's folder, as a program that uses it has it on its path."""
-    at = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "ah-rag_amd")
-    if at not in sys.path:
-        sys.path.insert(0, at)
-
-
 def _layout(lengths, key_lengths, dev):
     """The handle that a program keeps for a batch: made once, used by every layer."""
     if own:
-        _package()
         from ah_rag.packed import PackedLayout
         return PackedLayout(lengths, key_lengths=key_lengths, device=dev)
     return None
@@ -223,7 +213,6 @@ def run(state):
 
 
 def _run_own(s):
-    _package()
     from ah_rag.packed import packed_attention, packed_mean_pool, prefix_attention, qk_norm_rope
     case = s["case"]
     op = case["op"]
