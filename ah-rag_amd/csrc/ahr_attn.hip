@@ -234,8 +234,12 @@ __global__ __launch_bounds__(kWaves * 64, DP <= 64 ? 4 : 2) void attn_fwd_kernel
 #pragma unroll
       for (int r = 0; r < 16; ++r) x[r & 3] = fmaf(st.acc[b][r], 0.f, x[r & 3]);
     const bool odd = live && !(fabsf((x[0] + x[1]) + (x[2] + x[3])) < INFINITY);
-    // (both half-lanes of a row have to agree)
-    if (__any(odd) && (odd || __shfl_xor((int)odd, 32, 64))) strict_row<T, DP>(st, p, it, hk, head, tok, lim, h);
+    if (__any(odd)) {
+      // Both halves of a row take the strict path where either has to: they share its weights and its sum. (The
+      // exchange runs in every lane: a lane that a branch has switched off hands over nothing.)
+      const bool other = __shfl_xor((int)odd, 32, 64) != 0;
+      if (odd || other) strict_row<T, DP>(st, p, it, hk, head, tok, lim, h);
+    }
   }
   if (!live) return;
   const float l = st.l + other_half(st.l);

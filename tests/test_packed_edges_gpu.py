@@ -1,0 +1,103 @@
+"""Edges of the packed-sequence operators on the GPU, against the 64-bit restatement (oracle/packed_ref.py) and the
+bounds that it derives."""
+import math
+
+import pytest
+import torch
+
+from oracle import packed_ref as ref
+
+pytestmark = pytest.mark.gpu
+BF, HF = torch.bfloat16, torch.float16
+
+
+def _normal(shape, seed, dtype, dev):
+    return torch.randn(shape, generator=torch.Generator().manual_seed(seed)).to(dtype).to(dev)
+
+
+def _within(got, want, tol, what):
+    """Within tol where `want` is finite; the same infinity, or NaN, where it is not."""
+    got = got.detach().cpu().double()
+    assert got.shape == want.shape
+    fin = torch.isfinite(want)
+    off = (got - want).abs()[fin]
+    bad = ~(off <= tol[fin])
+    assert not bad.any(), f"{what}: {int(bad.sum())} of {bad.numel()} off, worst {float((off / tol[fin]).nan_to_num(1e9).max()):.3g} x the bound"
+    a, b = got[~fin], want[~fin]
+    assert ((a == b) | (a.isnan() & b.isnan())).all(), f"{what}: values that are not finite differ"
+
+
+# A value that is not finite in ONE column of one row of v: the columns of a row's output lie in two halves of a wave
+# (columns with d & 4, and the others), which have to take the same weights and the same sum.
+
+
+@pytest.mark.parametrize("dim,dt", [(24, BF), (32, HF), (64, BF), (56, HF), (96, HF), (80, BF), (128, BF), (128, HF)])
+@pytest.mark.parametrize("col", [0, 3, 4, 7, -1])
+@pytest.mark.parametrize("val", [math.nan, math.inf])
+def test_one_bad_column_of_a_value(cuda, dim, dt, col, val):
+    from ah_rag.packed import PackedLayout, packed_attention, prefix_attention
+    scale = dim ** -0.5
+    lens = [100, 30]
+    q, k, v, pv = (_normal((130, h, dim), 40 + i, dt, cuda) for i, h in enumerate((4, 2, 2, 2)))
+    pk, pv = k[20:90].clone(), pv[:70].clone()
+    bad = v.clone()
+    bad[37, 1, col] = val
+    lay = PackedLayout(lens, device=cuda)
+    _within(packed_attention(q, k, bad, lay, causal=True), *ref.attention(q, k, bad, lens, lens, True, scale), "causal")
+    _within(packed_attention(q, k, bad, lay), *ref.attention(q, k, bad, lens, lens, False, scale), "full")
+    _within(prefix_attention(q, k, bad, pk, pv, lay), *ref.attention(q, k, bad, lens, lens, True, scale, pk, pv), "own value, with a prefix")
+    pv[50, 0, col] = val
+    _within(prefix_attention(q, k, v, pk, pv, lay), *ref.attention(q, k, v, lens, lens, True, scale, pk, pv), "a prefix value")
+
+
+@pytest.mark.parametrize("dim,dt", [(64, BF), (40, HF), (128, BF), (96, HF)])
+@pytest.mark.parametrize("col", [0, 3, 4, 7, -1])
+def test_one_bad_column_in_split_plans(cuda, dim, dt, col):
+    """Keys in pieces that are joined: the piece with the bad value, hidden from the first query and read by the second;
+    and a prefix that is read apart."""
+    from ah_rag.packed import _CODES, PackedLayout, packed_attention, prefix_attention
+    scale = dim ** -0.5
+    ql, kl = [2, 1], [2000, 700]
+    q, k, v = (_normal((n, h, dim), 50 + i, dt, cuda) for i, (n, h) in enumerate(((3, 8), (2700, 2), (2700, 2))))
+    v[1999, 0, col] = math.nan
+    v[1000, 1, col] = math.inf
+    lay = PackedLayout(ql, kl, cuda)
+    assert lay._plan(_CODES[dt], 8, 2, dim, True, False, 0)[0].n_join > 0
+    _within(packed_attention(q, k, v, lay, causal=True), *ref.attention(q, k, v, ql, kl, True, scale), "pieces")
+    lens, prefix = [3] * 40, 1300
+    q, k, v, pk, pv = (_normal((n, h, dim), 60 + i, dt, cuda) for i, (n, h) in enumerate(((120, 8), (120, 4), (120, 4), (prefix, 4), (prefix, 4))))
+    v[61, 2, col] = math.inf
+    lay = PackedLayout(lens, device=cuda)
+    assert lay._plan(_CODES[dt], 8, 4, dim, True, False, prefix)[0].n_join > 0
+    _within(prefix_attention(q, k, v, pk, pv, lay), *ref.attention(q, k, v, lens, lens, True, scale, pk, pv), "a prefix read apart")
+    pv[777, 1, col] = math.nan
+    _within(prefix_attention(q, k, v, pk, pv, lay), *ref.attention(q, k, v, lens, lens, True, scale, pk, pv), "its values")
+
+
+@pytest.mark.parametrize("dim", [32, 64, 96, 128])
+@pytest.mark.parametrize("col", [0, 5])
+def test_values_that_overflow_one_half_of_a_row(cuda, dim, col):
+    """Large finite values in one column: weights relative to a reference that is raised late reach 2^8, so one half's
+    sums pass fp32 before they are divided. Output, log-sum and gradients are what finite inputs give."""
+    from ah_rag import packed
+    scale = dim ** -0.5
+    n = 150
+    q = torch.zeros(n, 1, dim)
+    q[:, 0, 1] = dim ** 0.5
+    k = torch.zeros(n, 1, dim)
+    k[140, 0, 1] = 5.0  # its score is 5 and the others' 0: 2^7.2 of the first tiles' reference
+    q, k, v, d_o = q.to(BF).to(cuda), k.to(BF).to(cuda), _normal((n, 1, dim), 70, BF, cuda), _normal((n, 1, dim), 71, BF, cuda)
+    v[140, 0, col] = 3e38
+    d_o[..., col] = 0.0
+    lay = packed.PackedLayout([n], device=cuda)
+    want, tol, w_g, t_g = ref.attention(q, k, v, [n], [n], False, scale, d_o=d_o)
+    assert torch.isfinite(want).all()
+    lse = torch.empty(n, 1, device=cuda)
+    _within(packed._attention(q, k, v, lay, False, scale, lse), want, tol, "o")
+    # (in fp32: the scores' error of (dim + 4) 2^-24 of sum |q k|, and a few steps of a value below 16 for the logarithm and the sum)
+    w_lse = math.log2(149 + math.exp(float(q[0, 0, 1].double() * 5 * scale)))
+    assert (lse.double() - w_lse).abs().max() < (dim + 4) * 2.0 ** -24 * 5 * 1.5 + 8 * 2.0 ** -21
+    leaves = [x.detach().requires_grad_() for x in (q, k, v)]
+    grads = torch.autograd.grad(packed.packed_attention(*leaves, lay), leaves, d_o)
+    for name, a, w, t in zip(("dq", "dk", "dv"), grads, w_g, t_g):
+        _within(a, w, t, name)
