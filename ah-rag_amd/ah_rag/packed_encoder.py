@@ -131,12 +131,12 @@ class PackedTransformer:
 
     def _qkv(self, i: int, x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
         """Queries, keys and values [tokens, heads, head_dim]: views of one projection's output, or three products
-        where the weights' gradients are wanted."""
+        where a gradient of the projections is wanted."""
         prefix, names = self.fused[i]
         ws = [self.w[prefix + n + ".weight"] for n in names]
         bs = [self.w.get(prefix + n + ".bias") for n in names]
         d = self.head_dim
-        if torch.is_grad_enabled() and any(t.requires_grad for t in ws):
+        if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (*ws, *bs)):
             return tuple(F.linear(x, a, b).view(x.shape[0], -1, d) for a, b in zip(ws, bs))
         if len({b is None for b in bs}) != 1:
             bs = [torch.zeros_like(a[:, 0]) if b is None else b for a, b in zip(ws, bs)]
