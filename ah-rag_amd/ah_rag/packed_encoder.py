@@ -46,6 +46,9 @@ def _get(cfg, *names, default=None):
 _POST = ("attention.self.query", "attention.self.key", "attention.self.value", "attention.output.dense", "attention.output.LayerNorm",
          "intermediate.dense", "output.dense", "output.LayerNorm")
 _CAUSAL = ("self_attn.q_proj", "self_attn.k_proj", "self_attn.v_proj", "self_attn.o_proj", "mlp.gate_proj", "mlp.up_proj", "mlp.down_proj")
+# Model types whose forward is that of their layout (None: a module that names no type). Others share the parameters' names
+# and settings, but start their positions elsewhere or compute attention in another way.
+_TYPES = {"post": (None, "bert", "bert-generation", "electra", "ernie", "splinter"), "causal": (None, "qwen3", "qwen3_vl_text")}
 _CAUSAL_NORMS = ("self_attn.q_norm", "self_attn.k_norm", "input_layernorm", "post_attention_layernorm")
 
 
@@ -72,7 +75,8 @@ class PackedTransformer:
                 raise UnsupportedLayoutError("packed forward: a decoder's masks")
             if _get(cfg, "position_embedding_type", default="absolute") != "absolute":
                 raise UnsupportedLayoutError("packed forward: positions other than absolute ones")
-            if "encoder.relative_attention_bias.weight" in w or _get(cfg, "model_type") in ("roberta", "xlm-roberta", "mpnet"):
+            table = getattr(getattr(model, "embeddings", None), "position_embeddings", None)
+            if getattr(table, "padding_idx", None) is not None:  # (the first token's row is the one after it)
                 raise UnsupportedLayoutError("packed forward: this model's positions are not those of its tokens")
             self.act = self._activation(cfg.hidden_act)
             self.fused = [("encoder.layer.%d.attention.self." % i, ("query", "key", "value")) for i in range(self.layers)]
@@ -105,6 +109,8 @@ class PackedTransformer:
             self._table: Optional[Tuple[torch.Tensor, torch.Tensor]] = None
         else:
             raise UnsupportedLayoutError("packed forward: unknown layer layout")
+        if _get(cfg, "model_type") not in _TYPES[self.kind]:
+            raise UnsupportedLayoutError(f"packed forward: a model of type {cfg.model_type!r}")
         p = next(iter(w.values()))
         if p.dtype not in (torch.float16, torch.bfloat16):
             raise UnsupportedLayoutError(f"packed forward: weights in float16 or bfloat16, got {p.dtype}")

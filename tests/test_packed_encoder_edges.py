@@ -37,3 +37,85 @@ def test_gradients_of_the_biases_alone(make, which):
     want = d.double().flatten(1).sum(0)
     # a sum of 7 values in fp32 at least, or in bf16 at worst: 7 roundings of the absolute sum
     assert ((got.double() - want).abs() <= 7 * ref.half_step(torch.bfloat16) * d.double().flatten(1).abs().sum(0)).all()
+
+
+def _tiny(model_type, **more):
+    """A model of that type with random weights, small enough for the CPU."""
+    from transformers import AutoConfig, AutoModel
+    c = AutoConfig.for_model(model_type)
+    small = dict(hidden_size=64, num_hidden_layers=2, num_attention_heads=4, intermediate_size=96, vocab_size=50, max_position_embeddings=40,
+                 num_key_value_heads=2, head_dim=16, embedding_size=64)
+    for n, x in {**{n: x for n, x in small.items() if hasattr(c, n)}, **more}.items():
+        setattr(c, n, x)
+    if getattr(c, "layer_types", None):
+        c.layer_types = ["full_attention"] * 2
+    c._attn_implementation = "eager"
+    torch.manual_seed(7)
+    m = AutoModel.from_config(c)
+    with torch.no_grad():
+        for p in m.parameters():  # (biases and norms too, so that none goes unseen)
+            p.add_(0.05 * torch.randn(p.shape))
+    return m.to(torch.bfloat16).eval()
+
+
+class _Layout:
+    """What the forward reads of a layout, on the host."""
+
+    def __init__(self, lengths):
+        self.lengths = torch.tensor(lengths).numpy()
+
+    def __len__(self):
+        return len(self.lengths)
+
+    def positions(self):
+        return torch.cat([torch.arange(n, dtype=torch.int32) for n in self.lengths.tolist()])
+
+
+def _plain_operators(monkeypatch):
+    """The forward on the CPU: the operators' 64-bit restatement in the place of the kernels."""
+    from ah_rag import packed_encoder
+
+    def attention(q, k, v, layout, causal=False):
+        lens = layout.lengths.tolist()
+        return ref.attention(q, k, v, lens, lens, causal, q.shape[2] ** -0.5)[0].to(q.dtype)
+
+    def rope(q, k, wq, wk, cos, sin, positions, eps):
+        return tuple(ref.rotate(x, w, cos, sin, positions, eps, False).to(x.dtype) for x, w in ((q, wq), (k, wk)))
+
+    monkeypatch.setattr(packed_encoder, "packed_attention", attention)
+    monkeypatch.setattr(packed_encoder, "qk_norm_rope", rope)
+
+
+@pytest.mark.parametrize("model_type", ["bert", "bert-generation", "electra", "ernie", "splinter", "qwen3", "qwen3_vl_text"])
+def test_accepted_models_give_their_own_hidden_states(monkeypatch, model_type):
+    """The forward over packed tokens against the model's own, one sequence at a time. Both round some twenty rows of
+    each layer to bf16 (half a step each), which at random add up like their square root: 16 half steps are well above
+    that and far below a wrong position, norm or mask (of order one)."""
+    from ah_rag.packed_encoder import PackedTransformer
+    m = _tiny(model_type)
+    _plain_operators(monkeypatch)
+    t = PackedTransformer(m, torch.device("cpu"))
+    ids = _ids([5, 17, 1, 33], vocab=50)
+    with torch.no_grad():
+        x = (t._post if t.kind == "post" else t._causal)(torch.tensor([i for s in ids for i in s]), _Layout([len(s) for s in ids]))
+        want = torch.cat([m(input_ids=torch.tensor([s])).last_hidden_state[0] for s in ids])
+    assert _off(x, want.double()) < 16 * ref.half_step(torch.bfloat16)
+
+
+@pytest.mark.parametrize("model_type", ["roberta", "xlm-roberta", "camembert", "data2vec-text", "ibert", "mra", "yoso", "big_bird"])
+def test_models_with_other_positions_or_attention_are_refused(model_type):
+    """Their parameters have the names of the bidirectional layout, but their positions do not start at 0 (or their
+    attention is another)."""
+    from ah_rag.packed_encoder import PackedTransformer, UnsupportedLayoutError
+    with pytest.raises(UnsupportedLayoutError):
+        PackedTransformer(_tiny(model_type), DEV)
+
+
+def test_a_padded_position_table_is_refused():
+    """A position table with a padding row gives the first token a position after it, whatever the model calls itself."""
+    from ah_rag.packed_encoder import PackedTransformer, UnsupportedLayoutError
+    m = post()
+    w = m.embeddings.position_embeddings.weight
+    m.embeddings.position_embeddings = torch.nn.Embedding(*w.shape, padding_idx=1, dtype=w.dtype)
+    with pytest.raises(UnsupportedLayoutError, match="positions"):
+        PackedTransformer(m, DEV)
