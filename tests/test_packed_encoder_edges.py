@@ -119,3 +119,113 @@ def test_a_padded_position_table_is_refused():
     m.embeddings.position_embeddings = torch.nn.Embedding(*w.shape, padding_idx=1, dtype=w.dtype)
     with pytest.raises(UnsupportedLayoutError, match="positions"):
         PackedTransformer(m, DEV)
+
+
+def _frozen(model):
+    return model.requires_grad_(False)
+
+
+@pytest.mark.parametrize("joins", [False, True])
+@pytest.mark.parametrize("make", [causal, post])
+def test_projections_follow_every_write_to_the_weights(monkeypatch, make, joins):
+    """In place, through .data, to inference tensors, by a loaded state dict: the next forward computes with what stands in
+    the weights, with each layer's projections joined for it or apart."""
+    from ah_rag import packed_encoder
+    from ah_rag.packed_encoder import PackedTransformer
+    if not joins:
+        monkeypatch.setattr(packed_encoder, "JOIN_UP_TO", 0)
+    with torch.inference_mode():
+        held = _frozen(make())
+    for m in (_frozen(make()), held):
+        t = PackedTransformer(m, torch.device("cpu"))
+        prefix, names = t.fused[1]
+        w, b = (dict(m.named_parameters()).get(prefix + names[1] + s) for s in (".weight", ".bias"))
+        x = torch.randn(5, m.config.hidden_size, generator=torch.Generator().manual_seed(1)).to(torch.bfloat16)
+
+        def keys():
+            with torch.inference_mode():
+                joined = t._joined()
+                assert (joined is not None) == joins
+                got = t._qkv(1, x, joined)[1].clone()
+                assert _off(got.flatten(1), x.double() @ w.double().T + (0 if b is None else b.double())) < 2 * ref.half_step(torch.bfloat16)
+                return got
+
+        first = keys()
+        with torch.inference_mode():
+            w.add_(0.5)
+        second = keys()
+        w.data.mul_(2.0)
+        third = keys()
+        assert not torch.equal(first, second) and not torch.equal(second, third)
+        if m is not held:
+            m.load_state_dict({n: p.detach() * 0.5 for n, p in m.named_parameters()})
+            assert not torch.equal(third, keys())
+
+
+@pytest.mark.parametrize("make", [causal, post])
+def test_joined_projections_give_what_three_products_give(make):
+    """One product over the three projections of a layer, or three: each value a sum in fp32 that is rounded once."""
+    from ah_rag.packed_encoder import PackedTransformer
+    m = make()
+    t = PackedTransformer(m, torch.device("cpu"))
+    assert t._joined() is None  # (the weights' gradients are wanted)
+    x = torch.randn(5, m.config.hidden_size, generator=torch.Generator().manual_seed(1)).to(torch.bfloat16)
+    with torch.no_grad():
+        for i in range(t.layers):
+            for a, b in zip(t._qkv(i, x, t._joined()), t._qkv(i, x)):
+                assert a.shape == b.shape and _off(a, b.double()) < 2 * ref.half_step(torch.bfloat16)
+    m.requires_grad_(False)
+    assert t._joined() is not None
+    list(m.parameters())[-1].requires_grad_()
+    assert t._joined() is not None
+    t.w[t.fused[0][0] + t.fused[0][1][1] + ".weight"].requires_grad_()
+    assert t._joined() is None
+    if make is causal:  # a bias in one layer alone: three products
+        m.layers._modules["0"].self_attn.k_proj.register_parameter("bias", torch.nn.Parameter(torch.ones(128, dtype=torch.bfloat16)))
+        t = PackedTransformer(m, torch.device("cpu"))
+        with torch.no_grad():
+            assert t._joined() is None and _off(t._qkv(0, x)[1].flatten(1) - 1, (x @ t.w["layers.0.self_attn.k_proj.weight"].T).double()) < 0.02
+
+
+# ---- on the GPU --------------------------------------------------------------------------------
+
+
+@pytest.mark.gpu
+def test_a_fresh_encoder_on_two_streams(cuda):
+    """The first calls of an encoder at once from two threads, each on a stream of its own, with writes to the weights
+    between rounds: every result is that of one call alone."""
+    import threading
+
+    from ah_rag.encoder import TorchEncoder
+    texts = ["Entity: " + "river city album " * (1 + i % 20) for i in range(60)]
+    for rnd in range(3):
+        enc = TorchEncoder("all-MiniLM-L6-v2", cuda, packed=True)
+        with torch.inference_mode():
+            assert enc.packed._joined() is not None
+        for change in range(3):
+            if change:
+                with torch.no_grad():
+                    for p in enc.model.parameters():
+                        p.data.mul_(1.0 + 0.01 * change)
+                torch.cuda.synchronize()
+            got, errors = {}, []
+
+            def work(i):
+                try:
+                    s = torch.cuda.Stream()
+                    with torch.cuda.stream(s):
+                        y = enc.encode(texts, normalize_embeddings=True, convert_to_tensor=True)
+                        s.synchronize()
+                        got[i] = y.cpu()
+                except Exception as e:  # noqa: BLE001
+                    errors.append(e)
+
+            threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+            for t in threads:
+                t.start()
+            for t in threads:
+                t.join()
+            assert not errors, errors
+            want = enc.encode(texts, normalize_embeddings=True, convert_to_tensor=True).cpu()
+            for y in got.values():
+                assert torch.equal(y, want)
