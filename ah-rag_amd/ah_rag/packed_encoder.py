@@ -20,7 +20,7 @@ Reference seam: SentenceTransformer.encode, src/ah_rag/graph/hierarchical_graph.
 """
 from __future__ import annotations
 
-from typing import Dict, List, Optional, Sequence, Tuple
+from typing import List, Mapping, Optional, Sequence, Tuple
 
 import numpy as np
 import torch
@@ -56,14 +56,35 @@ _TYPES = {"post": (None, "bert", "bert-generation", "electra", "ernie", "splinte
 _CAUSAL_NORMS = ("self_attn.q_norm", "self_attn.k_norm", "input_layernorm", "post_attention_layernorm")
 
 
+class _Parameters(Mapping):
+    """A model's parameters by name, each looked up in its module when it is read, so that one which another has taken the
+    place of is not used on."""
+
+    def __init__(self, model) -> None:
+        self._at = {}
+        for name, _ in model.named_parameters():
+            path, _, leaf = name.rpartition(".")
+            self._at[name] = (model.get_submodule(path)._parameters, leaf)
+
+    def __getitem__(self, name: str) -> torch.Tensor:
+        held, leaf = self._at[name]
+        return held[leaf]
+
+    def __iter__(self):
+        return iter(self._at)
+
+    def __len__(self) -> int:
+        return len(self._at)
+
+
 class PackedTransformer:
-    """Weights are the model's own tensors (parameters receive gradients); `model` stays referenced."""
+    """Weights are the model's own tensors (parameters receive gradients); `model` stays referenced, with the modules that
+    it has now."""
 
     def __init__(self, model, device: torch.device) -> None:
         self.model, self.device = model, device
         cfg = model.config
-        w: Dict[str, torch.Tensor] = dict(model.named_parameters())
-        self.w = w
+        self.w = w = _Parameters(model)
         self.heads = int(cfg.num_attention_heads)
         self.layers = int(cfg.num_hidden_layers)
         self.hidden = int(cfg.hidden_size)

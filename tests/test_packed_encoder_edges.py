@@ -187,6 +187,26 @@ def test_joined_projections_give_what_three_products_give(make):
             assert t._joined() is None and _off(t._qkv(0, x)[1].flatten(1) - 1, (x @ t.w["layers.0.self_attn.k_proj.weight"].T).double()) < 0.02
 
 
+@pytest.mark.parametrize("make", [causal, post])
+def test_replaced_parameters_are_used(make):
+    """Parameters that other ones have taken the place of (a state dict assigned, an attribute set): the forward reads and
+    trains the model's, not those that it had first."""
+    from ah_rag.packed_encoder import PackedTransformer
+    m = make()
+    t = PackedTransformer(m, torch.device("cpu"))
+    old = t.w[t.fused[1][0] + t.fused[1][1][0] + ".weight"]
+    m.load_state_dict({n: p.detach() * 2 for n, p in m.named_parameters()}, assign=True)
+    assert all(t.w[n] is p for n, p in m.named_parameters()) and set(t.w) == {n for n, _ in m.named_parameters()}
+    x = torch.randn(5, m.config.hidden_size, generator=torch.Generator().manual_seed(1)).to(torch.bfloat16)
+    y = t._qkv(1, x)[0]
+    d = torch.randn(y.shape, generator=torch.Generator().manual_seed(2)).to(torch.bfloat16)
+    new = t.w[t.fused[1][0] + t.fused[1][1][0] + ".weight"]
+    grad, = torch.autograd.grad(y, new, d)
+    assert new is not old and _off(grad, d.double().flatten(1).T @ x.double()) < 2 * ref.half_step(torch.bfloat16)
+    with torch.no_grad():
+        assert _off(t._qkv(1, x, t._joined())[0], y.double()) < 2 * ref.half_step(torch.bfloat16)
+
+
 # ---- on the GPU --------------------------------------------------------------------------------
 
 
