@@ -131,7 +131,7 @@ class PackedTransformer:
             self.theta = float(rope.get("rope_theta", _get(cfg, "rope_theta", default=10000.0)))
             self.act = self._activation(cfg.hidden_act)
             self.fused = [("layers.%d.self_attn." % i, ("q_proj", "k_proj", "v_proj")) for i in range(self.layers)]
-            self._table: Optional[Tuple[torch.Tensor, torch.Tensor]] = None
+            self._table: Optional[Tuple[torch.Tensor, torch.Tensor, Optional[torch.cuda.Stream]]] = None  # cos, sin, made on
         else:
             raise UnsupportedLayoutError("packed forward: unknown layer layout")
         if _get(cfg, "model_type") not in _TYPES[self.kind]:
@@ -214,9 +214,21 @@ class PackedTransformer:
         return x
 
     def _rotary(self, n: int) -> Tuple[torch.Tensor, torch.Tensor]:
-        if self._table is None or self._table[0].shape[0] < n:
-            self._table = rotary_table(max(512, n), self.head_dim, self.theta, self.device)
-        return self._table
+        """A table of n positions at least. It is complete when rotary_table returns (a blocking copy), and a stream that did
+        not make it is noted as its reader, since a longer one may take its place while that stream still reads it."""
+        held = self._table
+        if held is None or held[0].shape[0] < n:
+            table = rotary_table(max(512, n), self.head_dim, self.theta, self.device)
+            self._table = held = (*table, self._stream())
+        cos, sin, made_on = held
+        stream = self._stream()
+        if stream != made_on:
+            cos.record_stream(stream)
+            sin.record_stream(stream)
+        return cos, sin
+
+    def _stream(self) -> Optional[torch.cuda.Stream]:
+        return torch.cuda.current_stream(self.device) if self.device.type == "cuda" else None
 
     def _causal(self, ids: torch.Tensor, layout: PackedLayout, first: int = 0, shared: Optional[List[tuple]] = None,
                 keep: Optional[List[tuple]] = None) -> torch.Tensor:

@@ -207,6 +207,33 @@ def test_replaced_parameters_are_used(make):
         assert _off(t._qkv(1, x, t._joined())[0], y.double()) < 2 * ref.half_step(torch.bfloat16)
 
 
+def test_a_rotary_table_is_long_enough_whatever_another_thread_stores():
+    """Another thread stores a shorter table between the look at its length and its use: the call goes on with one of the
+    length that it asked for (rows past a shorter one would be NaN)."""
+    from ah_rag.packed_encoder import PackedTransformer
+    t = PackedTransformer(causal(), torch.device("cpu"))
+    t._rotary(700)
+    long, short = t._table, (torch.zeros(512, 32), torch.zeros(512, 32), *t._table[2:])
+
+    for swap_at in (1, 2, 3):
+        class Swapped(PackedTransformer):
+            looks = 0
+
+            @property
+            def _table(self):
+                self.looks += 1
+                return long if self.looks < swap_at else short
+
+            @_table.setter
+            def _table(self, new):
+                pass
+
+        t.__dict__.pop("_table", None)
+        t.__dict__.pop("looks", None)
+        t.__class__ = Swapped
+        assert all(x.shape[0] >= 650 for x in t._rotary(650)[:2]), swap_at
+
+
 # ---- on the GPU --------------------------------------------------------------------------------
 
 
@@ -249,3 +276,28 @@ def test_a_fresh_encoder_on_two_streams(cuda):
             want = enc.encode(texts, normalize_embeddings=True, convert_to_tensor=True).cpu()
             for y in got.values():
                 assert torch.equal(y, want)
+
+
+@pytest.mark.gpu
+def test_a_replaced_rotary_table_outlives_its_readers(cuda):
+    """A longer text on one stream replaces the table that another stream still waits to read: its memory is not handed out
+    before."""
+    from ah_rag.packed_encoder import PackedTransformer
+    t = PackedTransformer(causal(layers=1).to(cuda), cuda)
+    side = torch.cuda.Stream()
+    with torch.inference_mode():
+        want = torch.cat(t._rotary(300))
+        fresh = [torch.full((512, 32), 1.0, device=cuda) for _ in range(64)]
+        del fresh
+        torch.cuda.synchronize()
+        old = {x.data_ptr() for x in t._rotary(300)}
+        with torch.cuda.stream(side):
+            torch.cat(t._rotary(300))
+            torch.cuda._sleep(1_000_000_000)  # (a finite wait on the device's clock)
+            got = torch.cat(t._rotary(300))
+        t._rotary(900)  # a longer table here, which lets the old one go
+        # memory of the old table's size: none of it may be the old table's while the side stream still reads that
+        fresh = [torch.full((512, 32), float("nan"), device=cuda) for _ in range(64)]
+        assert not side.query() and not {f.data_ptr() for f in fresh} & old
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
