@@ -36,6 +36,7 @@ from typing import Dict, Optional, Sequence, Tuple, Union
 
 import numpy as np
 import torch
+from torch.autograd import forward_ad
 
 from . import _native as nat
 
@@ -158,6 +159,15 @@ def _on_device(device: torch.device, *tensors: Optional[torch.Tensor]) -> None:
     for t in tensors:
         if t is not None and t.device != device:
             raise ValueError(f"tensors must be on {device}, got one on {t.device}")
+
+
+def _no_tangent(*tensors: Optional[torch.Tensor]) -> None:
+    """Forward-mode derivatives are refused: past autograd's function, a tangent would be dropped and read as zero."""
+    if forward_ad._current_level < 0:
+        return
+    for t in tensors:
+        if isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None:
+            raise RuntimeError("the packed operators have no forward-mode derivative")
 
 
 def _aligned(t: torch.Tensor) -> torch.Tensor:
@@ -348,6 +358,7 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, layout: 
     after the current stream's work; the caller orders what follows. A key or value that a row's mask
     hides never reaches that row's output, whatever it holds; in the gradients a value that is not finite may
     reach any row of its own sequence, and none of another."""
+    _no_tangent(q, k, v)
     scale = _check_attention(q, k, v, layout, scale)
     _check_out(out, q)
     grad = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)
@@ -371,6 +382,7 @@ def prefix_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, prefix_k
     sequences together where sequences are short, so its cost does not grow with their number. causal
     concerns the own keys alone. No gradient: inputs that require one are refused while gradients are
     enabled."""
+    _no_tangent(q, k, v, prefix_k, prefix_v)
     scale = _check_attention(q, k, v, layout, scale)
     _check_out(out, q)
     _like(prefix_k, "prefix_k", q)
@@ -473,6 +485,7 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: Optional[torch.Tens
     outside [0, n) gives NaN rows. Pairs: element i with i + rot / 2, or with interleaved 2 i with
     2 i + 1. head_dim even, at most 512. Computed in fp32, rounded once. Differentiable in q, k and the
     weights (whose gradients are summed in a fixed order)."""
+    _no_tangent(q, k, q_weight, k_weight, cos, sin)
     _heads(q, "q")
     _like(k, "k", q)
     if q.dtype not in _CODES:
@@ -561,6 +574,7 @@ def packed_mean_pool(rows: torch.Tensor, layout: PackedLayout, normalize: bool =
     """float32 [sequences, width]: the mean of each sequence's rows, summed in fp32; with normalize divided
     by max(its L2 norm, 1e-12). rows [tokens, width] in float32, float16 or bfloat16, any row stride. A
     sequence without rows gives zeros. Differentiable in rows."""
+    _no_tangent(rows)
     if not isinstance(rows, torch.Tensor) or rows.dim() != 2 or rows.shape[1] < 1 or rows.shape[1] > 1 << 20:
         raise ValueError("rows must be a [tokens, width] tensor")
     if rows.dtype not in _CODES:

@@ -4,6 +4,7 @@ import subprocess
 import sys
 
 import pytest
+import torch
 
 
 @pytest.mark.parametrize("path", [["."], ["ah-rag_amd"], [".", "ah-rag_amd"], ["ah-rag_amd", "."]], ids="+".join)
@@ -22,3 +23,27 @@ def test_the_package_imports_from_the_repository_root(path):
     init, packed, _ = (os.path.normpath(x) for x in out.stdout.split()[:3])
     pkg = os.path.join(root, "ah-rag_amd", "ah_rag")
     assert init == os.path.join(pkg, "__init__.py") and packed == os.path.join(pkg, "packed.py")
+
+
+def test_forward_mode_derivatives_are_refused():
+    """A tangent of any input is refused, whether or not a gradient is wanted too, and before anything else is looked at."""
+    import torch.autograd.forward_ad as fwd
+    from ah_rag.packed import PackedLayout, packed_attention, packed_mean_pool, prefix_attention, qk_norm_rope
+    lay = PackedLayout([3], device="cuda:0")
+
+    def new(*shape, dtype=torch.bfloat16):
+        return torch.ones(shape, dtype=dtype)
+
+    x, w, table, pos = new(3, 2, 16), new(16, dtype=torch.float32), new(8, 8, dtype=torch.float32), torch.zeros(3, dtype=torch.int32)
+    calls = [(lambda *a: packed_attention(*a, lay), [x, x, x]), (lambda *a: prefix_attention(*a, lay), [x, x, x, x, x]),
+             (lambda *a: qk_norm_rope(*a, pos), [x, x, w, w, table, table]), (lambda a: packed_mean_pool(a, lay), [new(3, 16)])]
+    with fwd.dual_level():
+        for call, args in calls:
+            for i, a in enumerate(args):
+                for wants in (False, True):
+                    dual = fwd.make_dual(a.clone().requires_grad_(wants), torch.ones_like(a))
+                    with pytest.raises(RuntimeError, match="forward-mode"):
+                        call(*args[:i], dual, *args[i + 1:])
+            with pytest.raises((ValueError, RuntimeError)) as e:  # without a tangent: the host tensors are refused
+                call(*args)
+            assert "forward-mode" not in str(e.value)
