@@ -178,12 +178,12 @@ class PackedTransformer:
     def _qkv(self, i: int, x: torch.Tensor, joined: Optional[List[Tuple[torch.Tensor, Optional[torch.Tensor]]]] = None
              ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
         """Queries, keys and values [tokens, heads, head_dim]: views of one product's output, or three products."""
-        d = self.head_dim
+        h, hk, d = self.heads, self.kv_heads, self.head_dim
         if joined is not None:
-            y = F.linear(x, *joined[i]).view(x.shape[0], -1, d)
-            return y[:, :self.heads], y[:, self.heads:self.heads + self.kv_heads], y[:, self.heads + self.kv_heads:]
+            y = F.linear(x, *joined[i]).view(x.shape[0], h + 2 * hk, d)
+            return y[:, :h], y[:, h:h + hk], y[:, h + hk:]
         prefix, names = self.fused[i]
-        return tuple(self._lin(prefix + n, x).view(x.shape[0], -1, d) for n in names)
+        return tuple(self._lin(prefix + n, x).view(x.shape[0], m, d) for n, m in zip(names, (h, hk, hk)))
 
     def refresh(self) -> None:
         """Nothing to do, for programs that call it after writing to the weights: nothing made from them is kept."""

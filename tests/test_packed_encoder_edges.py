@@ -234,6 +234,25 @@ def test_a_rotary_table_is_long_enough_whatever_another_thread_stores():
         assert all(x.shape[0] >= 650 for x in t._rotary(650)[:2]), swap_at
 
 
+@pytest.mark.parametrize("make", [causal, post])
+@pytest.mark.parametrize("grad", [False, True])
+@pytest.mark.parametrize("ids", [[], [[]], [[], []]], ids=str)
+def test_batches_without_tokens(monkeypatch, make, grad, ids):
+    """No text, or texts without a token (an empty string, where the tokenizer adds none): no rows."""
+    from ah_rag.packed_encoder import PackedTransformer
+    _plain_operators(monkeypatch)
+    m = make()
+    t = PackedTransformer(m, torch.device("cpu"))
+
+    class Layout(_Layout):
+        def positions(self):
+            return torch.zeros(0, dtype=torch.int32)
+
+    with torch.set_grad_enabled(grad):
+        x = (t._post if t.kind == "post" else t._causal)(torch.zeros(0, dtype=torch.int64), Layout([0] * len(ids)))
+    assert x.shape == (0, m.config.hidden_size)
+
+
 # ---- on the GPU --------------------------------------------------------------------------------
 
 
@@ -301,3 +320,21 @@ def test_a_replaced_rotary_table_outlives_its_readers(cuda):
         assert not side.query() and not {f.data_ptr() for f in fresh} & old
         torch.cuda.synchronize()
         assert torch.equal(got, want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("make", [causal, post])
+def test_texts_without_tokens(cuda, make):
+    """Zeros for a text without tokens (the mean of no rows), alone or among others, and zero gradients."""
+    from ah_rag.packed_encoder import PackedTransformer
+    m = make().to(cuda)
+    t = PackedTransformer(m, cuda)
+    some = _ids([4, 7], vocab=50)
+    for ids in ([], [[]], [[], []], [[], some[0], [], some[1]]):
+        with torch.inference_mode():
+            y = t.pooled(ids, True)
+            alone = t.pooled([s for s in ids if s], True)
+        assert y.shape == (len(ids), m.config.hidden_size) and y.dtype == torch.float32
+        assert torch.equal(y[[i for i, s in enumerate(ids) if s]], alone) and not y[[i for i, s in enumerate(ids) if not s]].any()
+        grads = torch.autograd.grad(t.pooled(ids, False).sum(), list(m.parameters()), allow_unused=True)
+        assert all(g is None or g.isfinite().all() for g in grads)
