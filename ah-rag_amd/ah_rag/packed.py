@@ -54,7 +54,8 @@ def _host_lengths(x: Lengths, what: str) -> np.ndarray:
         a = a.astype(np.int64).reshape(-1)
     if a.ndim != 1 or a.dtype.kind not in "iu":
         raise ValueError(f"{what} must be a list of whole numbers")
-    if a.size and (a.min() < 0 or int(a.sum(dtype=np.int64)) > 1 << 30):
+    # (each, then the sum: that of large values would wrap)
+    if a.size and (int(a.min()) < 0 or int(a.max()) > 1 << 30 or int(a.sum(dtype=np.int64)) > 1 << 30):
         raise ValueError(f"{what} must be >= 0 and sum to at most 2**30")
     own = np.array(a, dtype=np.int32)  # (a copy, and read-only: the work lists are made from it once)
     own.setflags(write=False)

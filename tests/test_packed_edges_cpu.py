@@ -3,6 +3,7 @@ import os
 import subprocess
 import sys
 
+import numpy as np
 import pytest
 import torch
 
@@ -47,3 +48,12 @@ def test_forward_mode_derivatives_are_refused():
             with pytest.raises((ValueError, RuntimeError)) as e:  # without a tangent: the host tensors are refused
                 call(*args)
             assert "forward-mode" not in str(e.value)
+
+
+@pytest.mark.parametrize("lengths", [[2 ** 62] * 4, [1 << 33], np.array([2 ** 63], np.uint64), np.array([2 ** 64 - 1, 1], np.uint64),
+                                     [2 ** 30, 1]], ids=str)
+def test_lengths_whose_sum_wraps_are_refused(lengths):
+    from ah_rag.packed import PackedLayout
+    for a, b in ((lengths, None), ([1] * len(lengths), lengths)):
+        with pytest.raises(ValueError, match="2\\*\\*30"):
+            PackedLayout(a, b, device="cuda:0")
