@@ -235,7 +235,11 @@ def _elsewhere(stream: Optional[torch.cuda.Stream], device: torch.device) -> boo
 
 
 def _on(stream: Optional[torch.cuda.Stream], device: torch.device, *tensors: Optional[torch.Tensor]):
-    return torch.cuda.device(device) if stream is None else _side(stream, device, *tensors)
+    if stream is None:
+        return torch.cuda.device(device)
+    if stream.device != device:
+        raise ValueError(f"a stream of {stream.device} for tensors on {device}")
+    return _side(stream, device, *tensors)
 
 
 def _keep(lists: Optional[torch.Tensor], stream: int, device: torch.device) -> None:

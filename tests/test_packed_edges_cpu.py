@@ -57,3 +57,12 @@ def test_lengths_whose_sum_wraps_are_refused(lengths):
     for a, b in ((lengths, None), ([1] * len(lengths), lengths)):
         with pytest.raises(ValueError, match="2\\*\\*30"):
             PackedLayout(a, b, device="cuda:0")
+
+
+def test_a_stream_of_another_device_is_refused():
+    """(It was left aside, and the call ran on the tensors' device's current stream.)"""
+    from types import SimpleNamespace
+
+    from ah_rag.packed import _on
+    with pytest.raises(ValueError, match="a stream of cuda:1"):
+        _on(SimpleNamespace(device=torch.device("cuda", 1)), torch.device("cuda", 0))
