@@ -285,6 +285,8 @@ def _attention(q, k, v, layout, causal, scale, lse, prefix_k=None, prefix_v=None
     plan, lists = layout._plan(_CODES[q.dtype], shape[1], k.shape[1], shape[2], causal, False, 0 if prefix_k is None else prefix_k.shape[0])
     o = _new(q) if out is None else out
     _launch_attention(_calls().attn_forward, "ahr_attn_forward", plan, lists, scale, q, k, v, prefix_k, prefix_v, o, lse, None, None, None, None)
+    if out is not None and not out.is_inference():
+        torch.autograd.graph.increment_version(out)  # (a graph that saved out has to notice the write)
     return o
 
 
@@ -340,6 +342,8 @@ def _check_out(out: Optional[torch.Tensor], q: torch.Tensor) -> None:
         return
     if out.shape != q.shape or out.dtype != q.dtype or out.device != q.device:
         raise ValueError("out must have q's shape, dtype and device")
+    if torch.is_grad_enabled() and out.requires_grad:
+        raise ValueError("out must not require a gradient")
     if any(n > 1 and st == 0 for n, st in zip(out.shape, out.stride())):
         raise ValueError("out must not be expanded")
     if _aligned(out) is not out:

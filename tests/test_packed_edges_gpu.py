@@ -101,3 +101,24 @@ def test_values_that_overflow_one_half_of_a_row(cuda, dim, col):
     grads = torch.autograd.grad(packed.packed_attention(*leaves, lay), leaves, d_o)
     for name, a, w, t in zip(("dq", "dk", "dv"), grads, w_g, t_g):
         _within(a, w, t, name)
+
+
+def test_a_write_to_out_is_noticed(cuda):
+    """out behaves as what torch writes in place: a graph that saved it refuses its backward pass afterwards, and one that
+    wants a gradient is refused."""
+    from ah_rag.packed import PackedLayout, packed_attention, prefix_attention
+    q, k, v = (_normal((9, 2, 16), 80 + i, BF, cuda) for i in range(3))
+    lay = PackedLayout([9], device=cuda)
+    for call in (lambda out: packed_attention(q, k, v, lay, out=out), lambda out: prefix_attention(q, k, v, k, v, lay, out=out)):
+        buf, leaf = torch.ones_like(q), torch.ones_like(q, requires_grad=True)
+        y = (leaf * buf).sum()
+        call(buf)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.backward()
+        with pytest.raises(ValueError, match="require a gradient"):
+            call(torch.ones_like(q, requires_grad=True))
+        with torch.no_grad():
+            own = torch.ones_like(q, requires_grad=True)
+            assert torch.equal(call(own), call(None))
+        with torch.inference_mode():
+            assert torch.equal(call(torch.ones_like(q)), call(None))
