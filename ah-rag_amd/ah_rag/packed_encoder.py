@@ -126,7 +126,10 @@ class PackedTransformer:
             if _get(cfg, "use_sliding_window", default=False) and _get(cfg, "sliding_window") is not None:
                 raise UnsupportedLayoutError("packed forward: sliding windows")
             rope = dict(_get(cfg, "rope_parameters", "rope_scaling", default={}) or {})
-            if rope.get("rope_type", rope.get("type", "default")) != "default" or float(rope.get("partial_rotary_factor", 1.0)) != 1.0:
+            if any(isinstance(v, dict) for v in rope.values()):
+                raise UnsupportedLayoutError("packed forward: rotary positions that differ from layer to layer")
+            if (rope.get("rope_type", rope.get("type", "default")) != "default"
+                    or float(rope.get("partial_rotary_factor", _get(cfg, "partial_rotary_factor", default=1.0))) != 1.0):
                 raise UnsupportedLayoutError("packed forward: scaled or partial rotary positions")
             self.theta = float(rope.get("rope_theta", _get(cfg, "rope_theta", default=10000.0)))
             self.act = self._activation(cfg.hidden_act)

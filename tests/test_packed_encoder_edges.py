@@ -253,6 +253,16 @@ def test_batches_without_tokens(monkeypatch, make, grad, ids):
     assert x.shape == (0, m.config.hidden_size)
 
 
+def test_rotary_settings_that_the_forward_does_not_have_are_refused():
+    from ah_rag.packed_encoder import PackedTransformer, UnsupportedLayoutError
+    m = causal()
+    m.config.rope_parameters = {"full_attention": {"rope_type": "default", "rope_theta": 1e4}}  # for each type of layer
+    for bad in (m, causal(partial_rotary_factor=0.5)):
+        with pytest.raises(UnsupportedLayoutError, match="rotary"):
+            PackedTransformer(bad, DEV)
+    PackedTransformer(causal(partial_rotary_factor=1.0), DEV)
+
+
 # ---- on the GPU --------------------------------------------------------------------------------
 
 
