@@ -178,13 +178,14 @@ class TorchEncoder:
         arr = out.cpu().numpy()
         return arr[0] if single else arr
 
-
     def embed(self, texts: Sequence[str], normalize_embeddings: bool = False) -> torch.Tensor:
         """Device float32 [n, d] of one packed batch with gradients to the model's parameters: the forward of a
         fine-tuning step (packed encoders). The caller enables the parameters' gradients and takes the loss
-        and the optimizer's step."""
+        and the optimizer's step. The packed forward has no dropout, whatever the model's config and mode say."""
         if self.packed is None:
             raise ValueError("embed() needs a packed encoder: TorchEncoder(..., packed=True)")
+        if isinstance(texts, str):
+            raise ValueError("embed() takes a list of texts")
         with torch.cuda.device(self.device):
             return self.packed.pooled(self.tokenizer(list(texts)), normalize_embeddings)
 

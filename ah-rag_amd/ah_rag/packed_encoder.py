@@ -10,7 +10,7 @@ two layer layouts) and runs them over the tokens of a batch lying behind each ot
 
 Projections, norms of whole rows and activations are torch / hipBLASLt calls; attention, the heads' norm
 with the rotation, and pooling are this library's kernels. Other layouts are refused when the object is
-made, never approximated.
+made, never approximated. Dropout is not applied, in training either.
 
 In a causal model the hidden states of a prefix do not depend on what follows, so tokens that all texts of
 a batch begin with (an instruction in front of every query) are run once, and the rest of each text reads

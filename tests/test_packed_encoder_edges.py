@@ -263,6 +263,15 @@ def test_rotary_settings_that_the_forward_does_not_have_are_refused():
     PackedTransformer(causal(partial_rotary_factor=1.0), DEV)
 
 
+def test_embed_of_one_string_is_refused():
+    """(It would be taken for a list of its letters.)"""
+    from ah_rag.encoder import TorchEncoder
+    enc = object.__new__(TorchEncoder)
+    enc.packed = object()
+    with pytest.raises(ValueError, match="list of texts"):
+        enc.embed("a river")
+
+
 # ---- on the GPU --------------------------------------------------------------------------------
 
 
