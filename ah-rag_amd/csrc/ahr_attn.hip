@@ -340,7 +340,8 @@ static int keys_of(const Seq& s, bool causal, int t, int n) {
 }
 
 // Row lists: a tile takes the rows of as many tokens of one sequence as fit. Where there are fewer
-// workgroups than fill the chip, key ranges are cut into pieces and joined; a shared prefix is read
+// workgroups than fill the chip, or some far longer than the others, key ranges are cut into pieces and joined; a shared
+// prefix is read
 // within each sequence's tiles or, where those are mostly empty, by tiles over all tokens, and joined.
 static void plan_rows(const std::vector<Seq>& seqs, const ahr_attn_shape& sh, int64_t prefix, bool may_split, Lists& L) {
   const int G = sh.heads / sh.kv_heads;
@@ -383,14 +384,17 @@ static void plan_rows(const std::vector<Seq>& seqs, const ahr_attn_shape& sh, in
   const int64_t ptl = apart ? across : 0;  // prefix row tiles
   work += ptl * ptiles;
   const int64_t blocks = ((int64_t)base.size() + ptl) * sh.kv_heads;
-  // Pieces of about `chunk` key tiles, at least four (256 keys). Tiles of one wave's rows stream their
-  // keys from memory and gain from many workgroups (24 sequences of one token over 1k-33k keys, 8 key heads
-  // of 128: 512 / 1024 / 2048 / 4096 pieces 295 / 279 / 258 / 278 us); fuller ones compute, and take one
-  // round of resident workgroups (200 tokens, 32/8 heads, prefix 16000: 256 / 512 / 1024 / 2048 110 / 93 /
-  // 100 / 120 us).
-  const int64_t want = !apart && waves <= tiles ? 2048 : 512;
+  // Pieces of about `chunk` key tiles, at least four (256 keys); an item of up to one and a half stays whole. Tiles of
+  // one wave's rows stream their keys from memory and gain from many workgroups (24 sequences of one token over 1k-33k
+  // keys, 8 key heads of 128: 512 / 1024 / 2048 / 4096 pieces 295 / 279 / 258 / 278 us); fuller ones compute, and take
+  // one round of resident workgroups (200 tokens, 32/8 heads, prefix 16000: 256 / 512 / 1024 / 2048 110 / 93 / 100 / 120
+  // us). Where there are 512 workgroups without it, only items far above their share are cut, so that none is left
+  // running alone (single tokens, 32/8 heads of 128: 64 sequences, one over 32768 keys and the others over 1000, 84 us,
+  // uncut 656; 1000, one over 100000 and the others over 300, 301 and 2016); even batches take no join (64 over 1000
+  // keys each 44 us, in 2048 pieces 49; 128 over 4000 355 and 367).
+  const int64_t want = !apart && blocks < 512 && waves <= tiles ? 2048 : 512;
   int64_t chunk = INT32_MAX;
-  if (may_split && (blocks < 512 || apart)) chunk = std::max<int64_t>(4, up(work * sh.kv_heads, want));
+  if (may_split) chunk = std::max<int64_t>(4, up(work * sh.kv_heads, want));
 
   int prefix_pieces = 0;
   if (apart) {

@@ -7,6 +7,8 @@ import numpy as np
 import pytest
 import torch
 
+from test_packed_cpu import _plan
+
 
 @pytest.mark.parametrize("path", [["."], ["ah-rag_amd"], [".", "ah-rag_amd"], ["ah-rag_amd", "."]], ids="+".join)
 def test_the_package_imports_from_the_repository_root(path):
@@ -66,3 +68,28 @@ def test_a_stream_of_another_device_is_refused():
     from ah_rag.packed import _on
     with pytest.raises(ValueError, match="a stream of cuda:1"):
         _on(SimpleNamespace(device=torch.device("cuda", 1)), torch.device("cuda", 0))
+
+
+def _tiles(row):
+    return -(-(row["pe"] - row["pb"]) // 64) + -(-(row["ke"] - row["kb"]) // 64)
+
+
+@pytest.mark.parametrize("n", [40, 63, 64, 65, 128, 300, 2000])
+@pytest.mark.parametrize("few,many,q", [(1000, 32768, 1), (300, 100000, 1), (1, 9000, 1), (500, 20000, 9)])
+@pytest.mark.parametrize("heads,kv_heads", [(32, 8), (12, 12), (8, 1)])
+def test_no_row_item_is_left_running_alone(n, few, many, q, heads, kv_heads):
+    """One sequence with many keys among others with few: its rows are cut into pieces of no more than one and a half times
+    what each of 512 resident workgroups has to do on average (or six tiles), however many sequences there are."""
+    kl = [few] * n
+    kl[n // 3] = many
+    plan, rows, _, join = _plan([q] * n, kl, heads=heads, kv_heads=kv_heads, dim=128, causal=1)
+    work = sum(map(_tiles, rows)) * kv_heads
+    assert max(map(_tiles, rows)) <= max(6, 1.5 * (work / 512 + 1))
+    if n * kv_heads >= 512:  # the others stay whole
+        assert len(join) <= 1
+
+
+@pytest.mark.parametrize("n,keys", [(64, 1000), (128, 4000), (512, 70), (1000, 10000)])
+def test_even_batches_take_no_join(n, keys):
+    plan, rows, _, join = _plan([1] * n, [keys] * n, heads=32, kv_heads=8, dim=128, causal=1)
+    assert not join and plan.ws_bytes == 0 and len(rows) == n

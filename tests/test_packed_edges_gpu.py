@@ -122,3 +122,17 @@ def test_a_write_to_out_is_noticed(cuda):
             assert torch.equal(call(own), call(None))
         with torch.inference_mode():
             assert torch.equal(call(torch.ones_like(q)), call(None))
+
+
+@pytest.mark.parametrize("q_len,few,many,dt,dim", [(1, 70, 6000, HF, 128), (1, 1, 3000, BF, 64), (3, 40, 4001, BF, 40)])
+def test_one_long_sequence_in_a_large_batch(cuda, q_len, few, many, dt, dim):
+    """More than 512 workgroups, one sequence's keys in pieces that are joined, the others whole."""
+    from ah_rag.packed import _CODES, PackedLayout, packed_attention
+    n, heads, hk = 80, 8, 8
+    ql, kl = [q_len] * n, [few] * n
+    kl[33] = many
+    q, k, v = (_normal((sum(x), h, dim), 90 + i, dt, cuda) for i, (x, h) in enumerate(((ql, heads), (kl, hk), (kl, hk))))
+    lay = PackedLayout(ql, kl, cuda)
+    plan = lay._plan(_CODES[dt], heads, hk, dim, True, False, 0)[0]
+    assert plan.n_rows * hk > 512 and plan.n_join == 1
+    _within(packed_attention(q, k, v, lay, causal=True), *ref.attention(q, k, v, ql, kl, True, dim ** -0.5), "o")
