@@ -91,7 +91,7 @@ class AttnPlan(ctypes.Structure):
     _fields_ = [("shape", AttnShape), ("tokens", ctypes.c_int64), ("key_tokens", ctypes.c_int64),
                 ("ints", ctypes.c_int64), ("ws_bytes", ctypes.c_int64), ("part_rows", ctypes.c_int64),
                 ("n_rows", ctypes.c_int32), ("n_keys", ctypes.c_int32), ("n_join", ctypes.c_int32),
-                ("join_tokens", ctypes.c_int32), ("planes", ctypes.c_int32), ("reserved", ctypes.c_int32)]
+                ("join_tokens", ctypes.c_int32), ("planes", ctypes.c_int32), ("far_rows", ctypes.c_int32)]
 
 
 class Tensor3(ctypes.Structure):

@@ -49,7 +49,7 @@ struct Params {
   // strides in elements
   int64_t q_ts, q_hs, k_ts, k_hs, v_ts, v_hs, pk_ts, pk_hs, pv_ts, pv_hs, o_ts, o_hs, do_ts, do_hs;
   int64_t dq_ts, dq_hs, dk_ts, dk_hs, dv_ts, dv_hs;
-  int64_t prows;
+  int64_t prows, far_rows, parts;  // partial rows of a plane, of the planes behind, of all planes
   const RowItem* rows;
   const KeyItem* keys;
   const JoinItem* join;

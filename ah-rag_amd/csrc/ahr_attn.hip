@@ -153,6 +153,12 @@ __device__ __forceinline__ void strict_row(FwdState<T, DP>& st, const Params& p,
   });
 }
 
+// Where a partial row lies: planes of the first prows rows one behind the other from the start, those of the far_rows
+// others from the end.
+__device__ __forceinline__ int64_t part_row(const Params& p, int plane, int row) {
+  return row < p.prows ? plane * p.prows + row : p.parts - (plane + 1) * p.far_rows + row - p.prows;
+}
+
 template <typename T, int DP>
 __device__ __forceinline__ void fwd_step(const char* __restrict__ cur, char* __restrict__ nxt, FwdState<T, DP>& st,
                                          const Stager<DP / 8, kWaves, kKeys>& stager, const Params& p, const RowItem& it, int hk, int t, int np,
@@ -246,7 +252,7 @@ __global__ __launch_bounds__(kWaves * 64, DP <= 64 ? 4 : 2) void attn_fwd_kernel
   const float inv = l == 0.f ? 0.f : 1.f / l;
   const float lse = l == 0.f ? -INFINITY : st.m + __log2f(l);
   if (it.plane >= 0) {
-    const int64_t at = ((int64_t)it.plane * p.prows + it.prow + tok) * p.heads + head;
+    const int64_t at = part_row(p, it.plane, it.prow + tok) * p.heads + head;
     if (h == 0) p.part_l[at] = lse;
     float* op = p.part_o + at * dim;
 #pragma unroll
@@ -282,7 +288,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(Params p, int lanes) {
   const int r = blockIdx.y * per + threadIdx.x / lanes, d = (threadIdx.x % lanes) * 4;
   if (r >= it.nq * p.heads || d >= p.dim) return;
   const int i = r / p.heads, head = r - i * p.heads;
-  const int64_t plane = p.prows * p.heads, at = (int64_t)(it.prow + i) * p.heads + head;
+  const int64_t plane = (it.prow < p.prows ? p.prows : -p.far_rows) * p.heads, at = part_row(p, 0, it.prow + i) * p.heads + head;
   const float* pl = p.part_l + at;
   const float* po = p.part_o + at * p.dim + d;
   float m = -INFINITY, sum = 0.f;
@@ -325,7 +331,8 @@ struct Lists {
   std::vector<KeyItem> keys;
   std::vector<JoinItem> join;
   int planes = 0, join_tokens = 0;
-  int64_t prows = 0;
+  int64_t prows = 0, far_rows = 0;  // partial rows of a plane, those behind the grid of the others among them
+  int64_t parts = 0;                // forward: partial rows of all planes
 };
 
 struct Seq {
@@ -363,9 +370,10 @@ static void plan_rows(const std::vector<Seq>& seqs, const ahr_attn_shape& sh, in
   const double join = 1000 + 2600 * std::min(1.0, (double)tiles * sh.kv_heads / 512) + (double)total * sh.heads * sh.head_dim / 1300;
   const bool apart = prefix > 0 && may_split && saved > join;
   std::vector<RowItem> base;
-  std::vector<int> load;
-  for (const Seq& s : seqs)
-    for (int t = 0; t < s.qlen; t += per) {
+  std::vector<int> load, seq_of;
+  for (size_t i = 0; i < seqs.size(); ++i)
+    for (int t = 0; t < seqs[i].qlen; t += per) {
+      const Seq& s = seqs[i];
       RowItem r;
       memset(&r, 0, sizeof r);
       r.q0 = (int32_t)(s.q0 + t);
@@ -377,6 +385,7 @@ static void plan_rows(const std::vector<Seq>& seqs, const ahr_attn_shape& sh, in
       r.pe = apart ? 0 : (int32_t)prefix;
       r.plane = -1;
       base.push_back(r);
+      seq_of.push_back((int)i);
       load.push_back((int)(up(r.ke, kKeys) + (apart ? 0 : ptiles)));
     }
   int64_t work = 0;
@@ -396,42 +405,75 @@ static void plan_rows(const std::vector<Seq>& seqs, const ahr_attn_shape& sh, in
   int64_t chunk = INT32_MAX;
   if (may_split) chunk = std::max<int64_t>(4, up(work * sh.kv_heads, want));
 
+  auto pieces_of = [&](int64_t tiles) { return tiles > chunk + chunk / 2 ? (int)up(tiles, chunk) : 1; };
+
+  // Apart, the partial rows are a grid: planes (the prefix's pieces, then own keys) by tokens. Few sequences whose own
+  // keys are cut would add their planes to every token (16000 single tokens, 8 heads of 128, prefix 2000, own keys 2 but
+  // for one sequence with 131072: 22 planes, 1.45 GB, 302 us), so from 256 MB on those read the prefix in their own
+  // tiles instead, and have a grid of their own behind the others' (132 MB, 306 us).
   int prefix_pieces = 0;
+  int64_t step = 0;  // keys of a piece of the prefix
   if (apart) {
-    prefix_pieces = (int)std::max<int64_t>(1, up(ptiles, chunk));
-    const int64_t step = up(ptiles, prefix_pieces) * kKeys;
+    step = up(ptiles, std::max<int64_t>(1, up(ptiles, chunk))) * kKeys;
     prefix_pieces = (int)up(prefix, step);
-    for (int64_t t = 0; t < total; t += per)
-      for (int i = 0; i < prefix_pieces; ++i) {
-        RowItem r;
-        memset(&r, 0, sizeof r);
-        r.q0 = (int32_t)t;
-        r.nq = (int32_t)std::min<int64_t>(per, total - t);
-        r.pb = (int32_t)(i * step);
-        r.pe = (int32_t)std::min<int64_t>(prefix, (i + 1) * step);
-        r.plane = i;
-        r.prow = (int32_t)t;
-        L.rows.push_back(r);
-      }
-    L.planes = prefix_pieces;
-    L.prows = total;
   }
+  std::vector<char> alone(seqs.size(), 0);
+  if (apart) {
+    int most = 1;
+    for (int x : load) most = std::max(most, pieces_of(x));
+    if (most > 1 && (prefix_pieces + most) * total * sh.heads * (sh.head_dim + 1) * 4 > (int64_t)256 << 20)
+      for (size_t b = 0; b < base.size(); ++b) alone[seq_of[b]] |= pieces_of(load[b]) > 1;
+  }
+  std::vector<int64_t> row0(seqs.size(), 0);  // apart: the first partial row of a sequence
+  int64_t near_rows = 0;
+  if (apart)
+    for (size_t i = 0; i < seqs.size();) {
+      if (alone[i]) {
+        ++i;
+        continue;
+      }
+      const int64_t t0 = seqs[i].q0, at = near_rows;
+      for (; i < seqs.size() && !alone[i]; ++i) {
+        row0[i] = near_rows;
+        near_rows += seqs[i].qlen;
+      }
+      const int64_t t1 = t0 + near_rows - at;
+      for (int64_t t = t0; t < t1; t += per)
+        for (int j = 0; j < prefix_pieces; ++j) {
+          RowItem r;
+          memset(&r, 0, sizeof r);
+          r.q0 = (int32_t)t;
+          r.nq = (int32_t)std::min<int64_t>(per, t1 - t);
+          r.pb = (int32_t)(j * step);
+          r.pe = (int32_t)std::min<int64_t>(prefix, (j + 1) * step);
+          r.plane = j;
+          r.prow = (int32_t)(at + t - t0);
+          L.rows.push_back(r);
+        }
+    }
+  L.prows = near_rows;
+  int near_planes = near_rows ? prefix_pieces : 0, far_planes = 0;
   for (size_t b = 0; b < base.size(); ++b) {
     RowItem r = base[b];
-    int pieces = load[b] > chunk + chunk / 2 ? (int)up(load[b], chunk) : 1;
-    if (pieces == 1 && !apart) {
+    const bool near = apart && !alone[seq_of[b]];
+    if (apart && !near) {
+      r.pe = (int32_t)prefix;
+      load[b] += (int)ptiles;
+    }
+    const int pieces = pieces_of(load[b]);
+    if (pieces == 1 && !near) {
       L.rows.push_back(r);
       continue;
     }
     // the key tiles of the item, prefix first, dealt to its pieces
-    const int64_t own0 = apart ? 0 : ptiles;
-    const int64_t step = up(load[b], pieces);
-    const int64_t prow = apart ? r.q0 : L.prows;
-    int made = prefix_pieces;
+    const int64_t own0 = near ? 0 : ptiles;
+    const int64_t len = up(load[b], pieces);
+    const int64_t prow = near ? row0[seq_of[b]] + r.q0 - seqs[seq_of[b]].q0 : L.prows;
+    int made = near ? prefix_pieces : 0;
     if (load[b] > 0)
-      for (int64_t t = 0; t < load[b]; t += step) {
+      for (int64_t t = 0; t < load[b]; t += len) {
         RowItem x = r;
-        const int64_t e = std::min<int64_t>(load[b], t + step);
+        const int64_t e = std::min<int64_t>(load[b], t + len);
         x.pb = (int32_t)std::min<int64_t>(r.pe, t * kKeys);
         x.pe = (int32_t)std::min<int64_t>(r.pe, e * kKeys);
         x.kb = (int32_t)std::min<int64_t>(r.ke, std::max<int64_t>(0, t - own0) * kKeys);
@@ -440,11 +482,16 @@ static void plan_rows(const std::vector<Seq>& seqs, const ahr_attn_shape& sh, in
         x.prow = (int32_t)prow;
         L.rows.push_back(x);
       }
-    L.planes = std::max(L.planes, made);
-    if (!apart) L.prows += r.nq;
+    int& planes = near || !apart ? near_planes : far_planes;
+    planes = std::max(planes, made);
+    if (!near) L.prows += r.nq;
     L.join.push_back(JoinItem{r.q0, r.nq, (int32_t)prow, made});
     L.join_tokens = std::max(L.join_tokens, r.nq);
   }
+  if (!apart) near_rows = L.prows;
+  L.far_rows = L.prows - near_rows;
+  L.parts = near_planes * near_rows + far_planes * L.far_rows;
+  L.planes = std::max(near_planes, far_planes);
   std::stable_sort(L.rows.begin(), L.rows.end(), [](const RowItem& a, const RowItem& b) {
     return (a.pe - a.pb) + (a.ke - a.kb) > (b.pe - b.pb) + (b.ke - b.kb);  // longest first
   });
@@ -539,10 +586,11 @@ static int build(const int32_t* q_len, const int32_t* k_len, int n, const ahr_at
   plan->join_tokens = L.join_tokens;
   plan->planes = L.planes;
   plan->part_rows = L.prows;
+  plan->far_rows = (int32_t)L.far_rows;
   plan->ints = (int64_t)(L.rows.size() * sizeof(RowItem) + L.keys.size() * sizeof(KeyItem) + L.join.size() * sizeof(JoinItem)) / 4;
   // forward: partial rows and their lse; backward: delta, partial dk and dv
   plan->ws_bytes = sh.backward ? up(t * sh.heads, 4) * 16 + (int64_t)L.planes * L.prows * sh.kv_heads * 2 * sh.head_dim * 4
-                               : (int64_t)L.planes * L.prows * sh.heads * (sh.head_dim + 1) * 4;
+                               : L.parts * sh.heads * (sh.head_dim + 1) * 4;
   if (!buf) return AHR_OK;
   if (cap < plan->ints) return fail(AHR_EINVAL, "buffer smaller than the plan's lists");
   char* b = reinterpret_cast<char*>(buf);
@@ -602,10 +650,12 @@ static int fill(const ahr_attn_args* a, bool backward, Params* out) {
     p.delta = (float*)a->ws;
     p.part_o = (float*)a->ws + up(pl.tokens * sh.heads, 4) * 4;
   } else {
-    p.part_o = (float*)a->ws;  // [planes][prows][heads][dim], then the lse of each
-    p.part_l = (float*)a->ws + (int64_t)pl.planes * pl.part_rows * sh.heads * sh.head_dim;
+    p.part_o = (float*)a->ws;  // [parts][heads][dim], then the lse of each
+    p.parts = pl.ws_bytes / ((int64_t)sh.heads * (sh.head_dim + 1) * 4);
+    p.part_l = (float*)a->ws + p.parts * sh.heads * sh.head_dim;
   }
-  p.prows = pl.part_rows;
+  p.prows = pl.part_rows - pl.far_rows;
+  p.far_rows = pl.far_rows;
   p.n_rows = pl.n_rows, p.n_keys = pl.n_keys, p.n_join = pl.n_join;
   p.rows = reinterpret_cast<const RowItem*>(a->lists);
   p.keys = reinterpret_cast<const KeyItem*>(p.rows + pl.n_rows);

@@ -383,7 +383,7 @@ typedef struct ahr_attn_plan {
   int64_t ints;                 /* int32 values of the lists */
   int64_t ws_bytes;             /* workspace of one call */
   int64_t part_rows;
-  int32_t n_rows, n_keys, n_join, join_tokens, planes, reserved;
+  int32_t n_rows, n_keys, n_join, join_tokens, planes, far_rows;
 } ahr_attn_plan;
 
 /* Host only. q_len / k_len: host int32 [n], >= 0 (k_len NULL: as q_len). buf NULL: fills *plan alone;

@@ -93,3 +93,62 @@ def test_no_row_item_is_left_running_alone(n, few, many, q, heads, kv_heads):
 def test_even_batches_take_no_join(n, keys):
     plan, rows, _, join = _plan([1] * n, [keys] * n, heads=32, kv_heads=8, dim=128, causal=1)
     assert not join and plan.ws_bytes == 0 and len(rows) == n
+
+
+def _part_address(plan, heads, dim, plane, row):
+    """Where a partial row lies among the plan's, as the kernels compute it."""
+    parts = plan.ws_bytes // (heads * (dim + 1) * 4)
+    near = plan.part_rows - plan.far_rows
+    at = plane * near + row if row < near else parts - (plane + 1) * plan.far_rows + row - near
+    assert 0 <= at < parts
+    return at
+
+
+@pytest.mark.parametrize("q_lens,k_lens,prefix,heads,kv_heads,dim,most", [
+    ([1] * 16000, [2] * 8000 + [131072] + [2] * 7999, 2000, 8, 1, 128, 300e6),   # 22 planes for all were 1.45 GB
+    ([1] * 4000, [1] * 3999 + [100000], 4000, 8, 1, 128, 150e6),                 # 40 planes, 660 MB
+    ([3] * 2000, [90000] + [3] * 1998 + [50000], 3000, 16, 2, 128, 600e6),       # at both ends, several tokens
+    ([2, 0, 1] * 3000, ([2, 0, 70000] + [2, 0, 1] * 999) * 3, 1000, 32, 8, 64, 700e6),
+    ([1] * 5000, [2] * 5000, 2000, 8, 1, 128, 200e6),                            # none is long: one grid
+    ([1] * 60, [3] * 50 + [9000] * 10, 5000, 16, 4, 64, 256e6),                  # long, but a small batch: one grid
+])
+def test_long_sequences_behind_a_prefix_keep_the_workspace_small(q_lens, k_lens, prefix, heads, kv_heads, dim, most):
+    """Every token reads each of its keys and of the prefix's once, no partial row belongs to two of them, and one long
+    sequence does not add its planes to every token of a large batch."""
+    plan, rows, _, join = _plan(q_lens, k_lens, heads=heads, kv_heads=kv_heads, dim=dim, causal=1, prefix=prefix)
+    T, seq_of = sum(q_lens), np.repeat(np.arange(len(q_lens)), q_lens)
+    first, k_first = np.cumsum(q_lens) - q_lens, np.cumsum(k_lens) - k_lens
+    pre, own, parts, final = ([[] for _ in range(T)] for _ in range(4))
+    for r in rows:
+        assert 0 < r["nq"] and r["nq"] * heads // kv_heads <= 128 and r["q0"] + r["nq"] <= T
+        for i in range(r["nq"]):
+            t = r["q0"] + i
+            s = seq_of[t]
+            if r["pe"] > r["pb"]:
+                pre[t].append((r["pb"], r["pe"]))
+            if r["ke"] > r["kb"]:
+                assert r["k0"] == k_first[s] and r["klen"] == k_lens[s] and r["koff"] + i == k_lens[s] - q_lens[s] + t - first[s]
+                own[t].append((r["kb"], r["ke"]))
+            (final if r["plane"] < 0 else parts)[t].append((r["plane"], r["prow"] + i))
+    used, joined = set(), {}
+    for q0, nq, prow, n in join:
+        for i in range(nq):
+            assert q0 + i not in joined
+            joined[q0 + i] = [(j, prow + i) for j in range(n)]
+            at = [_part_address(plan, heads, dim, j, prow + i) for j in range(n)]
+            near = plan.part_rows - plan.far_rows
+            step = near if prow < near else -plan.far_rows
+            assert all(b - a == step for a, b in zip(at, at[1:])) and not used.intersection(at)
+            used.update(at)
+    for t in range(T):
+        lim = k_lens[seq_of[t]] - q_lens[seq_of[t]] + t - first[seq_of[t]] + 1
+        for spans, stop in ((sorted(pre[t]), prefix), (sorted(own[t]), max(0, lim))):
+            end = 0
+            for a, b in spans:
+                assert a == end or a >= stop  # (a tile's later tokens read further: its pieces past `lim` are hidden)
+                end = b
+            assert end >= stop
+        assert (len(final[t]) == 1 and not parts[t] and t not in joined) or (not final[t] and sorted(parts[t]) == joined[t])
+    assert plan.ws_bytes <= most
+    work = sum(map(_tiles, rows)) * kv_heads
+    assert max(map(_tiles, rows)) <= max(6, 1.5 * (work / 512 + 1))

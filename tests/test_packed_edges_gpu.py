@@ -136,3 +136,28 @@ def test_one_long_sequence_in_a_large_batch(cuda, q_len, few, many, dt, dim):
     plan = lay._plan(_CODES[dt], heads, hk, dim, True, False, 0)[0]
     assert plan.n_rows * hk > 512 and plan.n_join == 1
     _within(packed_attention(q, k, v, lay, causal=True), *ref.attention(q, k, v, ql, kl, True, dim ** -0.5), "o")
+
+
+@pytest.mark.parametrize("dt,dim,heads,kv_heads", [(HF, 128, 8, 1), (BF, 64, 16, 2)])
+def test_long_sequences_in_a_large_batch_behind_a_prefix(cuda, dt, dim, heads, kv_heads):
+    """Most tokens read the prefix apart, the long sequences in their own tiles, with partial rows of their own."""
+    from ah_rag.packed import _CODES, PackedLayout, prefix_attention
+    n, prefix, long = 6000, 2000, {0: 40000, 3001: 70000}
+    ql = [1 + i % 2 for i in range(n)]
+    kl = [long.get(i, 2 + i % 3) for i in range(n)]
+    q, k, v, pk, pv = (_normal((m, h, dim), 100 + i, dt, cuda) for i, (m, h) in enumerate(
+        ((sum(ql), heads), (sum(kl), kv_heads), (sum(kl), kv_heads), (prefix, kv_heads), (prefix, kv_heads))))
+    lay = PackedLayout(ql, kl, cuda)
+    plan = lay._plan(_CODES[dt], heads, kv_heads, dim, True, False, prefix)[0]
+    assert plan.far_rows == sum(ql[i] for i in long) and plan.ws_bytes < 500e6
+    o = prefix_attention(q, k, v, pk, pv, lay)
+    q0, k0 = [0], [0]
+    for a, b in zip(ql, kl):
+        q0.append(q0[-1] + a)
+        k0.append(k0[-1] + b)
+    some = sorted({*long, 1, 2, 2999, 3000, 3002, 3003, n - 2, n - 1, *range(100, n, 371)})
+    qi = torch.cat([torch.arange(q0[i], q0[i + 1]) for i in some])
+    ki = torch.cat([torch.arange(k0[i], k0[i + 1]) for i in some])
+    want, tol = ref.attention(q.cpu()[qi], k.cpu()[ki], v.cpu()[ki], [ql[i] for i in some], [kl[i] for i in some], True, dim ** -0.5, pk, pv)
+    _within(o.cpu()[qi], want, tol, "o")
+    assert o.isfinite().all()
