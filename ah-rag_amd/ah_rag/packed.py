@@ -429,8 +429,11 @@ def _launch_rope(call, name, q, k, cos, sin, positions, eps, interleaved, wq, wk
                            0 if wk is None else wk.data_ptr(), cos.data_ptr(), sin.data_ptr(), positions.data_ptr(),
                            0 if dwq is None else dwq.data_ptr(), 0 if dwk is None else dwk.data_ptr(),
                            0 if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel())
-    if call(args, nat.stream_ptr(device_index=q.device.index)):
+    stream = nat.stream_ptr(device_index=q.device.index)
+    if call(args, stream):
         nat.check(-1, name)
+    if getattr(positions, "ahr_stream", None) is not None:  # a layout's own
+        _keep(positions, stream, q.device)
 
 
 @functools.lru_cache(maxsize=64)

@@ -161,3 +161,45 @@ def test_long_sequences_in_a_large_batch_behind_a_prefix(cuda, dt, dim, heads, k
     want, tol = ref.attention(q.cpu()[qi], k.cpu()[ki], v.cpu()[ki], [ql[i] for i in some], [kl[i] for i in some], True, dim ** -0.5, pk, pv)
     _within(o.cpu()[qi], want, tol, "o")
     assert o.isfinite().all()
+
+
+def test_positions_outlive_their_layout(cuda):
+    """A layout's positions read by a captured rotation, and by one that another stream still waits to run, after the layout
+    and they themselves have been dropped and their memory asked for again."""
+    from ah_rag.packed import PackedLayout, qk_norm_rope, rotary_table
+    n = 700
+    q, k = _normal((n, 4, 32), 110, BF, cuda), _normal((n, 2, 32), 111, BF, cuda)
+    cos, sin = rotary_table(n, 32, device=cuda)
+    want = qk_norm_rope(q, k, None, None, cos, sin, PackedLayout([n], device=cuda).positions())
+
+    def fill():
+        junk = [torch.full((n,), n + 5, dtype=torch.int32, device=cuda) for _ in range(200)]
+        torch.cuda.synchronize()
+        return junk
+
+    pos = PackedLayout([n], device=cuda).positions()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        got = qk_norm_rope(q, k, None, None, cos, sin, pos)
+    del pos
+    for _ in range(3):
+        junk = fill()
+        for x in got:
+            x.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        del junk
+    lay = PackedLayout([n], device=cuda)
+    lay.positions()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(1_000_000_000)  # (a finite wait on the device's clock)
+        got = qk_norm_rope(q, k, None, None, cos, sin, lay.positions())
+    at = lay.positions().data_ptr()
+    del lay
+    junk = [torch.full((n,), n + 5, dtype=torch.int32, device=cuda) for _ in range(200)]
+    assert not side.query() and at not in {x.data_ptr() for x in junk}
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
