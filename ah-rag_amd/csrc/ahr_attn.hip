@@ -574,8 +574,10 @@ static int build(const int32_t* q_len, const int32_t* k_len, int n, const ahr_at
   Lists L;
   plan_rows(seqs, sh, sh.backward ? 0 : sh.prefix, !sh.backward, L);
   if (sh.backward) plan_keys(seqs, sh, L);
-  const int64_t blocks = (int64_t)std::max(std::max(L.rows.size(), L.keys.size()) * (size_t)sh.kv_heads, L.join.size() * (size_t)sh.heads);
-  if (blocks > INT32_MAX / 2) return fail(AHR_EINVAL, "too many work items");
+  // a launch takes fewer than 2^32 threads in x and 2^16 workgroups in y (of the kernels that join or add partial results)
+  const int64_t blocks = std::max<int64_t>(std::max(L.rows.size(), L.keys.size()) * (size_t)sh.kv_heads, L.join.size());
+  const int64_t join_values = (int64_t)L.join_tokens * (sh.backward ? 2 * sh.kv_heads : sh.heads) * sh.head_dim;
+  if (blocks >= 1 << 24 || join_values >= 1 << 24) return fail(AHR_EUNSUP, "too many sequences or heads for one call");
   memset(plan, 0, sizeof *plan);
   plan->shape = sh;
   plan->tokens = t;
@@ -621,7 +623,7 @@ static int fill(const ahr_attn_args* a, bool backward, Params* out) {
   int st = check_shape(sh);
   if (st != AHR_OK) return st;
   if ((sh.backward != 0) != backward) return fail(AHR_EINVAL, backward ? "not a backward plan" : "not a forward plan");
-  if (!(a->scale > 0.f) || !std::isfinite(a->scale)) return fail(AHR_EINVAL, "scale must be positive and finite");
+  if (!(a->scale > 0.f) || !std::isfinite((float)((double)a->scale * 1.4426950408889634))) return fail(AHR_EINVAL, "scale must be positive and finite");
   if (pl.ints > 0 && !a->lists) return fail(AHR_EINVAL, "null plan lists");
   if (pl.ws_bytes > 0 && (!a->ws || a->ws_bytes < pl.ws_bytes || reinterpret_cast<uintptr_t>(a->ws) % 16)) return fail(AHR_EINVAL, "workspace smaller than the plan's ws_bytes, or not aligned");
   const struct { const ahr_tensor3* t; int64_t rows; int heads; const char* name; bool on; } all[] = {

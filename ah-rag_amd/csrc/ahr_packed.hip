@@ -616,6 +616,8 @@ static int pool_check(int dtype, int width, const int32_t* lists, int n_chunks, 
   if (dtype != AHR_F32 && dtype != AHR_F16 && dtype != AHR_BF16) return fail(AHR_EINVAL, "unknown dtype");
   if (width < 1 || width > (1 << 20)) return fail(AHR_EINVAL, "width out of range");
   if (n < 0 || n_chunks < 0 || (n > 0 && !lists) || reinterpret_cast<uintptr_t>(lists) % 16) return fail(AHR_EINVAL, "null or unaligned lists");
+  // a launch takes fewer than 2^32 threads: 1024 for a sequence, 256 for a chunk
+  if (n >= 1 << 22 || n_chunks >= 1 << 24) return fail(AHR_EUNSUP, "too many sequences for one call");
   return AHR_OK;
 }
 

@@ -152,3 +152,30 @@ def test_long_sequences_behind_a_prefix_keep_the_workspace_small(q_lens, k_lens,
     assert plan.ws_bytes <= most
     work = sum(map(_tiles, rows)) * kv_heads
     assert max(map(_tiles, rows)) <= max(6, 1.5 * (work / 512 + 1))
+
+
+def test_batches_past_a_launch_are_refused():
+    """More workgroups than a launch takes, or a scale whose base-2 form is no number: refused on the host."""
+    import ctypes
+
+    from ah_rag import _native as nat
+    lib = nat.lib()
+    n = (1 << 24) // 12 + 1
+    for backward in (0, 1):
+        with pytest.raises(nat.NativeLibraryError, match="too many"):
+            _plan([1] * n, backward=backward)
+    with pytest.raises(nat.NativeLibraryError, match="too many"):  # a prefix apart, whose join has more rows than a launch takes
+        _plan([40] * 30, heads=4000, kv_heads=2000, dim=128, prefix=5000)
+    many = np.ones(1 << 22, np.int32)
+    chunks = ctypes.c_int()
+    assert lib.ahr_pool_plan_build(many.ctypes.data, len(many), None, 0, ctypes.byref(chunks)) == nat.AHR_OK
+    for call in (lambda: lib.ahr_pool_mean(2, 4096, 8, 8, 4096, chunks.value, len(many), 0, 4096, None, 4096, 1 << 40, None),
+                 lambda: lib.ahr_pool_mean_backward(2, 4096, 8, 4096, chunks.value, len(many), 0, 4096, 4096, 4096, None)):
+        assert call() == nat.AHR_EUNSUP and b"too many" in lib.ahr_last_error()
+    plan, *_ = _plan([4, 2], heads=4, kv_heads=2)
+    a = nat.AttnArgs()
+    a.plan, a.lists = ctypes.pointer(plan), 4096
+    for t in (a.q, a.k, a.v, a.o):
+        t.p, t.ts, t.hs = 4096, 256, 64
+    a.scale = 2.9e38
+    assert lib.ahr_attn_forward(ctypes.byref(a), None) == nat.AHR_EINVAL and b"scale" in lib.ahr_last_error()
