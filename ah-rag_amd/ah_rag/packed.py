@@ -18,8 +18,8 @@ Everything runs in libahr_hip.so (include/ahr.h); there is no CPU fallback. Call
 current stream of the tensors' device (or `stream`), synchronise nothing and may be captured into a
 hipGraph once a layout has served a call of the same shape (its work lists are copied to the device
 then; a captured backward pass also needs leaves without a living graph from outside the capture, whose
-gradients torch accumulates on the stream of that graph). Tensors that the kernels cannot read in place (rows that do not start at multiples of 16
-bytes, a strided last dimension) are copied first.
+gradients torch accumulates on the stream of that graph). Tensors that the kernels cannot read in place
+(rows that do not start at multiples of 16 bytes, a strided last dimension) are copied first.
 
 Replaces, behind the reference's SentenceTransformer.encode seam
 (src/ah_rag/graph/hierarchical_graph.py:655-656, :709-712), that library's padded attention and
@@ -437,9 +437,10 @@ def _launch_rope(call, name, q, k, cos, sin, positions, eps, interleaved, wq, wk
 
 
 @functools.lru_cache(maxsize=64)
-def _rope_ws(tokens: int, dim: int) -> int:
+def _rope_ws(dim: int) -> int:
+    """Bytes of the backward pass's workspace (the same for any number of tokens)."""
     n = ctypes.c_int64()
-    nat.check(nat.lib().ahr_rope_ws_bytes(tokens, dim, ctypes.byref(n)), "ahr_rope_ws_bytes")
+    nat.check(nat.lib().ahr_rope_ws_bytes(0, dim, ctypes.byref(n)), "ahr_rope_ws_bytes")
     return n.value
 
 
@@ -475,7 +476,7 @@ class _QkNormRope(torch.autograd.Function):
         dq, dk = _new(q), _new(k)
         ws = gq = gk = None
         if wq is not None:
-            ws = q.new_empty(_rope_ws(q.shape[0], q.shape[2]), dtype=torch.uint8)
+            ws = q.new_empty(_rope_ws(q.shape[2]), dtype=torch.uint8)
             gq, gk = _new(wq), _new(wk)
         _launch_rope(_calls().rope_backward, "ahr_qk_norm_rope_backward", q, k, cos, sin, positions, ctx.eps, ctx.interleaved, wq, wk,
                      _unit(dyq), _unit(dyk), dq, dk, gq, gk, ws)

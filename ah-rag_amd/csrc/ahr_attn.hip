@@ -606,13 +606,12 @@ static int build(const int32_t* q_len, const int32_t* k_len, int n, const ahr_at
 
 // ---- host: argument checks and launches ------------------------------------------------------
 
-static int check_tensor(const ahr_tensor3& t, int64_t rows, int heads, int dim, const char* name) {
+static int check_tensor(const ahr_tensor3& t, int64_t rows, int heads, const char* name) {
   if (rows == 0) return AHR_OK;
   if (!t.p) return fail(AHR_EINVAL, std::string(name) + ": null tensor");
   if (reinterpret_cast<uintptr_t>(t.p) % 16 || t.ts % 8 || t.hs % 8) return fail(AHR_EINVAL, std::string(name) + ": rows must start at multiples of 16 bytes");
   // offsets within a staged tile: 24-bit token strides in bytes, 32 bits for its tokens and all heads
   if (t.ts < 0 || t.hs < 0 || t.ts >= (1 << 22) || t.hs > ((int64_t)1 << 29) / heads) return fail(AHR_EUNSUP, std::string(name) + ": stride too large");
-  (void)dim;
   return AHR_OK;
 }
 
@@ -633,7 +632,7 @@ static int fill(const ahr_attn_args* a, bool backward, Params* out) {
       {&a->d_o, pl.tokens, sh.heads, "d_o", backward},   {&a->dq, pl.tokens, sh.heads, "dq", backward},
       {&a->dk, pl.key_tokens, sh.kv_heads, "dk", backward}, {&a->dv, pl.key_tokens, sh.kv_heads, "dv", backward}};
   for (const auto& x : all)
-    if (x.on && (st = check_tensor(*x.t, x.rows, x.heads, sh.head_dim, x.name)) != AHR_OK) return st;
+    if (x.on && (st = check_tensor(*x.t, x.rows, x.heads, x.name)) != AHR_OK) return st;
   if (backward && pl.tokens > 0 && !a->lse) return fail(AHR_EINVAL, "null lse");
   Params p;
   memset(&p, 0, sizeof p);

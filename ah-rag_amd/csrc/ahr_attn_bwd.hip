@@ -283,12 +283,9 @@ __device__ __forceinline__ void key_loop(const Params& p, const KeyItem& it, int
       for (int x = 0; x < 4; ++x) {
         const int d = b * 32 + x * 8 + h * 4;
         if (DP != dim && d >= dim) continue;
-        
-          *reinterpret_cast<f32x4*>(out + d) =
-              f32x4{st.gk[b][4 * x], st.gk[b][4 * x + 1], st.gk[b][4 * x + 2], st.gk[b][4 * x + 3]} * k_out;
-        
-          *reinterpret_cast<f32x4*>(out + dim + d) =
-              f32x4{st.gv[b][4 * x], st.gv[b][4 * x + 1], st.gv[b][4 * x + 2], st.gv[b][4 * x + 3]} * v_out;
+        const f32x16 &a = st.gk[b], &e = st.gv[b];
+        *reinterpret_cast<f32x4*>(out + d) = f32x4{a[4 * x], a[4 * x + 1], a[4 * x + 2], a[4 * x + 3]} * k_out;
+        *reinterpret_cast<f32x4*>(out + dim + d) = f32x4{e[4 * x], e[4 * x + 1], e[4 * x + 2], e[4 * x + 3]} * v_out;
       }
     return;
   }
@@ -300,14 +297,9 @@ __device__ __forceinline__ void key_loop(const Params& p, const KeyItem& it, int
     for (int x = 0; x < 4; ++x) {
       const int d = b * 32 + x * 8 + h * 4;
       if (DP != dim && d >= dim) continue;
-      {
-        const f32x16& a = st.gk[b];
-        store4<T>(kp + d * 2, a[4 * x] * k_out, a[4 * x + 1] * k_out, a[4 * x + 2] * k_out, a[4 * x + 3] * k_out);
-      }
-      {
-        const f32x16& e = st.gv[b];
-        store4<T>(vp + d * 2, e[4 * x] * v_out, e[4 * x + 1] * v_out, e[4 * x + 2] * v_out, e[4 * x + 3] * v_out);
-      }
+      const f32x16 &a = st.gk[b], &e = st.gv[b];
+      store4<T>(kp + d * 2, a[4 * x] * k_out, a[4 * x + 1] * k_out, a[4 * x + 2] * k_out, a[4 * x + 3] * k_out);
+      store4<T>(vp + d * 2, e[4 * x] * v_out, e[4 * x + 1] * v_out, e[4 * x + 2] * v_out, e[4 * x + 3] * v_out);
     }
 }
 
