@@ -13,15 +13,17 @@
 // second operand of O^T = V^T P^T when V^T is read with its keys in accumulator order (col_frag). Keys
 // and values go through LDS by DMA, double buffered, one barrier per 64 keys.
 //
-// What bounds it. Many rows: the matrix units, whose products and the exponentials between them overlap only
-// across the two waves of a SIMD (4 causal sequences of 1.5k-8.2k tokens, 32/8 heads of 128, bf16: 1.06-1.12
-// ms, 1.0 PFLOP/s where a library product of 8192^3 reaches 1.18). Single tokens: memory (24 over 1k-33k keys
-// each, 8 key heads of 128, f16: 240 us and 7 for the join, 5.4 TB/s). Short texts lie between (256 of up to
-// 384 tokens, 12 heads of 64: 73 us, 3.3 TB/s). Few workgroups (64 queries of 4-40 tokens behind a prefix of
-// 700, 16/8 heads of 64: 23 us) wait out each tile's chain of barrier, products, exponentials, products. Three
-// tile buffers instead of two (1.45 ms for the long sequences, no change for the prefix), two waves that share a
-// tile's keys where an item has few rows (6 % less for the prefix, but 2 % more for the long ones) and an order of the
-// workgroups that spreads key heads over the XCDs (1.16 ms) were measured and not kept.
+// What bounds it (kernel times in calls one after the other on the same inputs). Many rows: the matrix units, whose
+// products and the exponentials between them overlap only across the two waves of a SIMD (4 causal sequences of
+// 1.5k-8.2k tokens, 32/8 heads of 128, bf16: 1.12 ms, 0.99 PFLOP/s where a library product of 8192^3 reaches 1.18; up to
+// 1.30 ms where each call follows a pause). Single tokens: memory (24 over 1k-33k keys each, 8 key heads of 128, f16: 236
+// us and 7 for the join, 5.5 TB/s). Short texts lie between (256 of up to 384 tokens, 12 heads of 64: 73 to 87 us from
+// one card to the next, 2.8 to 3.3 TB/s). Few workgroups (64 queries of 4-40 tokens behind a prefix of 900, 16/8 heads of
+// 64: 19 us and 5 for the join) wait out each tile's chain of barrier, products, exponentials, products, at most five in
+// a row; that chain, the start and the partial rows' way through memory were not told apart. Measured and not kept, each
+// against the form of its time: three tile buffers instead of two (a third slower for the long sequences, no change for
+// the prefix), two waves that share a tile's keys where an item has few rows (6 % less for the prefix, but 2 % more for
+// the long ones) and an order of the workgroups that spreads key heads over the XCDs (10 % more).
 #include "ahr_attn_common.h"
 
 #include <algorithm>
@@ -182,7 +184,8 @@ __device__ __forceinline__ void fwd_step(const char* __restrict__ cur, char* __r
 }
 
 // (Up to 64 wide: 128 registers, four waves a SIMD. 256 texts of up to 384 tokens, 12 heads of 64: 73 us, 79
-// with the 162 registers that the compiler takes when left alone.)
+// with the 162 registers that the compiler takes when left alone. 20 bytes a lane are put aside for it, before the loop
+// over the tiles, and read back after it.)
 template <typename T, int DP>
 __global__ __launch_bounds__(kWaves * 64, DP <= 64 ? 4 : 2) void attn_fwd_kernel(Params p) {
   constexpr int DB = DP / 32;
@@ -520,8 +523,8 @@ static void plan_keys(const std::vector<Seq>& seqs, const ahr_attn_shape& sh, Li
       work += tiles_of(k.t1 - k.t0);
     }
   const int64_t slots = sh.head_dim > 64 ? 256 : 512;  // resident workgroups
-  // (5.8k causal tokens in 3 sequences, 16/4 heads of 128: two thirds of a slot's share 438 us for the whole
-  // step, a whole share 474, half 470, two shares 605)
+  // (5.8k causal tokens in 3 sequences, 16/4 heads of 128: two thirds of a slot's share 457 us for the whole
+  // step, a whole share 493, half 493, two shares 612, in one run)
   const int64_t piece = std::max<int64_t>(16, up(work * sh.kv_heads * 2, slots * 3));
   for (const KeyItem& k : base) {
     const int64_t tiles = tiles_of(k.t1 - k.t0);

@@ -8,13 +8,13 @@
 // needs five, but nothing is added through memory: no atomics, no fp32 copy of dq, the same bits
 // every time.
 //
-// What bounds it: 3 causal sequences of 0.7k-4.1k tokens, 16/4 heads of 128, bf16: dq 155 us (three products,
-// 0.73 PFLOP/s), dk and dv 235 us (four, 0.64), the sums of cut key tiles 11. The dk/dv kernel holds 128
-// accumulators and 64 registers of keys and values a lane, so one wave a SIMD, which issues products (38 % of its
-// time) and the vector instructions between them in turn; its pieces fill 256 slots to 0.8. 64 texts of up to 384
-// tokens, 12 heads of 64: dq 31 us, dk and dv 40. Measured and not kept: the exponentials of one half of a tile
-// issued between the products of the other (228 us; 43 for the texts), accumulators in ordinary registers
-// (about 290), eight waves with the products' roles split between them.
+// What bounds it (kernel times in calls one after the other): 3 causal sequences of 0.7k-4.1k tokens, 16/4 heads of 128,
+// bf16: dq 145 us (three products, 0.78 PFLOP/s), dk and dv 200 us (four, 0.75), the sums of cut key tiles 10. The dk/dv
+// kernel holds 128 accumulators and 64 registers of keys and values a lane, so one wave a SIMD, which issues products (38 %
+// of its time) and the vector instructions between them in turn; its pieces fill 256 slots to 0.8. 64 texts of up to 384
+// tokens, 12 heads of 64: dq 30 us, dk and dv 39. Measured and not kept (of dk and dv, then at 235 us): the exponentials of
+// one half of a tile issued between the products of the other (228 us; 43 for the texts), accumulators in ordinary
+// registers (about 290), eight waves with the products' roles split between them.
 #include "ahr_attn_common.h"
 
 namespace ahr {
