@@ -359,8 +359,9 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, layout: 
     multiple of kv_heads (query head i reads key head i * kv_heads // heads); head_dim a multiple of 8 up
     to 128; any strides. scale: default head_dim ** -0.5. causal: query i of a sequence with n queries
     and m keys reads the keys j <= i + m - n (the last query reads all). A row that reads no key gives
-    zeros, and zero gradients. Scores, sums and accumulators are fp32; the weights p are rounded to the
-    tensors' type for the product with v, and o once at the end.
+    zeros, and zero gradients; one whose scores are all minus infinity NaN. Scores, sums and accumulators are
+    fp32; the weights p are rounded to the tensors' type for the product with v, and o once at the end. The
+    gradients use a row's log-sum in fp32, whose rounding shows in them where scaled scores pass 2^14.
 
     Differentiable in q, k and v (no atomics: repeated runs give the same bits). `out`, where no gradient
     is wanted: written in place of a new tensor; it must not overlap the inputs. `stream`: runs there,

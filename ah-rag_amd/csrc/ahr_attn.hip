@@ -35,6 +35,10 @@ namespace ahr {
 namespace attn {
 
 constexpr float kRaise = 8.f;  // how far (log2) a score may exceed the reference before it is raised
+// The exponent c s - m is one rounding of the exact value, while m itself is rounded: past 2^24 the largest weight is off
+// by a power of two, which l shares, but which passes f16's range from 2^27 on and fp32's from 2^31.
+constexpr float kFar = 0x1p26f;
+constexpr float kNone = -3.4028234663852886e38f;  // log-sum of a piece whose keys' scores are all minus infinity
 
 // What a wave carries from tile to tile: its 32 rows' queries, and one row for each lane (the other
 // half-lane the same row, other keys).
@@ -110,7 +114,8 @@ __device__ __forceinline__ void fwd_tile(const char* __restrict__ cur, FwdState<
 
 // The row of this lane again, in plain steps: where a product of zero weights with a value that is not finite
 // reached an accumulator (a tile's matrix product multiplies every row's weight, also the zero of a key that
-// the row does not read, with every value), or where inputs that the row does read are not finite.
+// the row does not read, with every value), where inputs that the row does read are not finite, or where its scores
+// are too large for weights relative to a rounded reference (the largest score is subtracted before the scale).
 template <typename T, int DP>
 __device__ __forceinline__ void strict_row(FwdState<T, DP>& st, const Params& p, const RowItem& it, int hk, int head, int tok, int lim, int h) {
   typedef typename Elem<T>::v8 v8;
@@ -131,16 +136,16 @@ __device__ __forceinline__ void strict_row(FwdState<T, DP>& st, const Params& p,
       f(p.k + ((int64_t)(it.k0 + j) * p.k_ts + hk * p.k_hs) * 2, p.v + ((int64_t)(it.k0 + j) * p.v_ts + hk * p.v_hs) * 2);
   };
   float m = -INFINITY;
-  each([&](const char* k, const char*) { m = fmaxf(m, score(k) * p.scale_log2); });
+  each([&](const char* k, const char*) { m = fmaxf(m, score(k)); });
   const float ref = m == -INFINITY ? 0.f : m;
-  st.m = m;
+  st.m = m == -INFINITY ? m : fminf(fmaxf(m * p.scale_log2, 0.5f * kNone), -0.5f * kNone);
   st.l = 0.f;
 #pragma unroll
   for (int b = 0; b < DP / 32; ++b)
 #pragma unroll
     for (int r = 0; r < 16; ++r) st.acc[b][r] = 0.f;
   each([&](const char* k, const char* v) {
-    const float w = ex2(fmaf(score(k), p.scale_log2, -ref));
+    const float w = ex2((score(k) - ref) * p.scale_log2);
     if (h == 0) st.l += w;
 #pragma unroll
     for (int b = 0; b < DP / 32; ++b)
@@ -242,7 +247,8 @@ __global__ __launch_bounds__(kWaves * 64, DP <= 64 ? 4 : 2) void attn_fwd_kernel
     for (int b = 0; b < DB; ++b)
 #pragma unroll
       for (int r = 0; r < 16; ++r) x[r & 3] = fmaf(st.acc[b][r], 0.f, x[r & 3]);
-    const bool odd = live && !(fabsf((x[0] + x[1]) + (x[2] + x[3])) < INFINITY);
+    const bool far = st.m > -INFINITY && !(fabsf(st.m) < kFar);
+    const bool odd = live && (far || !(fabsf((x[0] + x[1]) + (x[2] + x[3])) < INFINITY));
     if (__any(odd)) {
       // Both halves of a row take the strict path where either has to: they share its weights and its sum. (The
       // exchange runs in every lane: a lane that a branch has switched off hands over nothing.)
@@ -252,8 +258,11 @@ __global__ __launch_bounds__(kWaves * 64, DP <= 64 ? 4 : 2) void attn_fwd_kernel
   }
   if (!live) return;
   const float l = st.l + other_half(st.l);
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-  const float lse = l == 0.f ? -INFINITY : st.m + __log2f(l);
+  // Without a weight: a row that reads no key here, or keys whose scores are all minus infinity. The first gives zeros, the
+  // second has no softmax; in a piece it only adds nothing.
+  const bool none = l == 0.f && (it.pe > it.pb || min(it.ke, lim) > it.kb);
+  const float inv = l == 0.f ? (none && it.plane < 0 ? NAN : 0.f) : 1.f / l;
+  const float lse = l == 0.f ? (none && it.plane >= 0 ? kNone : -INFINITY) : st.m + __log2f(l);
   if (it.plane >= 0) {
     const int64_t at = part_row(p, it.plane, it.prow + tok) * p.heads + head;
     if (h == 0) p.part_l[at] = lse;
@@ -320,8 +329,8 @@ __global__ __launch_bounds__(256) void attn_join_kernel(Params p, int lanes) {
     }
     m = to;
   }
-  const float inv = sum == 0.f ? 0.f : 1.f / sum;
-  if (p.lse && d == 0) p.lse[(int64_t)(it.q0 + i) * p.heads + head] = sum == 0.f ? -INFINITY : m + __log2f(sum);
+  const float inv = sum == 0.f ? 0.f : m == kNone ? NAN : 1.f / sum;
+  if (p.lse && d == 0) p.lse[(int64_t)(it.q0 + i) * p.heads + head] = sum == 0.f || m == kNone ? -INFINITY : m + __log2f(sum);
   store4<T>(p.o + ((int64_t)(it.q0 + i) * p.o_ts + (int64_t)head * p.o_hs + d) * 2, a[0] * inv, a[1] * inv, a[2] * inv, a[3] * inv);
 }
 

@@ -203,3 +203,61 @@ def test_positions_outlive_their_layout(cuda):
     assert not side.query() and at not in {x.data_ptr() for x in junk}
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def _bounds(dt):
+    return {BF: 1e17, HF: 6e4}[dt]
+
+
+@pytest.mark.parametrize("dt,dim", [(BF, 64), (BF, 128), (BF, 40), (HF, 32), (HF, 96)])
+def test_scores_of_any_size(cuda, dt, dim):
+    """Scores far beyond what fp32 tells apart by one (2^24): the largest takes the whole weight, whatever its size and sign."""
+    from ah_rag.packed import PackedLayout, packed_attention, prefix_attention
+    size = _bounds(dt)
+    for sign in (1.0, -1.0):
+        for case, (ql, kl, heads, hk, prefix) in enumerate((([70, 1], [200, 150], 4, 2, 0), ([2], [3000], 8, 2, 0), ([3] * 40, [3] * 40, 8, 4, 1300))):
+            g = torch.Generator().manual_seed(120 + case)
+            q = torch.zeros(sum(ql), heads, dim)
+            q[..., :5] = size * (1 + torch.rand(sum(ql), heads, 5, generator=g)) * sign / 2
+            k = torch.zeros(sum(kl) + prefix, hk, dim)
+            k[..., :5] = size * (1 + torch.rand(sum(kl) + prefix, hk, 5, generator=g)) / 2
+            q, k = q.to(dt).to(cuda), k.to(dt).to(cuda)
+            v = _normal((sum(kl) + prefix, hk, dim), 130, dt, cuda)
+            lay = PackedLayout(ql, kl, cuda)
+            pk, pv, k, v = k[:prefix], v[:prefix], k[prefix:], v[prefix:]
+            o = prefix_attention(q, k, v, pk, pv, lay, causal=False) if prefix else packed_attention(q, k, v, lay)
+            qd, kd, vd, pkd, pvd = (x.cpu().double() for x in (q, k, v, pk, pv))
+            q0 = k0 = 0
+            for a, b in zip(ql, kl):
+                for h in range(heads):
+                    K, V = torch.cat((pkd[:, h * hk // heads], kd[k0:k0 + b, h * hk // heads])), torch.cat((pvd[:, h * hk // heads], vd[k0:k0 + b, h * hk // heads]))
+                    s = qd[q0:q0 + a, h] @ K.T
+                    top = s.topk(2, 1).values
+                    # (rows whose best two are told apart by more than the fp32 sums may be off)
+                    clear = (top[:, 0] - top[:, 1]) * dim ** -0.5 > 8 * 2.0 ** -24 * s.abs().amax(1) * dim ** -0.5 + 200
+                    want = V[s.argmax(1)]
+                    assert torch.equal(o[q0:q0 + a, h].cpu().double()[clear], want[clear]) and clear.any()
+                q0, k0 = q0 + a, k0 + b
+
+
+@pytest.mark.parametrize("dt,dim", [(BF, 64), (HF, 96)])
+def test_rows_whose_scores_are_all_minus_infinity(cuda, dt, dim):
+    """They have no softmax (NaN, as the definition gives); rows that read no key give zeros; others are untouched."""
+    from ah_rag.packed import PackedLayout, packed_attention, prefix_attention
+    scale = dim ** -0.5
+    for ql, kl, heads, hk in (([5, 3, 2], [5, 0, 130], 4, 2), ([2, 1], [2000, 700], 8, 2)):
+        q, k, v = (_normal((n, h, dim), 140 + i, dt, cuda) for i, (n, h) in enumerate(((sum(ql), heads), (sum(kl), hk), (sum(kl), hk))))
+        q[..., 0] = q[..., 0].abs() + 0.1
+        first = 5 if len(ql) == 3 else 2000
+        k[:first, 1, 0] = -math.inf  # every key of the first sequence, for half the heads
+        lay = PackedLayout(ql, kl, cuda)
+        o = packed_attention(q, k, v, lay).cpu()
+        want, tol = ref.attention(q[:, :heads // 2], k[:, :1], v[:, :1], ql, kl, False, scale)
+        _within(o[:, :heads // 2], want, tol, "heads without")
+        assert o[:ql[0], heads // 2:].isnan().all() and o[ql[0]:].isfinite().all()
+        if len(ql) == 3:
+            assert not o[5:8].any()
+        one = k[:1].clone()  # a prefix of one key that is read: its value alone
+        one[:, :, 0] = 0.0
+        p = prefix_attention(q, k, v, one, v[:1].clone(), lay, causal=False).cpu()
+        assert torch.equal(p[:ql[0], heads // 2:], v[:1, 1:].cpu().expand(ql[0], heads // 2, dim))
