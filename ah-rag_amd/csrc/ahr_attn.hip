@@ -15,7 +15,7 @@
 //
 // What bounds it (kernel times in calls one after the other on the same inputs). Many rows: the matrix units, whose
 // products and the exponentials between them overlap only across the two waves of a SIMD (4 causal sequences of
-// 1.5k-8.2k tokens, 32/8 heads of 128, bf16: 1.12 ms, 0.99 PFLOP/s where a library product of 8192^3 reaches 1.18; up to
+// 1.5k-8.2k tokens, 32/8 heads of 128, bf16: 1.09-1.12 ms, 1.0 PFLOP/s where a library product of 8192^3 reaches 1.18; up to
 // 1.30 ms where each call follows a pause). Single tokens: memory (24 over 1k-33k keys each, 8 key heads of 128, f16: 236
 // us and 7 for the join, 5.5 TB/s). Short texts lie between (256 of up to 384 tokens, 12 heads of 64: 73 to 87 us from
 // one card to the next, 2.8 to 3.3 TB/s). Few workgroups (64 queries of 4-40 tokens behind a prefix of 900, 16/8 heads of

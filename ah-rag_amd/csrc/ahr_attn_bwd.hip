@@ -9,10 +9,10 @@
 // every time.
 //
 // What bounds it (kernel times in calls one after the other): 3 causal sequences of 0.7k-4.1k tokens, 16/4 heads of 128,
-// bf16: dq 145 us (three products, 0.78 PFLOP/s), dk and dv 200 us (four, 0.75), the sums of cut key tiles 10. The dk/dv
+// bf16: dq 143 us (three products, 0.79 PFLOP/s), dk and dv 200 us (four, 0.75), the sums of cut key tiles 11. The dk/dv
 // kernel holds 128 accumulators and 64 registers of keys and values a lane, so one wave a SIMD, which issues products (38 %
 // of its time) and the vector instructions between them in turn; its pieces fill 256 slots to 0.8. 64 texts of up to 384
-// tokens, 12 heads of 64: dq 30 us, dk and dv 39. Measured and not kept (of dk and dv, then at 235 us): the exponentials of
+// tokens, 12 heads of 64: dq 30 us, dk and dv 41. Measured and not kept (of dk and dv, then at 235 us): the exponentials of
 // one half of a tile issued between the products of the other (228 us; 43 for the texts), accumulators in ordinary
 // registers (about 290), eight waves with the products' roles split between them.
 #include "ahr_attn_common.h"
