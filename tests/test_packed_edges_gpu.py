@@ -261,3 +261,31 @@ def test_rows_whose_scores_are_all_minus_infinity(cuda, dt, dim):
         one[:, :, 0] = 0.0
         p = prefix_attention(q, k, v, one, v[:1].clone(), lay, causal=False).cpu()
         assert torch.equal(p[:ql[0], heads // 2:], v[:1, 1:].cpu().expand(ql[0], heads // 2, dim))
+
+
+@pytest.mark.parametrize("dim,dt", [(32, BF), (64, HF), (96, BF), (128, HF)])
+@pytest.mark.parametrize("col", [0, 4, -1])
+def test_log_sums_and_gradients_beside_a_bad_column(cuda, dim, dt, col):
+    """The log-sums that the backward pass reads are those of the rows' keys, whatever one column of a value holds, and the
+    gradients of the other sequence keep their bits."""
+    from ah_rag import packed
+    scale, lens = dim ** -0.5, [100, 30]
+    q, k, v, d_o = (_normal((130, h, dim), 150 + i, dt, cuda) for i, h in enumerate((4, 2, 2, 4)))
+    bad = v.clone()
+    bad[37, 1, col] = math.nan
+    lay = packed.PackedLayout(lens, device=cuda)
+    lse = torch.empty(130, 4, device=cuda)
+    packed._attention(q, k, bad, lay, True, scale, lse)
+    for h in range(4):
+        for a, b in ((0, 100), (100, 130)):
+            s = scale * (q[a:b, h].double() @ k[a:b, h // 2].double().T)
+            s = s.masked_fill(torch.ones_like(s, dtype=torch.bool).triu(1), -math.inf)
+            # scores in fp32 ((dim + 4) half steps of sum |q k|), the logarithm and the sum a few half steps of 16
+            off = ((q[a:b, h].double().abs() @ k[a:b, h // 2].double().abs().T).amax(1) * scale * (dim + 4) + 16 * 8) * 2.0 ** -24 * 1.5
+            assert ((lse[a:b, h].double() - torch.logsumexp(s, 1) / math.log(2)).abs() <= off).all()
+    grads = []
+    for x in (v, bad):
+        leaves = [t.detach().requires_grad_() for t in (q, k, x)]
+        grads.append(torch.autograd.grad(packed.packed_attention(*leaves, lay, causal=True), leaves, d_o))
+    for a, b in zip(*grads):
+        assert torch.equal(a[100:], b[100:]) and a.isfinite().all()
