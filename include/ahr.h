@@ -399,7 +399,7 @@ typedef struct ahr_tensor3 {  /* [tokens][heads][head_dim] */
 typedef struct ahr_attn_args {
   const ahr_attn_plan* plan;  /* host */
   const int32_t* lists;       /* device: the plan's lists */
-  float scale;                /* > 0 */
+  float scale;                /* > 0; scale log2(e) finite */
   int32_t reserved;
   ahr_tensor3 q, k, v;        /* q [tokens][heads], k and v [key_tokens][kv_heads] */
   ahr_tensor3 prefix_k, prefix_v; /* [prefix][kv_heads], or null with prefix 0 */
@@ -413,8 +413,8 @@ typedef struct ahr_attn_args {
   int64_t ws_bytes;
 } ahr_attn_args;
 
-/* o = softmax(scale q k^T) v within each sequence. A row that reads no key gives zeros. Allocates
- * nothing and synchronises nothing: capturable. */
+/* o = softmax(scale q k^T) v within each sequence. A row that reads no key gives zeros, one whose scores
+ * are all minus infinity NaN. Allocates nothing and synchronises nothing: capturable. */
 int ahr_attn_forward(const ahr_attn_args* a, void* stream);
 /* dq, dk, dv from d_o, with o and lse of the forward pass. No atomics: the same inputs give the same
  * bits. Gradients of a key head are summed over its query heads in fp32. */
