@@ -385,9 +385,11 @@ __device__ __forceinline__ void row_tile(const char* __restrict__ cur, RowState<
   }
 }
 
-// delta = sum_j p_j (do . v_j) of this lane's row, whose keys all lie in one staged tile. Equal to sum_d do o but
+// delta = sum_j p_j (do . v_j) of this lane's row, whose keys all lie in the first staged tile. Equal to sum_d do o but
 // for o's rounding to 16 bits, which with few keys is as large as that of ds (in units of dq, bf16, against
-// 0.0024 with an exact delta: 0.0030 for 4 keys a row, 0.0025 for 16, 0.0024 from 64 on, where it no longer counts).
+// 0.0024 with an exact delta: 0.0030 for 4 keys a row, 0.0025 for 16, 0.0024 from 64 on, where it hardly counts). So too
+// the early rows of a causal sequence whose row tile reads on (31 texts of up to 1154 tokens, 12 heads of 32: dq 0.00255
+// off with o's delta for them, 0.00241 so).
 template <typename T, int DP>
 __device__ __forceinline__ float row_delta(const char* __restrict__ cur, const RowState<T, DP>& st, int mine, float c, int lane) {
   constexpr int NC = DP / 8, KS = DP / 16;
@@ -475,9 +477,11 @@ __global__ __launch_bounds__(kWaves * 64, 2) void attn_dq_kernel(Params p) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) x = fmaf((float)ov[ks][i], (float)st.of[ks][i], x);
     st.delta = x + other_half(x);
-    if (nt == 1) {
+    // where the rows of the workgroup's first wave, which read the fewest keys, have them in the first tile
+    const int few = p.causal ? min(it.klen, it.koff + (((min(32, n_rows) - 1) * p.group_inv) >> 16) + 1) : it.klen;
+    if (nt > 0 && few <= kKeys) {
       tile_barrier();
-      if (wave_live) st.delta = row_delta<T, DP>(smem, st, min(lim, it.ke), p.scale_log2, lane);
+      if (wave_live && lim_hi <= kKeys) st.delta = row_delta<T, DP>(smem, st, min(lim, it.ke), p.scale_log2, lane);
     }
     if (live && h == 0) p.delta[li] = st.delta;
   }

@@ -289,3 +289,36 @@ def test_log_sums_and_gradients_beside_a_bad_column(cuda, dim, dt, col):
         grads.append(torch.autograd.grad(packed.packed_attention(*leaves, lay, causal=True), leaves, d_o))
     for a, b in zip(*grads):
         assert torch.equal(a[100:], b[100:]) and a.isfinite().all()
+
+
+@pytest.mark.parametrize("dt", [BF, HF])
+@pytest.mark.parametrize("lens,kls", [([300], None), ([130, 64, 65], None), ([200], [150]), ([100], [130])])
+def test_early_rows_of_long_causal_sequences_keep_the_small_gradients(cuda, dt, lens, kls):
+    """Rows that read at most one tile's keys, 128 of them in a tile of rows whose last ones read more: their delta is exact
+    too. Bounds as where all rows of a sequence read one tile: with u half a step of the type, ds_j is off by u |ds_j| +
+    2^-16 p_j (|dp_j| + sum_i p_i |dp_i|), and dq by the sum of these times |k_j| and its own rounding."""
+    from ah_rag.packed import PackedLayout, packed_attention
+    h, d = 4, 64
+    kls = kls or lens
+    q, do = (_normal((sum(lens), h, d), 160 + i, dt, cuda) for i in range(2))
+    k, v = (_normal((sum(kls), h, d), 162 + i, dt, cuda) for i in range(2))
+    leaf = q.clone().requires_grad_()
+    packed_attention(leaf, k, v, PackedLayout(lens, kls, cuda), scale=1.0, causal=True).backward(do)
+    u = torch.finfo(dt).eps / 2
+    q0 = k0 = 0
+    for n, m in zip(lens, kls):
+        # the rows of whole waves (32 rows) whose last one reads at most 64 keys
+        rows = max(0, (min(n, 64 - (m - n)) // 32) * 32)
+        Q, D = (x[q0:q0 + rows].transpose(0, 1).cpu().double() for x in (q, do))
+        K, V = (x[k0:k0 + m].transpose(0, 1).cpu().double() for x in (k, v))
+        s = Q @ K.transpose(1, 2)
+        assert rows == 0 or float(s.abs().max()) * 1.4427 < 128
+        see = ref.visible(n, m, True)[:rows]
+        p = torch.softmax(s.masked_fill(~see, -math.inf), 2).nan_to_num(0.0)
+        dp = D @ V.transpose(1, 2)
+        ds = p * (dp - (p * dp).sum(2, keepdim=True))
+        off = u * ds.abs() + 2.0 ** -16 * p * (dp.abs() + (p * dp.abs()).sum(2, keepdim=True))
+        want = (ds @ K).transpose(0, 1)
+        _within(leaf.grad[q0:q0 + rows], want, (off @ K.abs()).transpose(0, 1) * 1.01 + u * want.abs() + 1e-7, "dq of %d over %d" % (n, m))
+        q0, k0 = q0 + n, k0 + m
+    assert leaf.grad.isfinite().all()
